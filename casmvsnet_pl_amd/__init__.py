@@ -7,6 +7,7 @@ mirrors the reference's `models/mvsnet.py` / `models/modules.py` API.
 from .inplace_abn import ABN, InPlaceABN
 from .modules import ConvBnReLU, ConvBnReLU3D, depth_regression, get_depth_values, homo_warp
 from .mvsnet import CascadeMVSNet, CostRegNet, FeatureNet
+from .norm import LayerNormAct
 
 __all__ = ["ABN", "InPlaceABN", "ConvBnReLU", "ConvBnReLU3D", "depth_regression", "get_depth_values",
-           "homo_warp", "CascadeMVSNet", "CostRegNet", "FeatureNet"]
+           "homo_warp", "CascadeMVSNet", "CostRegNet", "FeatureNet", "LayerNormAct"]

@@ -17,6 +17,8 @@ ABI_VERSION = 6
 CONV_S1, CONV_S2, CONV_T2 = 0, 1, 2
 CONV2D_K3, CONV2D_K5S2, CONV2D_K1, CONV2D_K1_UP = 3, 4, 5, 6
 
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+
 # every symbol include/casmvs.h declares: name -> (restype, argtypes)
 _FP = c_void_p  # device / host float* passed as integer addresses
 SYMBOLS = {
@@ -134,6 +136,18 @@ SYMBOLS = {
     "casmvs_costvol_var_backward_f32": (c_int, [_FP] * 5 + [c_void_p] + [c_int] * 6 + [c_void_p]),
     "casmvs_costvol_gwc_backward_f32": (c_int, [_FP] * 5 + [c_void_p] + [c_int] * 7 + [c_void_p]),
     "casmvs_normalize_images_u8": (c_int, [_FP, _FP, c_int, c_int, c_int, POINTER(c_float), POINTER(c_float), c_void_p]),
+    "casmvs_layer_norm_forward": (c_int, [c_void_p, _FP, _FP, c_void_p, c_int, c_size_t, c_int, c_size_t, c_float, c_float, c_void_p]),
+    "casmvs_layer_norm_backward_workspace_bytes": (c_size_t, [c_int, c_size_t, c_int, c_size_t]),
+    "casmvs_layer_norm_backward": (c_int, [c_void_p, c_void_p, _FP, _FP, c_void_p, _FP, _FP, c_void_p, c_int, c_size_t, c_int, c_size_t, c_float, c_float, c_void_p]),
+    "casmvs_pack8": (c_int, [c_void_p, c_int, c_size_t, c_size_t, c_void_p, c_void_p, c_void_p]),
+    "casmvs_unpack8": (c_int, [c_void_p, c_void_p, _FP, _FP, c_int, c_float, c_void_p, c_int, c_size_t, c_size_t, c_void_p]),
+    "casmvs_abn8_train_apply_f32": (c_int, [_FP, _FP, c_int, c_double, _FP, _FP, c_float, c_float, c_float] + [_FP] * 4 + [c_void_p] * 3 + [c_int, c_int, c_size_t, c_float, c_void_p]),
+    "casmvs_abn8_backward_sums_blocks": (c_int, [c_int, c_size_t]),
+    "casmvs_abn8_backward_sums_f64": (c_int, [_FP] + [c_void_p] * 3 + [_FP, c_int, c_int, c_size_t, c_float, c_void_p]),
+    "casmvs_abn8_backward_apply_f32": (c_int, [_FP] + [c_void_p] * 3 + [_FP, c_int, c_double, _FP, c_float] + [_FP] * 4 + [c_int, c_int, c_size_t, c_float, c_void_p]),
+    "casmvs_depth_ce_workspace_bytes": (c_size_t, [c_int, c_int, c_size_t]),
+    "casmvs_depth_ce_forward": (c_int, [c_void_p] + [_FP] * 2 + [c_void_p] + [_FP] * 4 + [c_void_p, c_int, c_int, c_int, c_size_t, c_int, c_void_p]),
+    "casmvs_depth_ce_backward": (c_int, [c_void_p] + [_FP] * 4 + [c_void_p, c_int, c_int, c_int, c_size_t, c_void_p]),
     "casmvs_selftest_mfma": (c_int, [_FP]),
     "casmvs_selftest_mfma_rate": (c_int, [c_int, c_int, c_int, POINTER(c_float)]),
 }

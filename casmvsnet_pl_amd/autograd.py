@@ -11,6 +11,13 @@ convolution gradients:
 
 A variance / correlation cost volume built from `homo_warp` outputs with torch's elementwise ops (the reference's own
 training-mode code, mvsnet.py:150-153) is therefore differentiable end to end down to the feature maps.
+
+Two more that a training step uses and the reference does not have:
+
+  layer_norm(x, weight, bias, eps, slope, channels_last)     normalisation per position over the channels + leaky ReLU, in the place of
+      batch statistics (norm.LayerNormAct is the module); gradients w.r.t. x, weight and bias.
+  depth_cross_entropy(cost, depth_values, depth_gt, mask)    the depth as a classification over the hypotheses, the other loss beside
+      SmoothL1 on softmax_depth_regression; gradient w.r.t. the cost volume.
 """
 import ctypes
 
@@ -86,3 +93,81 @@ def softmax_depth_regression(cost, depth_values):
     if not cost.is_cuda:
         raise RuntimeError("casmvsnet_pl_amd.autograd.softmax_depth_regression runs on the MI355X only; there is no CPU fallback")
     return _SoftmaxDepthRegression.apply(cost, depth_values)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, slope, channels_last):
+        x = x.contiguous()
+        ctx.save_for_backward(x, weight, bias)
+        ctx.args = eps, slope, channels_last
+        return ops.layer_norm(x, weight, bias, eps, slope, channels_last)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, weight, bias = ctx.saved_tensors
+        gx, gw, gb = ops.layer_norm_backward(x, gy, weight, bias, *ctx.args, need_x=ctx.needs_input_grad[0],
+                                             need_affine=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        return gx, (gw if ctx.needs_input_grad[1] else None), (gb if ctx.needs_input_grad[2] else None), None, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, slope=1.0, channels_last=False):
+    """Differentiable ops.layer_norm: x (N,C,*spatial) or (..,C) with channels_last, float32 / float16 / bfloat16; weight, bias (C,) float32 or None.
+    What it keeps for the backward pass is x."""
+    if not x.is_cuda:
+        raise RuntimeError("casmvsnet_pl_amd.autograd.layer_norm runs on the MI355X only; there is no CPU fallback")
+    return _LayerNorm.apply(x, weight, bias, float(eps), float(slope), bool(channels_last))
+
+
+class _DepthCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, cost, depth_values, depth_gt, mask):
+        cost = ops._float_dev(cost, "cost")
+        if cost.dim() != 4:
+            raise ValueError(f"depth_cross_entropy: cost {tuple(cost.shape)}, expected (B,D,h,w)")
+        B, D, h, w = cost.shape
+        depth_values, depth_gt = (ops._same_device(cost, ops._dev(t, name), name) for t, name in ((depth_values, "depth_values"), (depth_gt, "depth_gt")))
+        if tuple(depth_values.shape) not in ((B, D, h, w), (B, D)) or tuple(depth_gt.shape) != (B, h, w):
+            raise ValueError(f"depth_cross_entropy: cost {tuple(cost.shape)}, depth_values {tuple(depth_values.shape)}, depth_gt {tuple(depth_gt.shape)}")
+        if mask is not None:
+            if mask.dtype != torch.bool or tuple(mask.shape) != (B, h, w):
+                raise ValueError(f"depth_cross_entropy: mask {tuple(mask.shape)} {mask.dtype}, expected a bool ({B}, {h}, {w})")
+            mask = ops._same_device(cost, mask, "mask").contiguous()
+        if B * D == 0:
+            raise ValueError(f"depth_cross_entropy: cost {tuple(cost.shape)} has no hypotheses")
+        lib, code = _lib.load(), ops._DTYPES[cost.dtype]
+        loss = torch.empty((), dtype=torch.float32, device=cost.device)
+        # per pixel the running maximum and 1 / sum; behind them 1 / count
+        stats = torch.empty(2 * B * h * w + 1, dtype=torch.float32, device=cost.device)
+        target = torch.empty((B, h, w), dtype=torch.int32, device=cost.device)
+        ws = torch.empty(lib.casmvs_depth_ce_workspace_bytes(B, D, h * w), dtype=torch.uint8, device=cost.device)
+        with torch.cuda.device(cost.device):
+            rc = lib.casmvs_depth_ce_forward(_ptr(cost), _ptr(depth_values), _ptr(depth_gt), None if mask is None else _ptr(mask), _ptr(stats), _ptr(target),
+                                             _ptr(loss), _ptr(stats[-1:]), _ptr(ws), code, B, D, h * w, int(depth_values.dim() == 4), _stream(cost))
+        _lib.check(rc, "casmvs_depth_ce_forward")
+        ctx.save_for_backward(cost, stats, target)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gloss):
+        cost, stats, target = ctx.saved_tensors
+        B, D, h, w = cost.shape
+        gloss = gloss.contiguous().float()
+        gcost = torch.empty_like(cost)
+        with torch.cuda.device(cost.device):
+            rc = _lib.load().casmvs_depth_ce_backward(_ptr(cost), _ptr(stats), _ptr(target), _ptr(stats[-1:]), _ptr(gloss), _ptr(gcost), ops._DTYPES[cost.dtype],
+                                                      B, D, h * w, _stream(cost))
+        _lib.check(rc, "casmvs_depth_ce_backward")
+        return gcost, None, None, None
+
+
+def depth_cross_entropy(cost, depth_values, depth_gt, mask=None):
+    """Softmax cross entropy over the depth hypotheses, the mean over the pixels that count (a float32 scalar): cost (B,D,h,w) float32 / float16 / bfloat16,
+    depth_values (B,D,h,w) or (B,D) and depth_gt (B,h,w) float32 (finite), mask (B,h,w) bool or None.  The class of a pixel is the hypothesis nearest to
+    depth_gt, the lowest index on ties; a pixel counts if its mask is set and depth_gt lies inside the range of its hypotheses (and not all of its costs are -inf).
+    Where no pixel counts the loss and its gradient are 0.  Gradient with respect to cost only."""
+    if not cost.is_cuda:
+        raise RuntimeError("casmvsnet_pl_amd.autograd.depth_cross_entropy runs on the MI355X only; there is no CPU fallback")
+    return _DepthCrossEntropy.apply(cost, depth_values, depth_gt, mask)

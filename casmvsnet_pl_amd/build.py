@@ -14,8 +14,8 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_ROOT = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libcasmvs_hip.so")
-SOURCES = ["abi.hip", "costvol.hip", "costvol_lds.hip", "depth_ops.hip", "fusion.hip", "backward.hip", "train.hip", "prob_wgrad.hip", "prob_regress.hip", "conv11_prob_zfused.hip", "fpn_fused.hip", "fpn_fused_sf.hip", "conv0_splitbf16.hip", "conv0_splitf16.hip", "conv0_zmarch.hip", "deconv11_splitf16.hip", "deconv9_splitf16.hip", "conv_ci_splitf16.hip", "conv_s2_splitf16.hip", "conv2d_ci_splitf16.hip", "conv2d_k5s2_splitf16.hip", "fnet_conv0_mm.hip", "debug_disturb.hip", "conv3d_mfma.hip"]
-HEADERS = [os.path.join(CSRC, h) for h in ("common.h", "plane_sweep.h", "buffer_ops.h", "softmax_regress.h", "split_f16.h", "fixed_accum.h")] + [os.path.join(REPO_ROOT, "include", "casmvs.h")]
+SOURCES = ["abi.hip", "costvol.hip", "costvol_lds.hip", "depth_ops.hip", "fusion.hip", "backward.hip", "train.hip", "prob_wgrad.hip", "prob_regress.hip", "conv11_prob_zfused.hip", "fpn_fused.hip", "fpn_fused_sf.hip", "conv0_splitbf16.hip", "conv0_splitf16.hip", "conv0_zmarch.hip", "deconv11_splitf16.hip", "deconv9_splitf16.hip", "conv_ci_splitf16.hip", "conv_s2_splitf16.hip", "conv2d_ci_splitf16.hip", "conv2d_k5s2_splitf16.hip", "fnet_conv0_mm.hip", "layer_norm.hip", "checkpoint8.hip", "depth_ce.hip", "debug_disturb.hip", "conv3d_mfma.hip"]
+HEADERS = [os.path.join(CSRC, h) for h in ("common.h", "plane_sweep.h", "buffer_ops.h", "softmax_regress.h", "split_f16.h", "fixed_accum.h", "elem_types.h", "block8.h")] + [os.path.join(REPO_ROOT, "include", "casmvs.h")]
 
 
 def _sources():
@@ -29,6 +29,10 @@ IO_HEADERS = [os.path.join(REPO_ROOT, "include", "casmvs_io.h")]
 IO_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-shared", "-pthread", "-Wall", "-Wextra"]
 
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC"]
+# sources compiled without packed float32 instructions altogether: nothing in them gains from those, and then there is none to rewrite
+# (the host pass does not know the feature and says so)
+UNPACKED_SOURCES = ("layer_norm.hip", "checkpoint8.hip", "depth_ce.hip")
+UNPACKED_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # (+ -DCASMVS_PACKED_OPSEL_SAFE=1 on every source: _compile_source rewrites the device assembly, and casmvs_packed_opsel_safe() says so)
 
 
@@ -101,7 +105,8 @@ def _compile_source(hipcc, flags, inc, src, obj, verbose=False):
             raise RuntimeError(f"build step failed on {src}:\n{' '.join(cmd)}\n{res.stdout}")
 
     flags = list(flags) + ["-DCASMVS_PACKED_OPSEL_SAFE=1"]
-    run([hipcc] + flags + inc + ["--cuda-device-only", "-S", src, "-o", stem + ".s"])
+    unpacked = UNPACKED_FLAGS if os.path.basename(src) in UNPACKED_SOURCES else []
+    run([hipcc] + flags + unpacked + inc + ["--cuda-device-only", "-S", src, "-o", stem + ".s"])
     with open(stem + ".s") as f:
         text, count = rewrite_unsafe_packed(f.read())
     with open(stem + ".fixed.s", "w") as f:
@@ -119,7 +124,7 @@ def source_sha16():
     compiler flags): equal hashes = the same kernels, whichever machine linked the .so (hipcc's output is not bit-reproducible across
     builds, so the binary's own hash cannot say that).  Stamps the PMC files and the bench line (bench.py: traffic_source.same_library)."""
     import hashlib
-    h = hashlib.sha256(" ".join(FLAGS).encode())
+    h = hashlib.sha256(" ".join(FLAGS + UNPACKED_FLAGS).encode())
     for path in sorted(_sources() + HEADERS):
         h.update(os.path.basename(path).encode())
         with open(path, "rb") as f:

@@ -1,0 +1,384 @@
+// 8-bit activation checkpoints (block8.h has the format): packing and reading back on their own, and the train-mode ABN that keeps, for its backward pass,
+// 8 bits of the normalised input and one bit for the side of zero instead of its float32 input and output.
+//
+//   forward    xhat = (x - mean_c) rstd_c,  z = gamma_c xhat + beta_c,  y = z > 0 ? z : slope z;  kept: Q = 8 bits of xhat, s = [z > 0]
+//   backward   g = gy (s ? 1 : slope),  gbeta = sum g,  ggamma = sum g Q,  gx = gamma rstd (g - gbeta / M - Q ggamma / M)
+//
+// xhat enters the gradient through ggamma and its product with Q only (both averages over the channel), so its 8 bits cost little there; the side of zero
+// multiplies every gradient element, so it is kept exactly.  xhat and z are computed in 64 bits from the 64-bit statistics: a block's codes and the sign of z
+// are the ones of the definition, not of one order of float32 roundings.  y itself is the float32 fma of casmvs_abn_train_apply_f32, bit for bit, so
+// choosing the 8-bit checkpoint leaves a forward pass as it was.
+//
+// Everything here waits for memory: forward 4 + 4 + 33/32 + 1/8 bytes per element, backward sums 4 + 37/32, apply 8 + 37/32 (keeping x and y in
+// float32 reads 12 and 12 and writes 4).
+#include "block8.h"
+
+namespace {
+using casmvs::block8::kBlock;
+using casmvs::block8::kLanes;
+using casmvs::elem::Vec;
+
+constexpr int kThreads = 256;
+constexpr size_t kMostElements = (size_t)1 << 40;
+constexpr int kGroups = kThreads / kLanes;   // blocks of 32 values that a workgroup works on at a time
+
+// Four elements from `p` on, `left` of them real (0 .. 4); a missing one reads 0.
+template <class T, bool WIDE>
+__device__ __forceinline__ void load4(const T *p, int left, float (&v)[4]) {
+  if (WIDE) {
+    if (left > 0) {   // (planes of 4 n elements: all four or none)
+      const Vec<T, 4> t = casmvs::elem::load<T, 4>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (float)t.v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < left ? (float)p[i] : 0.0f;
+  }
+}
+template <class T, bool WIDE>
+__device__ __forceinline__ void store4(T *p, int left, const float (&v)[4]) {
+  if (WIDE) {
+    if (left > 0) {
+      Vec<T, 4> t;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t.v[i] = (T)v[i];
+      casmvs::elem::store<T, 4>(p, t);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) p[i] = (T)v[i];
+  }
+}
+__device__ __forceinline__ int left_of(size_t n, size_t first) { return first >= n ? 0 : n - first < 4 ? (int)(n - first) : 4; }
+
+// ---- pack / unpack ------------------------------------------------------------------------------------------------------------------------------------
+template <class T, bool WIDE>
+__global__ __launch_bounds__(kThreads) void pack8_kernel(const T *__restrict__ x, unsigned *__restrict__ codes, unsigned char *__restrict__ scales, size_t rows,
+                                                        size_t n, size_t nb) {
+  const size_t total = rows * nb;
+  const int lane = threadIdx.x & (kLanes - 1);
+  // every lane of a wave takes the same number of turns (the exchanges inside a block need its eight lanes); a turn past the end works on nothing
+  const size_t turns = (total + (size_t)gridDim.x * kGroups - 1) / ((size_t)gridDim.x * kGroups);
+  for (size_t turn = 0; turn < turns; ++turn) {
+    const size_t blk = (turn * gridDim.x + blockIdx.x) * kGroups + threadIdx.x / kLanes;
+    const bool live = blk < total;
+    const size_t row = live ? blk / nb : 0, first = (live ? blk % nb : 0) * kBlock + 4 * lane;
+    float v[4];
+    load4<T, WIDE>(x + row * n + first, live ? left_of(n, first) : 0, v);
+    const double d[4] = {v[0], v[1], v[2], v[3]};
+    unsigned scale;
+    const unsigned q = casmvs::block8::quantise(d, scale);
+    if (live) {
+      codes[blk * kLanes + lane] = q;
+      if (lane == 0) scales[blk] = (unsigned char)scale;
+    }
+  }
+}
+
+// out = the held value, or (AFFINE) act(value * weight[c] + bias[c]) with c = row % C: an ABN's output from what its backward pass keeps
+template <class T, bool WIDE, bool AFFINE>
+__global__ __launch_bounds__(kThreads) void unpack8_kernel(const unsigned *__restrict__ codes, const unsigned char *__restrict__ scales, T *__restrict__ out,
+                                                          const float *__restrict__ weight, const float *__restrict__ bias, int C, float slope, size_t rows,
+                                                          size_t n, size_t nb) {
+  const size_t total = rows * nb, step_blocks = (size_t)gridDim.x * kGroups;
+  const int lane = threadIdx.x & (kLanes - 1);
+  for (size_t blk = (size_t)blockIdx.x * kGroups + threadIdx.x / kLanes; blk < total; blk += step_blocks) {
+    const size_t row = blk / nb, first = (blk % nb) * kBlock + 4 * lane;
+    const float step = casmvs::block8::step_of(scales[blk]);
+    const unsigned q = codes[blk * kLanes + lane];
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = casmvs::block8::value_of(q, i, step);
+    if (AFFINE) {
+      const float w = weight[row % C], b = bias[row % C];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float z = fmaf(v[i], w, b);
+        v[i] = z > 0.0f ? z : z * slope;
+      }
+    }
+    store4<T, WIDE>(out + row * n + first, left_of(n, first), v);
+  }
+}
+
+// ---- train-mode ABN -------------------------------------------------------------------------------------------------------------------------------------
+// The channel's two totals from the partial sums (C, blocks, 2), in every workgroup: one value per thread and a fixed-order tree.
+__device__ __forceinline__ void channel_totals(const double *__restrict__ sums, int blocks, int c, double &t0, double &t1) {
+  __shared__ double red[2][kThreads];
+  double s0 = 0.0, s1 = 0.0;
+  for (int b = threadIdx.x; b < blocks; b += kThreads) {
+    s0 += sums[((size_t)c * blocks + b) * 2];
+    s1 += sums[((size_t)c * blocks + b) * 2 + 1];
+  }
+  red[0][threadIdx.x] = s0;
+  red[1][threadIdx.x] = s1;
+  __syncthreads();
+  for (int st = kThreads / 2; st > 0; st >>= 1) {
+    if ((int)threadIdx.x < st) {
+      red[0][threadIdx.x] += red[0][threadIdx.x + st];
+      red[1][threadIdx.x] += red[1][threadIdx.x + st];
+    }
+    __syncthreads();
+  }
+  t0 = red[0][0];
+  t1 = red[1][0];
+}
+
+constexpr int kTurns = 8;   // blocks per group of eight lanes and workgroup: 256 x 32 = 8192 elements share one read of the channel's partial sums
+
+// blockIdx.x = (plane, chunk of kTurns * kGroups blocks); vec (4, C): scale = gamma rstd, shift, gamma, beta of the forward pass
+template <bool WIDE>
+__global__ __launch_bounds__(kThreads) void abn8_apply_kernel(const float *__restrict__ x, const double *__restrict__ sums, int blocks, double M,
+                                                             const float *__restrict__ weight, const float *__restrict__ bias, float abs_eps, float eps,
+                                                             float momentum, float *__restrict__ rmean, float *__restrict__ rvar, float *__restrict__ vec,
+                                                             float *__restrict__ y, unsigned *__restrict__ codes, unsigned char *__restrict__ scales,
+                                                             unsigned *__restrict__ signs, int C, size_t n, size_t nb, unsigned chunks, float slope) {
+  const size_t plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const int c = (int)(plane % C);
+  double s0, s1;
+  channel_totals(sums, blocks, c, s0, s1);
+  const double mu = s0 / M;
+  double var = s1 / M - mu * mu;   // biased
+  var = var > 0.0 ? var : 0.0;
+  const double rs = 1.0 / sqrt(var + (double)eps);
+  const float gamma = abs_eps >= 0.0f ? fabsf(weight[c]) + abs_eps : weight[c], beta = bias[c];
+  const float a = (float)((double)gamma * rs), bq = (float)((double)beta - mu * (double)gamma * rs);
+  if (chunk == 0 && plane == (size_t)c && threadIdx.x == 0) {
+    vec[c] = a;
+    vec[C + c] = bq;
+    vec[2 * C + c] = gamma;
+    vec[3 * C + c] = beta;
+    if (rmean) {   // F.batch_norm: running = (1 - momentum) * running + momentum * batch (running_var: unbiased)
+      const float keep = (float)(1.0 - (double)momentum);
+      rmean[c] = rmean[c] * keep + momentum * (float)mu;
+      rvar[c] = rvar[c] * keep + momentum * (float)(var * (M / (M > 1.0 ? M - 1.0 : 1.0)));
+    }
+  }
+  const int lane = threadIdx.x & (kLanes - 1);
+  const float *xp = x + plane * n;
+  float *yp = y + plane * n;
+#pragma unroll 2
+  for (int turn = 0; turn < kTurns; ++turn) {
+    const size_t blk = (chunk * kTurns + turn) * kGroups + threadIdx.x / kLanes, first = blk * kBlock + 4 * lane;
+    const int left = left_of(n, first);   // 0 past the plane's last block
+    float v[4], o[4];
+    load4<float, WIDE>(xp + first, left, v);
+    double h[4];
+    unsigned up = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[i] = i < left ? ((double)v[i] - mu) * rs : 0.0;
+      up |= (h[i] * (double)gamma + (double)beta > 0.0 ? 1u : 0u) << i;
+      const float t = fmaf(v[i], a, bq);
+      o[i] = t > 0.0f ? t : t * slope;
+    }
+    unsigned scale;
+    const unsigned q = casmvs::block8::quantise(h, scale);
+    const unsigned sign = casmvs::block8::over_block(up << (4 * lane), [](unsigned p, unsigned r) { return p | r; });
+    store4<float, WIDE>(yp + first, left, o);
+    if (blk < nb) {
+      codes[(plane * nb + blk) * kLanes + lane] = q;
+      if (lane == 0) {
+        scales[plane * nb + blk] = (unsigned char)scale;
+        signs[plane * nb + blk] = sign;
+      }
+    }
+  }
+}
+
+// out (C, blocks, 2): this workgroup's part of sum g and sum g Q of channel blockIdx.y; blockIdx.x owns the blocks [lo, hi) of every plane of the channel
+template <bool WIDE>
+__global__ __launch_bounds__(kThreads) void abn8_backward_sums_kernel(const float *__restrict__ gy, const unsigned *__restrict__ codes,
+                                                                     const unsigned char *__restrict__ scales, const unsigned *__restrict__ signs,
+                                                                     double *__restrict__ out, int N, int C, size_t n, size_t nb, float slope) {
+  const int c = blockIdx.y, lane = threadIdx.x & (kLanes - 1);
+  const size_t per = (nb + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < nb ? lo + per : nb;
+  double s0 = 0.0, s1 = 0.0;
+  for (int img = 0; img < N; ++img) {
+    const size_t plane = (size_t)img * C + c;
+    for (size_t blk = lo + threadIdx.x / kLanes; blk < hi; blk += kGroups) {
+      const size_t first = blk * kBlock + 4 * lane, at = plane * nb + blk;
+      float v[4];
+      load4<float, WIDE>(gy + plane * n + first, left_of(n, first), v);
+      const unsigned q = codes[at * kLanes + lane], up = signs[at] >> (4 * lane);
+      const float step = casmvs::block8::step_of(scales[at]);
+      float p0 = 0.0f, p1 = 0.0f;   // four values in float32, then 64 bits
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float g = v[i] * ((up >> i) & 1u ? 1.0f : slope);
+        p0 += g;
+        p1 = fmaf(g, casmvs::block8::value_of(q, i, step), p1);
+      }
+      s0 += p0;
+      s1 += p1;
+    }
+  }
+  __shared__ double red[2][kThreads];
+  red[0][threadIdx.x] = s0;
+  red[1][threadIdx.x] = s1;
+  __syncthreads();
+  for (int st = kThreads / 2; st > 0; st >>= 1) {
+    if ((int)threadIdx.x < st) {
+      red[0][threadIdx.x] += red[0][threadIdx.x + st];
+      red[1][threadIdx.x] += red[1][threadIdx.x + st];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    out[((size_t)c * gridDim.x + blockIdx.x) * 2] = red[0][0];
+    out[((size_t)c * gridDim.x + blockIdx.x) * 2 + 1] = red[1][0];
+  }
+}
+
+template <bool WIDE>
+__global__ __launch_bounds__(kThreads) void abn8_backward_apply_kernel(const float *__restrict__ gy, const unsigned *__restrict__ codes,
+                                                                      const unsigned char *__restrict__ scales, const unsigned *__restrict__ signs,
+                                                                      const double *__restrict__ sums, int blocks, double M, const float *__restrict__ weight,
+                                                                      float abs_eps, const float *__restrict__ vec, float *__restrict__ gweight,
+                                                                      float *__restrict__ gbias, float *__restrict__ gx, int C, size_t n, size_t nb,
+                                                                      unsigned chunks, float slope) {
+  const size_t plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const int c = (int)(plane % C);
+  double s0, s1;
+  channel_totals(sums, blocks, c, s0, s1);
+  const float m1 = (float)(s0 / M), m2 = (float)(s1 / M), a = vec[c];
+  if (chunk == 0 && plane == (size_t)c && threadIdx.x == 0) {
+    const float w = weight[c];
+    const float sgn = abs_eps >= 0.0f ? (w > 0.0f ? 1.0f : (w < 0.0f ? -1.0f : 0.0f)) : 1.0f;   // d|w| / dw
+    gweight[c] = (float)s1 * sgn;
+    gbias[c] = (float)s0;
+  }
+  if (!gx) return;
+  const int lane = threadIdx.x & (kLanes - 1);
+#pragma unroll 2
+  for (int turn = 0; turn < kTurns; ++turn) {
+    const size_t blk = (chunk * kTurns + turn) * kGroups + threadIdx.x / kLanes, first = blk * kBlock + 4 * lane, at = plane * nb + blk;
+    if (blk >= nb) break;
+    const int left = left_of(n, first);
+    float v[4];
+    load4<float, WIDE>(gy + plane * n + first, left, v);
+    const unsigned q = codes[at * kLanes + lane], up = signs[at] >> (4 * lane);
+    const float step = casmvs::block8::step_of(scales[at]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float g = v[i] * ((up >> i) & 1u ? 1.0f : slope);
+      v[i] = a * (g - m1 - casmvs::block8::value_of(q, i, step) * m2);
+    }
+    store4<float, WIDE>(gx + plane * n + first, left, v);
+  }
+}
+
+int sums_blocks(int N, size_t n) {
+  const size_t blocks = ((size_t)N * n + kThreads * 64 - 1) / (kThreads * 64);
+  return (int)(blocks < 1 ? 1 : blocks > 256 ? 256 : blocks);
+}
+size_t blocks_of(size_t n) { return (n + kBlock - 1) / kBlock; }
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+int check_planes(const char *what, int N, int C, size_t n) {
+  CASMVS_REQUIRE(N > 0 && C > 0 && C <= 65535 && n > 0, "%s: N=%d C=%d n=%zu", what, N, C, n);
+  const size_t chunks = (blocks_of(n) + kTurns * kGroups - 1) / (kTurns * kGroups);
+  CASMVS_REQUIRE((size_t)N * C <= ((size_t)1 << 31) / 1024 && chunks < ((size_t)1 << 31) / ((size_t)N * C), "%s: %d x %d planes of %zu elements", what, N, C, n);
+  return CASMVS_OK;
+}
+}  // namespace
+
+extern "C" int casmvs_pack8(const void *x, int dtype, size_t rows, size_t n, void *codes, void *scales, void *stream) {
+  casmvs::clear_error();
+  CASMVS_REQUIRE(casmvs::elem::known(dtype), "pack8: dtype %d", dtype);
+  if (rows == 0 || n == 0) return CASMVS_OK;
+  CASMVS_REQUIRE(x && codes && scales, "pack8: null pointer");
+  CASMVS_REQUIRE(((uintptr_t)codes & 3) == 0, "pack8: codes are written four at a time (4-byte alignment)");
+  CASMVS_REQUIRE(n <= kMostElements && rows <= kMostElements / n, "pack8: %zu rows of %zu", rows, n);
+  if (n % kBlock == 0) { n *= rows; rows = 1; }   // blocks do not end inside a row: one long row
+  const size_t nb = blocks_of(n), total = rows * nb;
+  const size_t wanted = (total + kGroups - 1) / kGroups;
+  const unsigned grid = (unsigned)(wanted < 8192 ? wanted : 8192);
+  const bool wide = n % 4 == 0 && aligned16(x);
+  CASMVS_WITH_DTYPE(dtype, {
+    if (wide)
+      hipLaunchKernelGGL((pack8_kernel<T, true>), dim3(grid), dim3(kThreads), 0, (hipStream_t)stream, (const T *)x, (unsigned *)codes, (unsigned char *)scales, rows, n, nb);
+    else
+      hipLaunchKernelGGL((pack8_kernel<T, false>), dim3(grid), dim3(kThreads), 0, (hipStream_t)stream, (const T *)x, (unsigned *)codes, (unsigned char *)scales, rows, n, nb);
+  });
+  return casmvs::check_launch("pack8_kernel");
+}
+
+extern "C" int casmvs_unpack8(const void *codes, const void *scales, const float *weight, const float *bias, int C, float slope, void *out, int dtype,
+                              size_t rows, size_t n, void *stream) {
+  casmvs::clear_error();
+  CASMVS_REQUIRE(casmvs::elem::known(dtype), "unpack8: dtype %d", dtype);
+  if (rows == 0 || n == 0) return CASMVS_OK;
+  CASMVS_REQUIRE(codes && scales && out, "unpack8: null pointer");
+  CASMVS_REQUIRE(((uintptr_t)codes & 3) == 0, "unpack8: codes are read four at a time (4-byte alignment)");
+  CASMVS_REQUIRE((weight == nullptr) == (bias == nullptr) && (!weight || C > 0), "unpack8: weight and bias go together, with their number of channels");
+  CASMVS_REQUIRE(n <= kMostElements && rows <= kMostElements / n, "unpack8: %zu rows of %zu", rows, n);
+  if (n % kBlock == 0 && !weight) { n *= rows; rows = 1; }
+  const size_t nb = blocks_of(n), total = rows * nb;
+  const size_t wanted = (total + kGroups - 1) / kGroups;
+  const unsigned grid = (unsigned)(wanted < 8192 ? wanted : 8192);
+  const bool wide = n % 4 == 0 && aligned16(out);
+#define CASMVS_UNPACK8(W, A)                                                                                                                          \
+  hipLaunchKernelGGL((unpack8_kernel<T, W, A>), dim3(grid), dim3(kThreads), 0, (hipStream_t)stream, (const unsigned *)codes, (const unsigned char *)scales, \
+                     (T *)out, weight, bias, C, slope, rows, n, nb)
+  CASMVS_WITH_DTYPE(dtype, {
+    if (weight) {
+      if (wide) CASMVS_UNPACK8(true, true); else CASMVS_UNPACK8(false, true);
+    } else {
+      if (wide) CASMVS_UNPACK8(true, false); else CASMVS_UNPACK8(false, false);
+    }
+  });
+#undef CASMVS_UNPACK8
+  return casmvs::check_launch("unpack8_kernel");
+}
+
+extern "C" int casmvs_abn8_train_apply_f32(const float *x, const double *sums, int blocks, double count, const float *weight, const float *bias,
+                                           float abs_eps, float eps, float momentum, float *running_mean, float *running_var, float *vec, float *y,
+                                           void *codes, void *scales, void *signs, int N, int C, size_t n, float slope, void *stream) {
+  casmvs::clear_error();
+  if (int rc = check_planes("abn8_train_apply", N, C, n)) return rc;
+  CASMVS_REQUIRE(x && sums && weight && bias && vec && y && codes && scales && signs && blocks > 0 && count > 0.0, "abn8_train_apply: bad arguments");
+  CASMVS_REQUIRE((running_mean == nullptr) == (running_var == nullptr), "abn8_train_apply: running_mean and running_var go together");
+  CASMVS_REQUIRE((((uintptr_t)codes | (uintptr_t)signs) & 3) == 0, "abn8_train_apply: codes and signs are written as 4-byte words");
+  const size_t nb = blocks_of(n), chunks = (nb + kTurns * kGroups - 1) / (kTurns * kGroups);
+  const dim3 grid((unsigned)((size_t)N * C * chunks));
+  auto kernel = n % 4 == 0 && aligned16(x) && aligned16(y) ? abn8_apply_kernel<true> : abn8_apply_kernel<false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, (hipStream_t)stream, x, sums, blocks, count, weight, bias, abs_eps, eps, momentum, running_mean,
+                     running_var, vec, y, (unsigned *)codes, (unsigned char *)scales, (unsigned *)signs, C, n, nb, (unsigned)chunks, slope);
+  return casmvs::check_launch("abn8_apply_kernel");
+}
+
+extern "C" int casmvs_abn8_backward_sums_blocks(int N, size_t n) { return sums_blocks(N, n); }
+
+extern "C" int casmvs_abn8_backward_sums_f64(const float *grad_y, const void *codes, const void *scales, const void *signs, double *sums, int N, int C, size_t n,
+                                             float slope, void *stream) {
+  casmvs::clear_error();
+  if (int rc = check_planes("abn8_backward_sums", N, C, n)) return rc;
+  CASMVS_REQUIRE(grad_y && codes && scales && signs && sums, "abn8_backward_sums: null pointer");
+  CASMVS_REQUIRE((((uintptr_t)codes | (uintptr_t)signs) & 3) == 0, "abn8_backward_sums: codes and signs are read as 4-byte words");
+  auto kernel = n % 4 == 0 && aligned16(grad_y) ? abn8_backward_sums_kernel<true> : abn8_backward_sums_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)sums_blocks(N, n), (unsigned)C), dim3(kThreads), 0, (hipStream_t)stream, grad_y, (const unsigned *)codes,
+                     (const unsigned char *)scales, (const unsigned *)signs, sums, N, C, n, blocks_of(n), slope);
+  return casmvs::check_launch("abn8_backward_sums_kernel");
+}
+
+extern "C" int casmvs_abn8_backward_apply_f32(const float *grad_y, const void *codes, const void *scales, const void *signs, const double *sums, int blocks,
+                                              double count, const float *weight, float abs_eps, const float *vec, float *grad_weight, float *grad_bias,
+                                              float *grad_x, int N, int C, size_t n, float slope, void *stream) {
+  casmvs::clear_error();
+  if (int rc = check_planes("abn8_backward_apply", N, C, n)) return rc;
+  CASMVS_REQUIRE(grad_y && codes && scales && signs && sums && weight && vec && grad_weight && grad_bias && blocks > 0 && count > 0.0,
+                 "abn8_backward_apply: bad arguments");
+  CASMVS_REQUIRE((((uintptr_t)codes | (uintptr_t)signs) & 3) == 0, "abn8_backward_apply: codes and signs are read as 4-byte words");
+  const size_t nb = blocks_of(n), chunks = (nb + kTurns * kGroups - 1) / (kTurns * kGroups);
+  const dim3 grid((unsigned)((size_t)N * C * chunks));
+  auto kernel = n % 4 == 0 && aligned16(grad_y) && (!grad_x || aligned16(grad_x)) ? abn8_backward_apply_kernel<true> : abn8_backward_apply_kernel<false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, (hipStream_t)stream, grad_y, (const unsigned *)codes, (const unsigned char *)scales,
+                     (const unsigned *)signs, sums, blocks, count, weight, abs_eps, vec, grad_weight, grad_bias, grad_x, C, n, nb, (unsigned)chunks, slope);
+  return casmvs::check_launch("abn8_backward_apply_kernel");
+}

@@ -1,0 +1,211 @@
+// Softmax cross entropy over the depth hypotheses, forward and backward.
+//
+//   t = argmin_k |d_k - gt| (lowest k on ties);  a pixel counts if its mask is set, min_k d_k <= gt <= max_k d_k and some cost is above -inf
+//   loss = mean over the counted pixels of (log sum_k exp(c_k) - c_t);   d loss / d c_k = (exp(c_k - m) / s - [k = t]) / count
+//
+// One pass over the hypothesis axis with the running maximum m and the sum s of exp(c_k - m); what the backward pass needs beside the costs is m, 1 / s and
+// t (12 bytes per pixel), never a volume of probabilities.  m and 1 / s are kept apart: their sum m + log s, rounded to float32, would move every
+// probability by the rounding of a number as large as the costs.  The distances to gt are formed in 64 bits, where the differences of float32 depths are exact, so
+// which of two planes is the nearer one does not depend on a rounding.
+// Both passes wait for memory: forward cost + depth value per hypothesis, backward cost in and gradient out.  A pixel whose mask is not set reads nothing.
+#include "elem_types.h"
+
+namespace {
+using casmvs::elem::Vec;
+
+constexpr int kThreads = 256;
+constexpr int kPixels = 64;               // pixels per workgroup
+constexpr int kPieces = kThreads / kPixels;   // pieces of the hypothesis axis, joined at the end
+constexpr int kChunk = 8;                 // hypotheses loaded before they are used
+
+struct Running {   // of one pixel over some of its hypotheses
+  float m, s;              // the largest cost, sum of exp(cost - m)
+  double near;             // the smallest distance to gt, where it is and the cost there
+  int at;
+  float cost_at, low, high;   // smallest / largest depth
+};
+
+// exp(a - m) where m may be -inf (then a is, too): 0
+__device__ __forceinline__ float exp_below(float a, float m) { return m == -INFINITY ? (a == -INFINITY ? 0.0f : expf(a)) : expf(a - m); }
+
+__device__ __forceinline__ void join(Running &r, const Running &o) {   // o: the hypotheses behind r's
+  const float m = fmaxf(r.m, o.m);
+  r.s = r.s * exp_below(r.m, m) + o.s * exp_below(o.m, m);
+  r.m = m;
+  if (o.near < r.near) {
+    r.near = o.near;
+    r.at = o.at;
+    r.cost_at = o.cost_at;
+  }
+  r.low = fminf(r.low, o.low);
+  r.high = fmaxf(r.high, o.high);
+}
+
+template <class T, bool PER_PIXEL>
+__global__ __launch_bounds__(kThreads) void depth_ce_forward_kernel(const T *__restrict__ cost, const float *__restrict__ depth, const float *__restrict__ gt,
+                                                                   const unsigned char *__restrict__ mask, float2 *__restrict__ stats, int *__restrict__ target,
+                                                                   double *__restrict__ partial, size_t pixels, int D, size_t hw) {
+  const int lane = threadIdx.x % kPixels, piece = threadIdx.x / kPixels;
+  const size_t p = (size_t)blockIdx.x * kPixels + lane;
+  const bool live = p < pixels && (!mask || mask[p]);
+  const size_t b = live ? p / hw : 0, s = live ? p % hw : 0;
+  Running r = {-INFINITY, 0.0f, INFINITY, 0, 0.0f, INFINITY, -INFINITY};
+  if (live) {
+    const int per = (D + kPieces - 1) / kPieces, lo = piece * per, hi = lo + per < D ? lo + per : D;
+    const double true_depth = gt[p];
+    const T *cp = cost + (b * D) * hw + s;
+    const float *dp = PER_PIXEL ? depth + (b * D) * hw + s : depth + b * D;
+    for (int k0 = lo; k0 < hi; k0 += kChunk) {
+      float c[kChunk], d[kChunk];
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        const int k = k0 + i < hi ? k0 + i : hi - 1;
+        c[i] = (float)cp[(size_t)k * hw];
+        d[i] = dp[PER_PIXEL ? (size_t)k * hw : (size_t)k];
+      }
+      float m = r.m;
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) m = fmaxf(m, c[i]);
+      r.s *= exp_below(r.m, m);
+      r.m = m;
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i)
+        if (k0 + i < hi) {
+          r.s += exp_below(c[i], m);
+          const double far = __builtin_fabs((double)d[i] - true_depth);
+          if (far < r.near) {
+            r.near = far;
+            r.at = k0 + i;
+            r.cost_at = c[i];
+          }
+          r.low = fminf(r.low, d[i]);
+          r.high = fmaxf(r.high, d[i]);
+        }
+    }
+  }
+  __shared__ Running joined[kPieces][kPixels];
+  __shared__ double red[2][kPixels];
+  joined[piece][lane] = r;
+  __syncthreads();
+  if (piece == 0) {
+    for (int q = 1; q < kPieces; ++q) join(r, joined[q][lane]);
+    bool counted = false;
+    if (live) {
+      const float g = gt[p];
+      counted = g >= r.low && g <= r.high && !(r.m == -INFINITY && r.s == 0.0f);
+    }
+    if (p < pixels) {
+      stats[p] = float2{counted ? r.m : 0.0f, counted ? 1.0f / r.s : 0.0f};
+      target[p] = counted ? r.at : -1;
+    }
+    red[0][lane] = counted ? (double)(logf(r.s) + (r.m - r.cost_at)) : 0.0;
+    red[1][lane] = counted ? 1.0 : 0.0;
+  }
+  __syncthreads();
+  for (int st = kPixels / 2; st > 0; st >>= 1) {
+    if ((int)threadIdx.x < st) {
+      red[0][threadIdx.x] += red[0][threadIdx.x + st];
+      red[1][threadIdx.x] += red[1][threadIdx.x + st];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    partial[2 * (size_t)blockIdx.x] = red[0][0];
+    partial[2 * (size_t)blockIdx.x + 1] = red[1][0];
+  }
+}
+
+// loss = the mean, share = 1 / count (0 where no pixel counts: the loss and every gradient are 0 then)
+__global__ __launch_bounds__(kThreads) void depth_ce_finish_kernel(const double *__restrict__ partial, size_t blocks, float *__restrict__ loss,
+                                                                  float *__restrict__ share) {
+  __shared__ double red[2][kThreads];
+  double s0 = 0.0, s1 = 0.0;
+  for (size_t b = threadIdx.x; b < blocks; b += kThreads) {
+    s0 += partial[2 * b];
+    s1 += partial[2 * b + 1];
+  }
+  red[0][threadIdx.x] = s0;
+  red[1][threadIdx.x] = s1;
+  __syncthreads();
+  for (int st = kThreads / 2; st > 0; st >>= 1) {
+    if ((int)threadIdx.x < st) {
+      red[0][threadIdx.x] += red[0][threadIdx.x + st];
+      red[1][threadIdx.x] += red[1][threadIdx.x + st];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    *loss = red[1][0] > 0.0 ? (float)(red[0][0] / red[1][0]) : 0.0f;
+    *share = red[1][0] > 0.0 ? (float)(1.0 / red[1][0]) : 0.0f;
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(kThreads) void depth_ce_backward_kernel(const T *__restrict__ cost, const float2 *__restrict__ stats, const int *__restrict__ target,
+                                                                    const float *__restrict__ share_of_one, const float *__restrict__ gloss,
+                                                                    T *__restrict__ grad, size_t pixels, int D, size_t hw) {
+  const size_t p = (size_t)blockIdx.x * kThreads + threadIdx.x;
+  if (p >= pixels) return;
+  const size_t b = p / hw, s = p % hw;
+  const int t = target[p];
+  const float2 st = stats[p];
+  const float share = *share_of_one * *gloss;
+  const int per = (D + (int)gridDim.y - 1) / (int)gridDim.y, lo = (int)blockIdx.y * per, hi = lo + per < D ? lo + per : D;
+  const T *cp = cost + (b * D) * hw + s;
+  T *gp = grad + (b * D) * hw + s;
+#pragma unroll 4
+  for (int k = lo; k < hi; ++k) {
+    const float q = t < 0 ? 0.0f : (exp_below((float)cp[(size_t)k * hw], st.x) * st.y - (k == t ? 1.0f : 0.0f)) * share;
+    gp[(size_t)k * hw] = (T)q;
+  }
+}
+
+int check_sizes(const char *what, int dtype, int B, int D, size_t hw) {
+  CASMVS_REQUIRE(casmvs::elem::known(dtype), "%s: dtype %d", what, dtype);
+  CASMVS_REQUIRE(B > 0 && D > 0 && D <= 65536 && hw < ((size_t)1 << 36) / (size_t)B, "%s: B=%d D=%d h*w=%zu", what, B, D, hw);
+  return CASMVS_OK;
+}
+size_t forward_blocks(size_t pixels) { return (pixels + kPixels - 1) / kPixels; }
+}  // namespace
+
+extern "C" size_t casmvs_depth_ce_workspace_bytes(int B, int D, size_t hw) {
+  if (B <= 0 || D <= 0) return 0;
+  return forward_blocks((size_t)B * hw) * 16 + 16;
+}
+
+extern "C" int casmvs_depth_ce_forward(const void *cost, const float *depth_values, const float *depth_gt, const void *mask, float *stats, int *target,
+                                       float *loss, float *share, void *workspace, int dtype, int B, int D, size_t hw, int per_pixel, void *stream) {
+  casmvs::clear_error();
+  if (int rc = check_sizes("depth_ce_forward", dtype, B, D, hw)) return rc;
+  CASMVS_REQUIRE(loss && share && workspace, "depth_ce_forward: null pointer");
+  const size_t pixels = (size_t)B * hw, blocks = pixels ? forward_blocks(pixels) : 0;
+  CASMVS_REQUIRE(!pixels || (cost && depth_values && depth_gt && stats && target), "depth_ce_forward: null pointer");
+  hipStream_t st = (hipStream_t)stream;
+  double *partial = (double *)workspace;
+  if (pixels) {
+    CASMVS_WITH_DTYPE(dtype, {
+      auto kernel = per_pixel ? depth_ce_forward_kernel<T, true> : depth_ce_forward_kernel<T, false>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, (const T *)cost, depth_values, depth_gt, (const unsigned char *)mask,
+                         (float2 *)stats, target, partial, pixels, D, hw);
+    });
+  }
+  hipLaunchKernelGGL(depth_ce_finish_kernel, dim3(1), dim3(kThreads), 0, st, partial, blocks, loss, share);
+  return casmvs::check_launch("depth_ce_forward");
+}
+
+extern "C" int casmvs_depth_ce_backward(const void *cost, const float *stats, const int *target, const float *share, const float *grad_loss, void *grad_cost,
+                                        int dtype, int B, int D, size_t hw, void *stream) {
+  casmvs::clear_error();
+  if (int rc = check_sizes("depth_ce_backward", dtype, B, D, hw)) return rc;
+  const size_t pixels = (size_t)B * hw;
+  if (!pixels) return CASMVS_OK;
+  CASMVS_REQUIRE(cost && stats && target && share && grad_loss && grad_cost, "depth_ce_backward: null pointer");
+  const size_t blocks = (pixels + kThreads - 1) / kThreads;
+  size_t split = 2048 / blocks;   // few pixels: pieces of the hypothesis axis
+  split = split < 1 ? 1 : split > (size_t)D ? (size_t)D : split;
+  CASMVS_WITH_DTYPE(dtype, {
+    hipLaunchKernelGGL(depth_ce_backward_kernel<T>, dim3((unsigned)blocks, (unsigned)split), dim3(kThreads), 0, (hipStream_t)stream, (const T *)cost,
+                       (const float2 *)stats, target, share, grad_loss, (T *)grad_cost, pixels, D, hw);
+  });
+  return casmvs::check_launch("depth_ce_backward_kernel");
+}

@@ -20,6 +20,7 @@ import torch.nn as nn
 from . import ops
 from .inplace_abn import InPlaceABN
 from .modules import ConvBnReLU, ConvBnReLU3D, _per_sample
+from .norm import LayerNormAct
 from .profiling import stage
 
 
@@ -163,6 +164,11 @@ class FeatureNet(_PackedWeights, nn.Module):
         self.timer = None         # optional profiling.StageTimer (bench.py)
         self.last_channels_last = None
 
+    @property
+    def foldable(self):
+        """Whether eval mode runs the fused engine: the norm folds into the convolutions (ABN does, layer norm does not)."""
+        return not isinstance(getattr(self.conv0[0], "bn", None), LayerNormAct)
+
     def packed_layers(self, device):
         """Folded + packed parameter images on `device` (re-packed whenever a tensor changed)."""
         sf = self.fuse_tail and self.tail_mode == "splitf16"
@@ -219,6 +225,10 @@ class FeatureNet(_PackedWeights, nn.Module):
         if self.training:   # batch statistics + autograd graph (training.py); eval mode = the fused engine below
             from .training import feature_net_train
             return feature_net_train(self, x.float())
+        if not self.foldable:   # layer norm: the layer-by-layer forward, without a graph
+            from .training import feature_net_train
+            with torch.no_grad():
+                return feature_net_train(self, x.float())
         N, _, H, W = x.shape
         if self.tail_mode not in ("splitf16", "f32"):
             raise ValueError(f"FeatureNet.tail_mode={self.tail_mode!r} (splitf16 or f32)")
@@ -294,6 +304,11 @@ class CostRegNet(_PackedWeights, nn.Module):
         self._ci_active = False     # ... and whether the five images of _ci_sf are
         self._s2_active = False     # ... and the two of _s2_sf
 
+    @property
+    def foldable(self):
+        """Whether eval mode runs the fused engine: the norm folds into the convolutions (ABN does, layer norm does not)."""
+        return not isinstance(getattr(self.conv0, "bn", None), LayerNormAct)
+
     # -- weight folding / packing -------------------------------------------------------------
     def _layer_tensors(self, name):
         m = getattr(self, name)
@@ -367,6 +382,10 @@ class CostRegNet(_PackedWeights, nn.Module):
         if self.training:   # batch statistics + autograd graph (training.py); eval mode = the fused engine below
             from .training import cost_reg_net_train
             return cost_reg_net_train(self, x)
+        if not self.foldable:   # layer norm: the layer-by-layer forward, without a graph
+            from .training import cost_reg_net_train
+            with torch.no_grad():
+                return cost_reg_net_train(self, x.float())
         B, _, D, h, w = x.shape
         packed = self.packed_layers(x.device)
         need = ops.costreg_workspace_bytes(B, D, h, w)
@@ -419,6 +438,9 @@ class CascadeMVSNet(nn.Module):
         self.keep_cost = False   # parity tests: keep the regularised cost (B,D,h,w) of every level in last_cost
         self.fuse_regress = True  # eval mode: `prob` + softmax regression in one library call (CostRegNet.regress)
         self.last_cost = {}
+        # train mode: what a step keeps for its backward pass, "f32" tensors or "8bit" checkpoints (training.py); whether the results hold cost_l / depth_values_l
+        self.checkpoint_mode = "f32"
+        self.return_cost = False
         self._const_cache = {}
 
     def _const(self, value, B, device):
@@ -457,7 +479,7 @@ class CascadeMVSNet(nn.Module):
                 volume = ops.costvol(feats_channels_last, proj_mats, depth_values, self.G, channels_last=True)
             else:
                 volume = ops.costvol(feats, proj_mats, depth_values, self.G)
-        if self.fuse_regress and isinstance(cost_reg, CostRegNet) and not cost_reg.training:
+        if self.fuse_regress and isinstance(cost_reg, CostRegNet) and cost_reg.foldable and not cost_reg.training:
             # mvsnet.py:174-193 inside the CostRegNet call: the `prob` head hands its cost values to the regression
             out = cost_reg.regress(volume, depth_values, return_index=self.keep_index)
             cost, depth, confidence = out[:3]
@@ -498,7 +520,7 @@ class CascadeMVSNet(nn.Module):
         t = self.timer
         with torch.no_grad():
             # (a user's replacement module, or FeatureNet left in train mode, returns the reference's (N,C,h,w) dict)
-            engine_feats = type(self.feature) is FeatureNet and not self.feature.training
+            engine_feats = type(self.feature) is FeatureNet and self.feature.foldable and not self.feature.training
             with stage(t, "feature"):
                 feats = self.feature(imgs, pixel_major_only=True) if engine_feats else self.feature(imgs)
             depth_l = None

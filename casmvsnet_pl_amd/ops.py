@@ -904,3 +904,151 @@ def selftest_mfma_rate(shape=1, blocks=2048, iters=4096):
     rc = _lib.load().casmvs_selftest_mfma_rate(shape, blocks, iters, ctypes.byref(out))
     _lib.check(rc, "casmvs_selftest_mfma_rate")
     return out.value
+
+
+# ---- training-side operators: layer norm, 8-bit activation checkpoints, cross entropy over depth hypotheses ---------------------------------------------------
+_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _float_dev(t, name):
+    """_dev for the operators that take float32, float16 and bfloat16 tensors."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t)}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name}: casmvsnet_pl_amd ops run on the MI355X only (got a {t.device} tensor); "
+                           "there is no CPU fallback")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name}: expected float32, float16 or bfloat16, got {t.dtype}")
+    return t.contiguous()
+
+
+def _same_device(ref, t, name):
+    if t.device != ref.device:
+        raise ValueError(f"{name}: on {t.device}, the other tensors are on {ref.device}")
+    return t
+
+
+def _layer_norm_args(x, weight, bias, eps, slope, channels_last):
+    """Checked (x, weight, bias) and the (outer, C, inner) that the library sees."""
+    x = _float_dev(x, "x")
+    if x.dim() < (1 if channels_last else 2):
+        raise ValueError(f"layer_norm: x {tuple(x.shape)} has no channel axis")
+    C = x.shape[-1 if channels_last else 1]
+    if not 1 <= C <= 65535:
+        raise ValueError(f"layer_norm: {C} channels (1 .. 65535)")
+    if not (eps >= 0 and eps < float("inf")) or slope != slope or abs(slope) == float("inf"):
+        raise ValueError(f"layer_norm: eps={eps} slope={slope}")
+    affine = []
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            t = _same_device(x, _dev(t, name), name)
+            if tuple(t.shape) != (C,):
+                raise ValueError(f"layer_norm: {name} {tuple(t.shape)}, expected ({C},)")
+        affine.append(t)
+    inner = 1
+    if not channels_last:
+        for s in x.shape[2:]:
+            inner *= s
+    outer = x.numel() // (C * inner) if x.numel() else 0
+    return x, affine[0], affine[1], outer, C, inner
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, slope=1.0, channels_last=False):
+    """Layer norm over the channel axis + leaky ReLU (casmvs_layer_norm_forward): x (N,C,*spatial) - or (..,C) with channels_last=True, the layout of the
+    pixel-major feature maps -, float32 / float16 / bfloat16; weight, bias (C,) float32 or None -> x's shape and type.  slope 1: no activation.
+    No autograd graph: autograd.layer_norm is the differentiable form."""
+    x, weight, bias, outer, C, inner = _layer_norm_args(x, weight, bias, eps, slope, channels_last)
+    y = torch.empty_like(x)
+    with torch.cuda.device(x.device):
+        rc = _lib.load().casmvs_layer_norm_forward(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _DTYPES[x.dtype], outer, C, inner, float(eps), float(slope),
+                                                   _stream(x))
+    _lib.check(rc, "casmvs_layer_norm_forward")
+    return y
+
+
+def layer_norm_backward(x, grad_y, weight=None, bias=None, eps=1e-5, slope=1.0, channels_last=False, need_x=True, need_affine=True):
+    """The gradients of layer_norm at x (casmvs_layer_norm_backward; the statistics are recomputed) -> (grad_x or None, grad_weight, grad_bias or None)."""
+    x, weight, bias, outer, C, inner = _layer_norm_args(x, weight, bias, eps, slope, channels_last)
+    grad_y = _same_device(x, _float_dev(grad_y, "grad_y"), "grad_y")
+    if grad_y.shape != x.shape or grad_y.dtype != x.dtype:
+        raise ValueError(f"layer_norm_backward: x {tuple(x.shape)} {x.dtype}, grad_y {tuple(grad_y.shape)} {grad_y.dtype}")
+    lib, code = _lib.load(), _DTYPES[x.dtype]
+    gx = torch.empty_like(x) if need_x else None
+    gw, gb = (torch.empty(C, dtype=torch.float32, device=x.device) for _ in range(2)) if need_affine else (None, None)
+    ws = torch.empty(lib.casmvs_layer_norm_backward_workspace_bytes(code, outer, C, inner), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        rc = lib.casmvs_layer_norm_backward(_ptr(x), _ptr(grad_y), _ptr(weight), _ptr(bias), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), code, outer, C, inner,
+                                            float(eps), float(slope), _stream(x))
+    _lib.check(rc, "casmvs_layer_norm_backward")
+    return gx, gw, gb
+
+
+class Packed8:
+    """An 8-bit checkpoint (casmvs_pack8): `codes` (planes, ceil(n / 32), 32) and `scales` (planes, ceil(n / 32)) uint8, the shape and type of the tensor it stands
+    for.  affine: None, or (weight, bias, slope) of the per-channel affine + leaky ReLU that unpack8 applies to the held values (channel = axis 1)."""
+
+    __slots__ = ("codes", "scales", "shape", "dtype", "affine")
+
+    def __init__(self, codes, scales, shape, dtype, affine=None):
+        self.codes, self.scales, self.shape, self.dtype, self.affine = codes, scales, tuple(shape), dtype, affine
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+
+def _planes(shape):
+    """(rows, n) of the 8-bit format: a plane is what lies behind the channel axis, (N,C | *spatial); a matrix's rows; a vector."""
+    cut = min(2, max(len(shape) - 1, 0))
+    rows = n = 1
+    for s in shape[:cut]:
+        rows *= s
+    for s in shape[cut:]:
+        n *= s
+    return rows, n
+
+
+def pack8(x):
+    """8-bit checkpoint of a float32 / float16 / bfloat16 tensor -> Packed8: blocks of 32 values along a plane (of (N,C,*spatial): one (n, c); of a matrix: a row), a
+    power-of-two step per block, sign and 7 bits per value; 33 bytes per 32 values, an error of at most 2^-7 of the block's largest power of two.
+    A block with an Inf or a NaN reads back as NaN."""
+    x = _float_dev(x, "x")
+    rows, n = _planes(x.shape)
+    nb = (n + 31) // 32
+    codes = torch.empty((rows, nb, 32), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((rows, nb), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        rc = _lib.load().casmvs_pack8(_ptr(x), _DTYPES[x.dtype], rows, n, _ptr(codes), _ptr(scales), _stream(x))
+    _lib.check(rc, "casmvs_pack8")
+    return Packed8(codes, scales, x.shape, x.dtype)
+
+
+def unpack8(packed):
+    """The tensor that a Packed8 stands for, in its shape and type (casmvs_unpack8)."""
+    if not isinstance(packed, Packed8):
+        raise TypeError(f"unpack8: expected a Packed8, got {type(packed)}")
+    rows, n = _planes(packed.shape)
+    nb = (n + 31) // 32
+    codes, scales = packed.codes, packed.scales
+    for t, name, shape in ((codes, "codes", (rows, nb, 32)), (scales, "scales", (rows, nb))):
+        if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_cuda or not t.is_contiguous():
+            raise ValueError(f"unpack8: {name} {tuple(t.shape)} {t.dtype} on {t.device}, expected a contiguous uint8 {shape} on the GPU")
+    _same_device(codes, scales, "scales")
+    if packed.dtype not in _DTYPES:
+        raise TypeError(f"unpack8: expected float32, float16 or bfloat16, got {packed.dtype}")
+    weight = bias = None
+    slope, C = 1.0, 1
+    if packed.affine is not None:
+        weight, bias, slope = packed.affine
+        if len(packed.shape) < 3:
+            raise ValueError(f"unpack8: an affine needs planes (N,C,*spatial), the shape is {packed.shape}")
+        C = packed.shape[1]
+        weight, bias = (_same_device(codes, _dev(t, name), name) for t, name in ((weight, "weight"), (bias, "bias")))
+        if tuple(weight.shape) != (C,) or tuple(bias.shape) != (C,):
+            raise ValueError(f"unpack8: affine {tuple(weight.shape)} {tuple(bias.shape)}, expected ({C},)")
+    out = torch.empty(packed.shape, dtype=packed.dtype, device=codes.device)
+    with torch.cuda.device(codes.device):
+        rc = _lib.load().casmvs_unpack8(_ptr(codes), _ptr(scales), _ptr(weight), _ptr(bias), C, float(slope), _ptr(out), _DTYPES[packed.dtype], rows, n,
+                                        _stream(codes))
+    _lib.check(rc, "casmvs_unpack8")
+    return out

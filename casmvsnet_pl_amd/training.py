@@ -13,6 +13,13 @@ ABN / InPlaceABN in train mode (modules.py:14,27)      casmvs_channel_sums_f64 -
 F.interpolate(x2, bilinear, align_corners) + lateral   casmvs_upsample2x_add_f32 / casmvs_upsample2x_backward_f32
 homo_warp + variance volume (mvsnet.py:137-167)        fused forward kernel; casmvs_costvol_var_backward_f32
 softmax + depth regression (mvsnet.py:175-177)         autograd.softmax_depth_regression
+(norm_act = norm.LayerNormAct)                         autograd.layer_norm
+(the loss as a classification over the hypotheses)     autograd.depth_cross_entropy
+
+What a step keeps for its backward pass: float32 tensors (checkpoint="f32": the convolutions' inputs, ABN's input and output), or with checkpoint="8bit"
+(CascadeMVSNet.checkpoint_mode) 8-bit checkpoints: an ABN keeps 8 bits of its normalised input and one bit per element, the convolution behind it rebuilds its
+input from the same bytes, and a convolution whose input is anything else (a cost volume, a skip sum) packs that.  The forward pass is the same, bit for bit;
+the gradients carry the rounding of the 8 bits.
 
 torch is the autograd tape and the allocator; the skip additions of the U-Net and the gradient accumulation are torch adds.  Nothing here runs on CPU tensors.  DESIGN.md 2.6 has the kernels and the measured step
 times (18 ms per step at the reference's default training configuration, 15 ms captured as one hipGraph).
@@ -343,11 +350,53 @@ class _Conv(torch.autograd.Function):
         return gx, gw, gb, None
 
 
-def conv(x, weight, bias, kind):
-    """Differentiable convolution of one of the model's layer kinds (forward, input, weight and bias gradients in HIP)."""
+def conv(x, weight, bias, kind, checkpoint="f32"):
+    """Differentiable convolution of one of the model's layer kinds (forward, input, weight and bias gradients in HIP).
+    checkpoint "8bit": the weight gradient is taken at an 8-bit checkpoint of x - the one that the ABN which made x keeps already, or a new one.  An x that no
+    gradient goes to (the images) is kept as it is: its owner holds it anyway."""
     if not x.is_cuda:
         raise RuntimeError("casmvsnet_pl_amd.training runs on the MI355X only; there is no CPU fallback")
+    _check_checkpoint(checkpoint)
+    if checkpoint == "8bit" and x.requires_grad and weight.requires_grad and torch.is_grad_enabled():
+        packed, version = getattr(x, "_casmvs_packed8", (None, None))
+        if packed is None or version != x._version:   # not an ABN's output, or written to since
+            packed = ops.pack8(x.detach().float())
+        return _Conv8.apply(x, weight, bias, kind, packed)
     return _Conv.apply(x, weight, bias, kind)
+
+
+CHECKPOINTS = ("f32", "8bit")
+
+
+def _check_checkpoint(checkpoint):
+    if checkpoint not in CHECKPOINTS:
+        raise ValueError(f"checkpoint={checkpoint!r} (f32 or 8bit)")
+
+
+class _Conv8(torch.autograd.Function):
+    """_Conv that keeps its input as a Packed8: the weight gradient is taken at the unpacked values (one more pass over them, 33/32 + 4 bytes per element)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, kind, packed):
+        x = x.contiguous().float()
+        ctx.kind, ctx.has_bias, ctx.shape = kind, bias is not None, tuple(x.shape)
+        affine = packed.affine or (None, None, 1.0)
+        ctx.slope = affine[2]
+        ctx.save_for_backward(weight, packed.codes, packed.scales, affine[0], affine[1])
+        return _conv_raw(kind, weight, bias, x)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        weight, codes, scales, aff_w, aff_b = ctx.saved_tensors
+        gy = gy.contiguous().float()
+        gx = conv_dgrad(ctx.kind, weight, gy, ctx.shape) if ctx.needs_input_grad[0] else None
+        gw = None
+        if ctx.needs_input_grad[1]:
+            x = ops.unpack8(ops.Packed8(codes, scales, ctx.shape, torch.float32, None if aff_w is None else (aff_w, aff_b, ctx.slope)))
+            gw = conv_wgrad(ctx.kind, x, gy, tuple(weight.shape))
+        gb = channel_sums(gy)[0].float() if (ctx.has_bias and ctx.needs_input_grad[2]) else None
+        return gx, gw, gb, None, None
 
 
 class _ABNTrain(torch.autograd.Function):
@@ -409,10 +458,72 @@ class _ABNTrain(torch.autograd.Function):
         return gx, out[0], out[1], None, None, None, None, None, None
 
 
-def abn_train(norm, x):
+class _ABNTrain8(torch.autograd.Function):
+    """_ABNTrain that keeps 8 bits of the normalised input and one bit per element (casmvs_abn8_*): -> (y, codes, scales, vec), y as _ABNTrain's, bit for bit."""
+
+    @staticmethod
+    def forward(ctx, x, weight, beta, running_mean, running_var, momentum, eps, slope, abs_eps):
+        x = x.contiguous().float()
+        N, C = x.shape[:2]
+        n = x.numel() // (N * C)
+        M, nb = N * n, (n + 31) // 32
+        lib = _lib.load()
+        blocks = lib.casmvs_channel_sums_blocks(N, n)
+        part = torch.empty((C, blocks, 2), dtype=torch.float64, device=x.device)
+        vec = torch.empty((4, C), dtype=torch.float32, device=x.device)   # scale, shift, gamma, beta
+        codes = torch.empty((N * C, nb, 32), dtype=torch.uint8, device=x.device)
+        scales = torch.empty((N * C, nb), dtype=torch.uint8, device=x.device)
+        signs = torch.empty((N * C, nb), dtype=torch.int32, device=x.device)
+        y = torch.empty_like(x)
+        w, bta = weight.detach().contiguous().float(), beta.detach().contiguous().float()
+        track = running_mean is not None and running_var is not None
+        with torch.cuda.device(x.device):
+            st = _stream(x)
+            rc = lib.casmvs_channel_sums_f64(_ptr(x), _ptr(part), N, C, n, st)
+            _lib.check(rc, "casmvs_channel_sums_f64")
+            rc = lib.casmvs_abn8_train_apply_f32(_ptr(x), _ptr(part), blocks, float(M), _ptr(w), _ptr(bta), float(abs_eps), float(eps), float(momentum),
+                                                 _ptr(running_mean) if track else None, _ptr(running_var) if track else None, _ptr(vec), _ptr(y),
+                                                 _ptr(codes), _ptr(scales), _ptr(signs), N, C, n, float(slope), st)
+            _lib.check(rc, "casmvs_abn8_train_apply_f32")
+        if track:   # the kernel wrote the buffers behind torch's back: bump their version counters (packed-weight caches key on them)
+            torch.autograd.graph.increment_version(running_mean)
+            torch.autograd.graph.increment_version(running_var)
+        ctx.save_for_backward(codes, scales, signs, w, vec)
+        ctx.slope, ctx.M, ctx.abs_eps, ctx.n = float(slope), M, float(abs_eps), n
+        ctx.mark_non_differentiable(codes, scales, vec)
+        return y, codes, scales, vec
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy, *_):
+        codes, scales, signs, w, vec = ctx.saved_tensors
+        gy = gy.contiguous().float()
+        N, C = gy.shape[:2]
+        lib = _lib.load()
+        blocks = lib.casmvs_abn8_backward_sums_blocks(N, ctx.n)
+        part = torch.empty((C, blocks, 2), dtype=torch.float64, device=gy.device)
+        out = torch.empty((2, C), dtype=torch.float32, device=gy.device)   # grad_weight, grad_bias
+        gx = torch.empty_like(gy) if ctx.needs_input_grad[0] else None
+        with torch.cuda.device(gy.device):
+            st = _stream(gy)
+            rc = lib.casmvs_abn8_backward_sums_f64(_ptr(gy), _ptr(codes), _ptr(scales), _ptr(signs), _ptr(part), N, C, ctx.n, ctx.slope, st)
+            _lib.check(rc, "casmvs_abn8_backward_sums_f64")
+            rc = lib.casmvs_abn8_backward_apply_f32(_ptr(gy), _ptr(codes), _ptr(scales), _ptr(signs), _ptr(part), blocks, float(ctx.M), _ptr(w), ctx.abs_eps,
+                                                    _ptr(vec), _ptr(out[0]), _ptr(out[1]), _ptr(gx), N, C, ctx.n, ctx.slope, st)
+            _lib.check(rc, "casmvs_abn8_backward_apply_f32")
+        return gx, out[0], out[1], None, None, None, None, None, None
+
+
+def abn_train(norm, x, checkpoint="f32"):
     """Train-mode forward of an ABN-like module (`weight`, `bias`, `running_mean`, `running_var`, `eps`, `momentum`,
-    leaky-relu slope): inplace_abn.ABN (gamma = weight) or InPlaceABN (gamma = |weight| + eps, see inplace_abn.py)."""
+    leaky-relu slope): inplace_abn.ABN (gamma = weight) or InPlaceABN (gamma = |weight| + eps, see inplace_abn.py); of a norm.LayerNormAct: layer norm.
+    checkpoint "8bit": what is kept for the backward pass is 8 bits of the normalised input + one bit per element (x and y in float32 otherwise).  Layer
+    norm keeps its float32 input in either case."""
     from .inplace_abn import InPlaceABN
+    from .norm import LayerNormAct
+    _check_checkpoint(checkpoint)
+    if isinstance(norm, LayerNormAct):
+        return norm(x.float())
     if not getattr(norm, "affine", True) or norm.weight is None:
         raise RuntimeError("training: ABN without affine parameters is not supported")
     if isinstance(norm, InPlaceABN):
@@ -420,8 +531,13 @@ def abn_train(norm, x):
     else:                                                    # any other module: its own gamma expression stays an autograd graph
         weight, abs_eps = (norm._gamma() if hasattr(norm, "_gamma") else norm.weight), -1.0
     slope = norm.leaky_slope() if hasattr(norm, "leaky_slope") else float(getattr(norm, "activation_param", 0.01))
-    return _ABNTrain.apply(x, weight, norm.bias, norm.running_mean, norm.running_var, float(norm.momentum), float(norm.eps), slope,
-                           abs_eps)
+    args = (x, weight, norm.bias, norm.running_mean, norm.running_var, float(norm.momentum), float(norm.eps), slope, abs_eps)
+    if checkpoint == "f32":
+        return _ABNTrain.apply(*args)
+    y, codes, scales, vec = _ABNTrain8.apply(*args)
+    if y.dim() > 2:   # the convolution behind takes these as its own checkpoint: y = lrelu(gamma xhat + beta)
+        y._casmvs_packed8 = (ops.Packed8(codes, scales, y.shape, torch.float32, (vec[2], vec[3], slope)), y._version)
+    return y
 
 
 class _UpsampleAdd(torch.autograd.Function):
@@ -555,63 +671,72 @@ _KIND2D = {(3, 1, 1): CONV2D_K3, (5, 2, 2): CONV2D_K5S2, (1, 1, 0): CONV2D_K1}
 _KIND3D = {(3, 1, 1): CONV_S1, (3, 2, 1): CONV_S2}
 
 
-def conv_bn_relu_2d(m, x):
+def conv_bn_relu_2d(m, x, checkpoint="f32"):
     """modules.py:8-18 in train mode."""
     kind = _KIND2D.get(m._geometry)
     if kind is None:
         raise RuntimeError(f"training: ConvBnReLU geometry {m._geometry} is not a FeatureNet layer shape")
-    return abn_train(m.bn, conv(x, m.conv.weight, None, kind))
+    return abn_train(m.bn, conv(x, m.conv.weight, None, kind, checkpoint), checkpoint)
 
 
-def conv_bn_relu_3d(m, x):
+def conv_bn_relu_3d(m, x, checkpoint="f32"):
     """modules.py:21-31 in train mode."""
     kind = _KIND3D.get(m._geometry)
     if kind is None:
         raise RuntimeError(f"training: ConvBnReLU3D geometry {m._geometry} is not a CostRegNet layer shape")
-    return abn_train(m.bn, conv(x, m.conv.weight, None, kind))
+    return abn_train(m.bn, conv(x, m.conv.weight, None, kind, checkpoint), checkpoint)
 
 
-def feature_net_train(net, x):
+def feature_net_train(net, x, checkpoint="f32"):
     """mvsnet.py:40-57 in train mode: x (N,3,H,W) -> {"level_0", "level_1", "level_2"} with an autograd graph."""
     c0 = x
     for m in net.conv0:
-        c0 = conv_bn_relu_2d(m, c0)
+        c0 = conv_bn_relu_2d(m, c0, checkpoint)
     c1 = c0
     for m in net.conv1:
-        c1 = conv_bn_relu_2d(m, c1)
+        c1 = conv_bn_relu_2d(m, c1, checkpoint)
     c2 = c1
     for m in net.conv2:
-        c2 = conv_bn_relu_2d(m, c2)
-    feat2 = conv(c2, net.toplayer.weight, net.toplayer.bias, CONV2D_K1)
-    feat1 = upsample_add(conv(c1, net.lat1.weight, net.lat1.bias, CONV2D_K1), feat2)
-    feat0 = upsample_add(conv(c0, net.lat0.weight, net.lat0.bias, CONV2D_K1), feat1)
-    feat1 = conv(feat1, net.smooth1.weight, net.smooth1.bias, CONV2D_K3)
-    feat0 = conv(feat0, net.smooth0.weight, net.smooth0.bias, CONV2D_K3)
+        c2 = conv_bn_relu_2d(m, c2, checkpoint)
+    feat2 = conv(c2, net.toplayer.weight, net.toplayer.bias, CONV2D_K1, checkpoint)
+    feat1 = upsample_add(conv(c1, net.lat1.weight, net.lat1.bias, CONV2D_K1, checkpoint), feat2)
+    feat0 = upsample_add(conv(c0, net.lat0.weight, net.lat0.bias, CONV2D_K1, checkpoint), feat1)
+    feat1 = conv(feat1, net.smooth1.weight, net.smooth1.bias, CONV2D_K3, checkpoint)
+    feat0 = conv(feat0, net.smooth0.weight, net.smooth0.bias, CONV2D_K3, checkpoint)
     return {"level_0": feat0, "level_1": feat1, "level_2": feat2}
 
 
-def cost_reg_net_train(net, x):
+def cost_reg_net_train(net, x, checkpoint="f32"):
     """mvsnet.py:91-104 in train mode: x (B,Cin,D,h,w) -> (B,1,D,h,w)."""
-    conv0 = conv_bn_relu_3d(net.conv0, x)
-    conv2 = conv_bn_relu_3d(net.conv2, conv_bn_relu_3d(net.conv1, conv0))
-    conv4 = conv_bn_relu_3d(net.conv4, conv_bn_relu_3d(net.conv3, conv2))
-    y = conv_bn_relu_3d(net.conv6, conv_bn_relu_3d(net.conv5, conv4))
-    y = conv4 + abn_train(net.conv7[1], conv(y, net.conv7[0].weight, None, CONV_T2))
-    y = conv2 + abn_train(net.conv9[1], conv(y, net.conv9[0].weight, None, CONV_T2))
-    y = conv0 + abn_train(net.conv11[1], conv(y, net.conv11[0].weight, None, CONV_T2))
-    return conv(y, net.prob.weight, net.prob.bias, CONV_S1)
+    def layer(m, x):
+        return conv_bn_relu_3d(m, x, checkpoint)
+
+    def up(m, x):
+        return abn_train(m[1], conv(x, m[0].weight, None, CONV_T2, checkpoint), checkpoint)
+
+    conv0 = layer(net.conv0, x)
+    conv2 = layer(net.conv2, layer(net.conv1, conv0))
+    conv4 = layer(net.conv4, layer(net.conv3, conv2))
+    y = layer(net.conv6, layer(net.conv5, conv4))
+    y = conv4 + up(net.conv7, y)
+    y = conv2 + up(net.conv9, y)
+    y = conv0 + up(net.conv11, y)
+    return conv(y, net.prob.weight, net.prob.bias, CONV_S1, checkpoint)
 
 
 def cascade_forward_train(model, imgs, proj_mats, init_depth_min, depth_interval):
     """mvsnet.py:197-244 in train mode (what train.py:99-103 calls): the same loop as the inference forward, on the
-    differentiable ops.  Depth hypotheses come from the DETACHED previous depth (mvsnet.py:231)."""
+    differentiable ops.  Depth hypotheses come from the DETACHED previous depth (mvsnet.py:231).
+    model.checkpoint_mode: what the step keeps (module docstring); model.return_cost: the results also hold cost_l (B,D,h,w) - the regularised costs, in the
+    graph - and depth_values_l, what cross_entropy_loss takes."""
     from .modules import _per_sample
     B, V, _, H, W = imgs.shape
     dev = imgs.device
     plan = pack_plan_of(model)
     set_active_plan(plan)   # this step's forward AND backward take their layer images from the plan
     plan.begin_step()
-    feats = feature_net_train(model.feature, imgs.reshape(B * V, 3, H, W).float())
+    checkpoint = model.checkpoint_mode
+    feats = feature_net_train(model.feature, imgs.reshape(B * V, 3, H, W).float(), checkpoint)
     proj = proj_mats.float()
     results = {}
     depth_l = None
@@ -637,10 +762,12 @@ def cascade_forward_train(model, imgs, proj_mats, init_depth_min, depth_interval
             volume = variance_volume(feats_l, proj_l, depth_values)
         else:
             volume = groupwise_volume(feats_l, proj_l, depth_values, model.G)
-        cost = cost_reg_net_train(getattr(model, f"cost_reg_{l}"), volume).squeeze(1)
+        cost = cost_reg_net_train(getattr(model, f"cost_reg_{l}"), volume, checkpoint).squeeze(1)
         depth_l, confidence_l = A.softmax_depth_regression(cost, depth_values)
         results[f"depth_{l}"] = depth_l
         results[f"confidence_{l}"] = confidence_l
+        if model.return_cost:
+            results[f"cost_{l}"], results[f"depth_values_{l}"] = cost, depth_values
     return results
 
 
@@ -665,21 +792,41 @@ def sl1_loss_masked(results, depths, masks, levels=3):
     return loss
 
 
-def train_steps(model, batches, optimizer, device="cuda"):
+def cross_entropy_loss(results, depths, masks, levels=3):
+    """The depth as a classification over each level's hypotheses: sum over the levels of autograd.depth_cross_entropy * 2^(1 - l), sl1_loss's weights.  The results
+    of a model with return_cost = True.  A pixel whose ground truth lies outside its hypotheses (the finer levels sweep around the previous depth) does not
+    count; no host sync, capturable."""
+    loss = 0
+    for l in range(levels):
+        if f"cost_{l}" not in results:
+            raise ValueError("cross_entropy_loss: the results hold no costs (set model.return_cost = True before the forward)")
+        mask = masks[f"level_{l}"]
+        loss = loss + A.depth_cross_entropy(results[f"cost_{l}"], results[f"depth_values_{l}"], depths[f"level_{l}"],
+                                            mask if mask.dtype == torch.bool else mask != 0) * 2 ** (1 - l)
+    return loss
+
+
+def train_steps(model, batches, optimizer, device="cuda", loss="sl1"):
     """train.py:99-103 + Lightning's optimisation step, without Lightning: for every batch (dicts from pipeline.collate
     over pipeline.DTUReader samples in training layout: imgs_u8 / imgs, proj_mats, depths, masks, init_depth_min,
-    depth_interval) forward in train mode, SL1 loss, backward, optimizer step.  -> list of loss values."""
+    depth_interval) forward in train mode, loss, backward, optimizer step.  -> list of loss values.
+    loss: "sl1" (train.py's, sl1_loss) or "cross_entropy" (cross_entropy_loss)."""
+    if loss not in ("sl1", "cross_entropy"):
+        raise ValueError(f"train_steps: loss={loss!r} (sl1 or cross_entropy)")
     from .pipeline import DevicePrefetcher
     model.train()
+    if loss == "cross_entropy":
+        model.return_cost = True
+    loss_of = sl1_loss if loss == "sl1" else cross_entropy_loss
     losses = []
     for b in DevicePrefetcher(batches, device, depth=2):
         depths = {k: torch.stack([d[k] for d in b["depths"]]).to(device) for k in b["depths"][0]}
         masks = {k: torch.stack([m[k] for m in b["masks"]]).to(device) for k in b["masks"][0]}
         optimizer.zero_grad(set_to_none=True)
         results = model(b["imgs"], b["proj_mats"], b["init_depth_min"], b["depth_interval"])
-        loss = sl1_loss(results, depths, masks)
-        loss.backward()
+        value = loss_of(results, depths, masks)
+        value.backward()
         optimizer.step()
         release_plan()   # the step's graph is consumed
-        losses.append(float(loss.detach()))
+        losses.append(float(value.detach()))
     return losses

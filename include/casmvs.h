@@ -12,7 +12,7 @@
  *   - return 0 (CASMVS_OK) or a negative CASMVS_ERR_* code; never throw across the ABI.
  *     `casmvs_last_error()` returns a thread-local human readable message for the last failure.
  *   - every tensor is fp32, contiguous, row-major in the reference's own layout (NCHW / NCDHW);
- *     the *_nhwc entry points (pixel-major feature maps) say so explicitly.
+ *     the *_nhwc entry points (pixel-major feature maps) say so explicitly, and so do the ones that take a `dtype`.
  *   - the CALLER owns every buffer (inputs, outputs, workspace, packed weights).  The library
  *     allocates no device memory and keeps no pointer after return.
  *   - device pointers are raw `hipDeviceptr`-style `float*` on the calling thread's current
@@ -621,6 +621,56 @@ int casmvs_costvol_var_backward_f32(const float *feats, const float *proj, const
  * channel-expanded gradient volume, one warp backward and one recomputed warped volume per source view. */
 int casmvs_costvol_gwc_backward_f32(const float *feats, const float *proj, const float *depth, const float *grad_vol, float *grad_feats, void *workspace,
                                     int B, int V, int C, int G, int h, int w, int D, void *stream);
+
+/* ---- training-side operators beside ABN, the convolutions' saved tensors and the depth regression -----------------------------------------------------------
+ * Element types of the tensors these entry points take (statistics, weights and their gradients are float32 whatever the type). */
+#define CASMVS_DTYPE_F32 0
+#define CASMVS_DTYPE_F16 1
+#define CASMVS_DTYPE_BF16 2
+
+/* Layer norm over the channel axis of a contiguous (outer, C, inner) tensor - inner = 1: rows of C - followed by the leaky ReLU of `slope` (1: none):
+ *   y = lrelu((x - mean) / sqrt(var + eps) * weight[c] + bias[c]), mean and biased variance over the C channels of a position.
+ * weight / bias may be NULL (1 / 0).  Statistics and the side of zero are computed in 64 bits.  C <= 65535; outer or inner may be 0.
+ * The backward pass takes the forward's x (no statistics are kept).  grad_x may be NULL; grad_weight / grad_bias are both given or both NULL; the sums are formed in
+ * a fixed order (the same bits run to run).  workspace: casmvs_layer_norm_backward_workspace_bytes, 8-byte aligned. */
+int casmvs_layer_norm_forward(const void *x, const float *weight, const float *bias, void *y, int dtype, size_t outer, int C, size_t inner, float eps,
+                              float slope, void *stream);
+size_t casmvs_layer_norm_backward_workspace_bytes(int dtype, size_t outer, int C, size_t inner);
+int casmvs_layer_norm_backward(const void *x, const void *grad_y, const float *weight, const float *bias, void *grad_x, float *grad_weight, float *grad_bias,
+                               void *workspace, int dtype, size_t outer, int C, size_t inner, float eps, float slope, void *stream);
+
+/* 8-bit checkpoints of activations.  x: contiguous (rows, n); every row is cut into blocks of 32 (the last one may be shorter), nb = ceil(n / 32):
+ *   codes (rows, nb, 32) bytes, 4-byte aligned: sign bit | min(127, rint(|v| / step)); scales (rows, nb) bytes: e + 127, step = 2^(e - 6),
+ *   e = max(floor(log2 of the block's largest magnitude), -127); 255: the block holds an Inf or a NaN and reads back as NaN.
+ * casmvs_unpack8 writes code * step, or with weight / bias (C floats each) act(code * step * weight[row % C] + bias[row % C]) with the leaky ReLU of `slope`. */
+int casmvs_pack8(const void *x, int dtype, size_t rows, size_t n, void *codes, void *scales, void *stream);
+int casmvs_unpack8(const void *codes, const void *scales, const float *weight, const float *bias, int C, float slope, void *out, int dtype, size_t rows,
+                   size_t n, void *stream);
+
+/* Train-mode ABN (as casmvs_abn_train_apply_f32 from the sums of casmvs_channel_sums_f64; y is the same, bit for bit) that keeps for its backward pass the
+ * 8-bit checkpoint of xhat = (x - mean) rstd over the planes (N C, n) - codes, scales - and signs (N C, nb) 32-bit words: bit i of a word = [z > 0] of the block's
+ * value i.  vec (4, C): scale = gamma rstd, shift, gamma (|weight| + abs_eps where abs_eps >= 0), bias as the forward pass used them.
+ * Backward: sums (C, casmvs_abn8_backward_sums_blocks, 2) doubles, then grad_weight / grad_bias / grad_x (may be NULL).  N * C <= 2^21. */
+int casmvs_abn8_train_apply_f32(const float *x, const double *sums, int blocks, double count, const float *weight, const float *bias, float abs_eps,
+                                float eps, float momentum, float *running_mean, float *running_var, float *vec, float *y, void *codes, void *scales,
+                                void *signs, int N, int C, size_t n, float slope, void *stream);
+int casmvs_abn8_backward_sums_blocks(int N, size_t n);
+int casmvs_abn8_backward_sums_f64(const float *grad_y, const void *codes, const void *scales, const void *signs, double *sums, int N, int C, size_t n,
+                                  float slope, void *stream);
+int casmvs_abn8_backward_apply_f32(const float *grad_y, const void *codes, const void *scales, const void *signs, const double *sums, int blocks,
+                                   double count, const float *weight, float abs_eps, const float *vec, float *grad_weight, float *grad_bias, float *grad_x,
+                                   int N, int C, size_t n, float slope, void *stream);
+
+/* Softmax cross entropy over the depth hypotheses: cost (B, D, h*w) of `dtype`, depth_values (B, D, h*w) (per_pixel) or (B, D), depth_gt (B, h*w), mask (B, h*w)
+ * bytes or NULL.  The class of a pixel is the hypothesis nearest to depth_gt (the lowest index on ties); a pixel counts if its mask is not 0, depth_gt
+ * lies inside [min, max] of its hypotheses and some cost is above -inf.  loss = mean over the counted pixels of -log softmax(cost)[class], share = 1 / count
+ * (one float each); both 0 where no pixel counts.  stats (B, h*w, 2) floats (8-byte aligned), target (B, h*w): what the backward pass takes beside cost.
+ * grad_loss: one device float; grad_cost has cost's type, 0 at every pixel that does not count.  workspace: casmvs_depth_ce_workspace_bytes. */
+size_t casmvs_depth_ce_workspace_bytes(int B, int D, size_t hw);
+int casmvs_depth_ce_forward(const void *cost, const float *depth_values, const float *depth_gt, const void *mask, float *stats, int *target, float *loss,
+                            float *share, void *workspace, int dtype, int B, int D, size_t hw, int per_pixel, void *stream);
+int casmvs_depth_ce_backward(const void *cost, const float *stats, const int *target, const float *share, const float *grad_loss, void *grad_cost, int dtype,
+                             int B, int D, size_t hw, void *stream);
 
 /* ---- self test ------------------------------------------------------------------------------
  * Runs the MFMA lane-mapping probes the conv kernels rely on (v_mfma_f32_16x16x4_f32 operand /
