@@ -141,10 +141,9 @@ SYMBOLS = {
     "casmvs_layer_norm_backward": (c_int, [c_void_p, c_void_p, _FP, _FP, c_void_p, _FP, _FP, c_void_p, c_int, c_size_t, c_int, c_size_t, c_float, c_float, c_void_p]),
     "casmvs_pack8": (c_int, [c_void_p, c_int, c_size_t, c_size_t, c_void_p, c_void_p, c_void_p]),
     "casmvs_unpack8": (c_int, [c_void_p, c_void_p, _FP, _FP, c_int, c_float, c_void_p, c_int, c_size_t, c_size_t, c_void_p]),
-    "casmvs_abn8_train_apply_f32": (c_int, [_FP, _FP, c_int, c_double, _FP, _FP, c_float, c_float, c_float] + [_FP] * 4 + [c_void_p] * 3 + [c_int, c_int, c_size_t, c_float, c_void_p]),
-    "casmvs_abn8_backward_sums_blocks": (c_int, [c_int, c_size_t]),
-    "casmvs_abn8_backward_sums_f64": (c_int, [_FP] + [c_void_p] * 3 + [_FP, c_int, c_int, c_size_t, c_float, c_void_p]),
-    "casmvs_abn8_backward_apply_f32": (c_int, [_FP] + [c_void_p] * 3 + [_FP, c_int, c_double, _FP, c_float] + [_FP] * 4 + [c_int, c_int, c_size_t, c_float, c_void_p]),
+    "casmvs_abn8_workspace_bytes": (c_size_t, [c_int, c_int, c_size_t]),
+    "casmvs_abn8_forward_f32": (c_int, [_FP] * 3 + [c_float] * 3 + [_FP] * 4 + [c_void_p] * 4 + [c_int, c_int, c_size_t, c_float, c_void_p]),
+    "casmvs_abn8_backward_f32": (c_int, [_FP] + [c_void_p] * 3 + [_FP, c_float] + [_FP] * 4 + [c_void_p, c_int, c_int, c_size_t, c_float, c_void_p]),
     "casmvs_depth_ce_workspace_bytes": (c_size_t, [c_int, c_int, c_size_t]),
     "casmvs_depth_ce_forward": (c_int, [c_void_p] + [_FP] * 2 + [c_void_p] + [_FP] * 4 + [c_void_p, c_int, c_int, c_int, c_size_t, c_int, c_void_p]),
     "casmvs_depth_ce_backward": (c_int, [c_void_p] + [_FP] * 4 + [c_void_p, c_int, c_int, c_int, c_size_t, c_void_p]),

@@ -20,6 +20,7 @@ Two more that a training step uses and the reference does not have:
       SmoothL1 on softmax_depth_regression; gradient w.r.t. the cost volume.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -95,6 +96,17 @@ def softmax_depth_regression(cost, depth_values):
     return _SoftmaxDepthRegression.apply(cost, depth_values)
 
 
+def _once(backward):
+    """A backward pass that has no second derivative: torch's once_differentiable where a graph is being built (create_graph), which makes a second derivative raise;
+    without a graph there is nothing to guard, and the guard's no_grad context is skipped (5 us of a call)."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def either(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return either
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, slope, channels_last):
@@ -104,7 +116,7 @@ class _LayerNorm(torch.autograd.Function):
         return ops.layer_norm(x, weight, bias, eps, slope, channels_last)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, gy):
         x, weight, bias = ctx.saved_tensors
         gx, gw, gb = ops.layer_norm_backward(x, gy, weight, bias, *ctx.args, need_x=ctx.needs_input_grad[0],
@@ -136,29 +148,30 @@ class _DepthCrossEntropy(torch.autograd.Function):
             mask = ops._same_device(cost, mask, "mask").contiguous()
         if B * D == 0:
             raise ValueError(f"depth_cross_entropy: cost {tuple(cost.shape)} has no hypotheses")
-        lib, code = _lib.load(), ops._DTYPES[cost.dtype]
+        lib, code, pixels = _lib.load(), ops._DTYPES[cost.dtype], B * h * w
         loss = torch.empty((), dtype=torch.float32, device=cost.device)
-        # per pixel the running maximum and 1 / sum; behind them 1 / count
-        stats = torch.empty(2 * B * h * w + 1, dtype=torch.float32, device=cost.device)
-        target = torch.empty((B, h, w), dtype=torch.int32, device=cost.device)
-        ws = torch.empty(lib.casmvs_depth_ce_workspace_bytes(B, D, h * w), dtype=torch.uint8, device=cost.device)
-        with torch.cuda.device(cost.device):
-            rc = lib.casmvs_depth_ce_forward(_ptr(cost), _ptr(depth_values), _ptr(depth_gt), None if mask is None else _ptr(mask), _ptr(stats), _ptr(target),
-                                             _ptr(loss), _ptr(stats[-1:]), _ptr(ws), code, B, D, h * w, int(depth_values.dim() == 4), _stream(cost))
+        # one buffer: per pixel the running maximum and 1 / sum (two floats) and the class (an int), 1 / count, and (8-byte aligned) the forward's workspace
+        at_target, at_share = 8 * pixels, 12 * pixels
+        at_ws = at_share + 4 + (at_share + 4) % 8
+        kept = torch.empty(at_ws + ops._workspace_bytes("casmvs_depth_ce_workspace_bytes", B, D, h * w), dtype=torch.uint8, device=cost.device)
+        base = kept.data_ptr()
+        with ops._on(cost):
+            rc = lib.casmvs_depth_ce_forward(cost.data_ptr(), depth_values.data_ptr(), depth_gt.data_ptr(), ops._at(mask), base, base + at_target, loss.data_ptr(),
+                                             base + at_share, base + at_ws, code, B, D, h * w, int(depth_values.dim() == 4), _stream(cost))
         _lib.check(rc, "casmvs_depth_ce_forward")
-        ctx.save_for_backward(cost, stats, target)
+        ctx.save_for_backward(cost, kept)
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, gloss):
-        cost, stats, target = ctx.saved_tensors
+        cost, kept = ctx.saved_tensors
         B, D, h, w = cost.shape
-        gloss = gloss.contiguous().float()
         gcost = torch.empty_like(cost)
-        with torch.cuda.device(cost.device):
-            rc = _lib.load().casmvs_depth_ce_backward(_ptr(cost), _ptr(stats), _ptr(target), _ptr(stats[-1:]), _ptr(gloss), _ptr(gcost), ops._DTYPES[cost.dtype],
-                                                      B, D, h * w, _stream(cost))
+        base, pixels = kept.data_ptr(), B * h * w
+        with ops._on(cost):
+            rc = _lib.load().casmvs_depth_ce_backward(cost.data_ptr(), base, base + 8 * pixels, base + 12 * pixels, gloss.contiguous().data_ptr(), gcost.data_ptr(),
+                                                      ops._DTYPES[cost.dtype], B, D, h * w, _stream(cost))
         _lib.check(rc, "casmvs_depth_ce_backward")
         return gcost, None, None, None
 

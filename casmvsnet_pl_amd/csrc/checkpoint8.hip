@@ -5,9 +5,8 @@
 //   backward   g = gy (s ? 1 : slope),  gbeta = sum g,  ggamma = sum g Q,  gx = gamma rstd (g - gbeta / M - Q ggamma / M)
 //
 // xhat enters the gradient through ggamma and its product with Q only (both averages over the channel), so its 8 bits cost little there; the side of zero
-// multiplies every gradient element, so it is kept exactly.  xhat and z are computed in 64 bits from the 64-bit statistics: a block's codes and the sign of z
-// are the ones of the definition, not of one order of float32 roundings.  y itself is the float32 fma of casmvs_abn_train_apply_f32, bit for bit, so
-// choosing the 8-bit checkpoint leaves a forward pass as it was.
+// multiplies every gradient element, so it is kept exactly.  The statistics, xhat and z are computed in 64 bits: a block's codes and the sign of z are the
+// ones of the definition, not of one order of float32 roundings.  y itself is the float32 fma of casmvs_abn_train_apply_f32.
 //
 // Everything here waits for memory: forward 4 + 4 + 33/32 + 1/8 bytes per element, backward sums 4 + 37/32, apply 8 + 37/32 (keeping x and y in
 // float32 reads 12 and 12 and writes 4).
@@ -107,14 +106,13 @@ __global__ __launch_bounds__(kThreads) void unpack8_kernel(const unsigned *__res
 }
 
 // ---- train-mode ABN -------------------------------------------------------------------------------------------------------------------------------------
-// The channel's two totals from the partial sums (C, blocks, 2), in every workgroup: one value per thread and a fixed-order tree.
-__device__ __forceinline__ void channel_totals(const double *__restrict__ sums, int blocks, int c, double &t0, double &t1) {
+// The sums over a channel are formed by kParts workgroups at most, each over its share [lo, hi) of every plane of the channel, and added up by every workgroup
+// of the pass behind: one partial sum per lane of a wave, in a fixed order.
+constexpr int kParts = 64;
+
+// sums of a workgroup's two values per thread, to thread 0
+__device__ __forceinline__ void workgroup_sums(double &s0, double &s1) {
   __shared__ double red[2][kThreads];
-  double s0 = 0.0, s1 = 0.0;
-  for (int b = threadIdx.x; b < blocks; b += kThreads) {
-    s0 += sums[((size_t)c * blocks + b) * 2];
-    s1 += sums[((size_t)c * blocks + b) * 2 + 1];
-  }
   red[0][threadIdx.x] = s0;
   red[1][threadIdx.x] = s1;
   __syncthreads();
@@ -125,30 +123,78 @@ __device__ __forceinline__ void channel_totals(const double *__restrict__ sums, 
     }
     __syncthreads();
   }
-  t0 = red[0][0];
-  t1 = red[1][0];
+  s0 = red[0][0];
+  s1 = red[1][0];
+}
+
+// The channel's two totals from its partial sums (C, parts, 2), parts <= 64, in every wave.
+__device__ __forceinline__ void channel_totals(const double *__restrict__ sums, int parts, int c, double &t0, double &t1) {
+  const int lane = threadIdx.x & 63;
+  t0 = lane < parts ? sums[((size_t)c * parts + lane) * 2] : 0.0;
+  t1 = lane < parts ? sums[((size_t)c * parts + lane) * 2 + 1] : 0.0;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    t0 += casmvs::elem::lane_xor(t0, d);
+    t1 += casmvs::elem::lane_xor(t1, d);
+  }
+}
+
+// sum x and sum x^2 of channel blockIdx.y, in 64 bits from the first addition on (x^2 is exact there): xhat's codes and the side of zero hang on the mean
+template <bool WIDE>
+__global__ __launch_bounds__(kThreads) void abn8_sums_kernel(const float *__restrict__ x, double *__restrict__ out, int N, int C, size_t n) {
+  const int c = blockIdx.y;
+  const size_t words = (n + 3) / 4, per = (words + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < words ? lo + per : words;
+  double s0 = 0.0, s1 = 0.0;
+  for (int img = 0; img < N; ++img) {
+    const float *xp = x + ((size_t)img * C + c) * n;
+    for (size_t e = lo + threadIdx.x; e < hi; e += 4 * kThreads) {
+      float v[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {   // four loads in flight
+        const size_t at = e + (size_t)k * kThreads;
+        load4<float, WIDE>(xp + 4 * at, at < hi ? left_of(n, 4 * at) : 0, v[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const double d = v[k][i];
+          s0 += d;
+          s1 = fma(d, d, s1);
+        }
+    }
+  }
+  workgroup_sums(s0, s1);
+  if (threadIdx.x == 0) {
+    out[((size_t)c * gridDim.x + blockIdx.x) * 2] = s0;
+    out[((size_t)c * gridDim.x + blockIdx.x) * 2 + 1] = s1;
+  }
 }
 
 constexpr int kTurns = 8;   // blocks per group of eight lanes and workgroup: 256 x 32 = 8192 elements share one read of the channel's partial sums
+constexpr int kAhead = 4;   // turns whose loads are issued together
 
 // blockIdx.x = (plane, chunk of kTurns * kGroups blocks); vec (4, C): scale = gamma rstd, shift, gamma, beta of the forward pass
 template <bool WIDE>
-__global__ __launch_bounds__(kThreads) void abn8_apply_kernel(const float *__restrict__ x, const double *__restrict__ sums, int blocks, double M,
+__global__ __launch_bounds__(kThreads) void abn8_apply_kernel(const float *__restrict__ x, const double *__restrict__ sums, int parts, double M,
                                                              const float *__restrict__ weight, const float *__restrict__ bias, float abs_eps, float eps,
                                                              float momentum, float *__restrict__ rmean, float *__restrict__ rvar, float *__restrict__ vec,
                                                              float *__restrict__ y, unsigned *__restrict__ codes, unsigned char *__restrict__ scales,
                                                              unsigned *__restrict__ signs, int C, size_t n, size_t nb, unsigned chunks, float slope) {
-  const size_t plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-  const int c = (int)(plane % C);
+  const unsigned plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const int c = (int)(plane % C), lane = threadIdx.x & (kLanes - 1);
+  const float *xp = x + plane * n;
+  float *yp = y + plane * n;
+  const size_t base = plane * nb;
   double s0, s1;
-  channel_totals(sums, blocks, c, s0, s1);
+  channel_totals(sums, parts, c, s0, s1);
   const double mu = s0 / M;
   double var = s1 / M - mu * mu;   // biased
   var = var > 0.0 ? var : 0.0;
   const double rs = 1.0 / sqrt(var + (double)eps);
   const float gamma = abs_eps >= 0.0f ? fabsf(weight[c]) + abs_eps : weight[c], beta = bias[c];
   const float a = (float)((double)gamma * rs), bq = (float)((double)beta - mu * (double)gamma * rs);
-  if (chunk == 0 && plane == (size_t)c && threadIdx.x == 0) {
+  if (chunk == 0 && plane == (unsigned)c && threadIdx.x == 0) {
     vec[c] = a;
     vec[C + c] = bq;
     vec[2 * C + c] = gamma;
@@ -159,39 +205,60 @@ __global__ __launch_bounds__(kThreads) void abn8_apply_kernel(const float *__res
       rvar[c] = rvar[c] * keep + momentum * (float)(var * (M / (M > 1.0 ? M - 1.0 : 1.0)));
     }
   }
-  const int lane = threadIdx.x & (kLanes - 1);
-  const float *xp = x + plane * n;
-  float *yp = y + plane * n;
-#pragma unroll 2
-  for (int turn = 0; turn < kTurns; ++turn) {
-    const size_t blk = (chunk * kTurns + turn) * kGroups + threadIdx.x / kLanes, first = blk * kBlock + 4 * lane;
-    const int left = left_of(n, first);   // 0 past the plane's last block
-    float v[4], o[4];
-    load4<float, WIDE>(xp + first, left, v);
-    double h[4];
-    unsigned up = 0;
+  for (int ahead = 0; ahead < kTurns; ahead += kAhead) {
+    float v[kAhead][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      h[i] = i < left ? ((double)v[i] - mu) * rs : 0.0;
-      up |= (h[i] * (double)gamma + (double)beta > 0.0 ? 1u : 0u) << i;
-      const float t = fmaf(v[i], a, bq);
-      o[i] = t > 0.0f ? t : t * slope;
+    for (int k = 0; k < kAhead; ++k) {
+      const size_t first = (((size_t)chunk * kTurns + ahead + k) * kGroups + threadIdx.x / kLanes) * kBlock + 4 * lane;
+      load4<float, WIDE>(xp + first, left_of(n, first), v[k]);   // 0 past the plane's last block
     }
-    unsigned scale;
-    const unsigned q = casmvs::block8::quantise(h, scale);
-    const unsigned sign = casmvs::block8::over_block(up << (4 * lane), [](unsigned p, unsigned r) { return p | r; });
-    store4<float, WIDE>(yp + first, left, o);
-    if (blk < nb) {
-      codes[(plane * nb + blk) * kLanes + lane] = q;
-      if (lane == 0) {
-        scales[plane * nb + blk] = (unsigned char)scale;
-        signs[plane * nb + blk] = sign;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const size_t blk = ((size_t)chunk * kTurns + ahead + k) * kGroups + threadIdx.x / kLanes, first = blk * kBlock + 4 * lane;
+      const int left = left_of(n, first);
+      float o[4];
+      double h[4];
+      unsigned up = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        h[i] = i < left ? ((double)v[k][i] - mu) * rs : 0.0;
+        up |= (fma(h[i], (double)gamma, (double)beta) > 0.0 ? 1u : 0u) << i;
+        const float t = fmaf(v[k][i], a, bq);
+        o[i] = t > 0.0f ? t : t * slope;
+      }
+      unsigned scale;
+      const unsigned q = casmvs::block8::quantise(h, scale);
+      const unsigned sign = casmvs::block8::over_block(up << (4 * lane), [](unsigned p, unsigned r) { return p | r; });
+      store4<float, WIDE>(yp + first, left, o);
+      if (blk < nb) {
+        codes[(base + blk) * kLanes + lane] = q;
+        if (lane == 0) {
+          scales[base + blk] = (unsigned char)scale;
+          signs[base + blk] = sign;
+        }
       }
     }
   }
 }
 
-// out (C, blocks, 2): this workgroup's part of sum g and sum g Q of channel blockIdx.y; blockIdx.x owns the blocks [lo, hi) of every plane of the channel
+// What the backward pass reads of four values: their gradient behind the activation and Q
+struct Kept {
+  float g[4];
+  unsigned q, up;
+  float step;
+};
+template <bool WIDE>
+__device__ __forceinline__ void load_kept(const float *__restrict__ gy, const unsigned *__restrict__ codes, const unsigned char *__restrict__ scales,
+                                          const unsigned *__restrict__ signs, size_t plane, size_t blk, size_t n, size_t nb, int lane, Kept &k) {
+  const size_t first = blk * kBlock + 4 * lane, at = plane * nb + (blk < nb ? blk : 0);
+  load4<float, WIDE>(gy + plane * n + first, left_of(n, first), k.g);   // 0 past the plane's last block
+  k.q = codes[at * kLanes + lane];
+  k.up = signs[at] >> (4 * lane);
+  k.step = casmvs::block8::step_of(scales[at]);
+}
+__device__ __forceinline__ float behind_activation(const Kept &k, int i, float slope) { return k.g[i] * ((k.up >> i) & 1u ? 1.0f : slope); }
+
+// this workgroup's part of sum g and sum g Q of channel blockIdx.y
 template <bool WIDE>
 __global__ __launch_bounds__(kThreads) void abn8_backward_sums_kernel(const float *__restrict__ gy, const unsigned *__restrict__ codes,
                                                                      const unsigned char *__restrict__ scales, const unsigned *__restrict__ signs,
@@ -201,81 +268,75 @@ __global__ __launch_bounds__(kThreads) void abn8_backward_sums_kernel(const floa
   double s0 = 0.0, s1 = 0.0;
   for (int img = 0; img < N; ++img) {
     const size_t plane = (size_t)img * C + c;
-    for (size_t blk = lo + threadIdx.x / kLanes; blk < hi; blk += kGroups) {
-      const size_t first = blk * kBlock + 4 * lane, at = plane * nb + blk;
-      float v[4];
-      load4<float, WIDE>(gy + plane * n + first, left_of(n, first), v);
-      const unsigned q = codes[at * kLanes + lane], up = signs[at] >> (4 * lane);
-      const float step = casmvs::block8::step_of(scales[at]);
-      float p0 = 0.0f, p1 = 0.0f;   // four values in float32, then 64 bits
+    for (size_t blk = lo + threadIdx.x / kLanes; blk < hi; blk += kAhead * kGroups) {
+      Kept k[kAhead];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float g = v[i] * ((up >> i) & 1u ? 1.0f : slope);
-        p0 += g;
-        p1 = fmaf(g, casmvs::block8::value_of(q, i, step), p1);
+      for (int j = 0; j < kAhead; ++j) {
+        const size_t at = blk + (size_t)j * kGroups;
+        load_kept<WIDE>(gy, codes, scales, signs, plane, at < hi ? at : nb, n, nb, lane, k[j]);
       }
-      s0 += p0;
-      s1 += p1;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (blk + (size_t)j * kGroups >= hi) break;
+        float p0 = 0.0f, p1 = 0.0f;   // four values in float32, then 64 bits
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float g = behind_activation(k[j], i, slope);
+          p0 += g;
+          p1 = fmaf(g, casmvs::block8::value_of(k[j].q, i, k[j].step), p1);
+        }
+        s0 += p0;
+        s1 += p1;
+      }
     }
   }
-  __shared__ double red[2][kThreads];
-  red[0][threadIdx.x] = s0;
-  red[1][threadIdx.x] = s1;
-  __syncthreads();
-  for (int st = kThreads / 2; st > 0; st >>= 1) {
-    if ((int)threadIdx.x < st) {
-      red[0][threadIdx.x] += red[0][threadIdx.x + st];
-      red[1][threadIdx.x] += red[1][threadIdx.x + st];
-    }
-    __syncthreads();
-  }
+  workgroup_sums(s0, s1);
   if (threadIdx.x == 0) {
-    out[((size_t)c * gridDim.x + blockIdx.x) * 2] = red[0][0];
-    out[((size_t)c * gridDim.x + blockIdx.x) * 2 + 1] = red[1][0];
+    out[((size_t)c * gridDim.x + blockIdx.x) * 2] = s0;
+    out[((size_t)c * gridDim.x + blockIdx.x) * 2 + 1] = s1;
   }
 }
 
 template <bool WIDE>
 __global__ __launch_bounds__(kThreads) void abn8_backward_apply_kernel(const float *__restrict__ gy, const unsigned *__restrict__ codes,
                                                                       const unsigned char *__restrict__ scales, const unsigned *__restrict__ signs,
-                                                                      const double *__restrict__ sums, int blocks, double M, const float *__restrict__ weight,
+                                                                      const double *__restrict__ sums, int parts, double M, const float *__restrict__ weight,
                                                                       float abs_eps, const float *__restrict__ vec, float *__restrict__ gweight,
                                                                       float *__restrict__ gbias, float *__restrict__ gx, int C, size_t n, size_t nb,
                                                                       unsigned chunks, float slope) {
-  const size_t plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-  const int c = (int)(plane % C);
+  const unsigned plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const int c = (int)(plane % C), lane = threadIdx.x & (kLanes - 1);
   double s0, s1;
-  channel_totals(sums, blocks, c, s0, s1);
+  channel_totals(sums, parts, c, s0, s1);
   const float m1 = (float)(s0 / M), m2 = (float)(s1 / M), a = vec[c];
-  if (chunk == 0 && plane == (size_t)c && threadIdx.x == 0) {
+  if (chunk == 0 && plane == (unsigned)c && threadIdx.x == 0) {
     const float w = weight[c];
     const float sgn = abs_eps >= 0.0f ? (w > 0.0f ? 1.0f : (w < 0.0f ? -1.0f : 0.0f)) : 1.0f;   // d|w| / dw
     gweight[c] = (float)s1 * sgn;
     gbias[c] = (float)s0;
   }
   if (!gx) return;
-  const int lane = threadIdx.x & (kLanes - 1);
-#pragma unroll 2
-  for (int turn = 0; turn < kTurns; ++turn) {
-    const size_t blk = (chunk * kTurns + turn) * kGroups + threadIdx.x / kLanes, first = blk * kBlock + 4 * lane, at = plane * nb + blk;
-    if (blk >= nb) break;
-    const int left = left_of(n, first);
-    float v[4];
-    load4<float, WIDE>(gy + plane * n + first, left, v);
-    const unsigned q = codes[at * kLanes + lane], up = signs[at] >> (4 * lane);
-    const float step = casmvs::block8::step_of(scales[at]);
+  for (int ahead = 0; ahead < kTurns; ahead += kAhead) {
+    const size_t blk = ((size_t)chunk * kTurns + ahead) * kGroups + threadIdx.x / kLanes;
+    Kept k[kAhead];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float g = v[i] * ((up >> i) & 1u ? 1.0f : slope);
-      v[i] = a * (g - m1 - casmvs::block8::value_of(q, i, step) * m2);
+    for (int j = 0; j < kAhead; ++j) load_kept<WIDE>(gy, codes, scales, signs, plane, blk + (size_t)j * kGroups, n, nb, lane, k[j]);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const size_t first = (blk + (size_t)j * kGroups) * kBlock + 4 * lane;
+      float o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = a * (behind_activation(k[j], i, slope) - m1 - casmvs::block8::value_of(k[j].q, i, k[j].step) * m2);
+      store4<float, WIDE>(gx + plane * n + first, left_of(n, first), o);
     }
-    store4<float, WIDE>(gx + plane * n + first, left, v);
   }
 }
 
-int sums_blocks(int N, size_t n) {
-  const size_t blocks = ((size_t)N * n + kThreads * 64 - 1) / (kThreads * 64);
-  return (int)(blocks < 1 ? 1 : blocks > 256 ? 256 : blocks);
+// Workgroups that form a channel's sums: at least 4096 elements each, at most 1024 workgroups in all (four per CU)
+int parts_of(int N, int C, size_t n) {
+  const size_t most = 1024 / (size_t)C < 1 ? 1 : 1024 / (size_t)C, wanted = ((size_t)N * n + 4095) / 4096;
+  const size_t parts = wanted < most ? wanted : most;
+  return (int)(parts < 1 ? 1 : parts > kParts ? kParts : parts);
 }
 size_t blocks_of(size_t n) { return (n + kBlock - 1) / kBlock; }
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -337,48 +398,52 @@ extern "C" int casmvs_unpack8(const void *codes, const void *scales, const float
   return casmvs::check_launch("unpack8_kernel");
 }
 
-extern "C" int casmvs_abn8_train_apply_f32(const float *x, const double *sums, int blocks, double count, const float *weight, const float *bias,
-                                           float abs_eps, float eps, float momentum, float *running_mean, float *running_var, float *vec, float *y,
-                                           void *codes, void *scales, void *signs, int N, int C, size_t n, float slope, void *stream) {
-  casmvs::clear_error();
-  if (int rc = check_planes("abn8_train_apply", N, C, n)) return rc;
-  CASMVS_REQUIRE(x && sums && weight && bias && vec && y && codes && scales && signs && blocks > 0 && count > 0.0, "abn8_train_apply: bad arguments");
-  CASMVS_REQUIRE((running_mean == nullptr) == (running_var == nullptr), "abn8_train_apply: running_mean and running_var go together");
-  CASMVS_REQUIRE((((uintptr_t)codes | (uintptr_t)signs) & 3) == 0, "abn8_train_apply: codes and signs are written as 4-byte words");
-  const size_t nb = blocks_of(n), chunks = (nb + kTurns * kGroups - 1) / (kTurns * kGroups);
-  const dim3 grid((unsigned)((size_t)N * C * chunks));
-  auto kernel = n % 4 == 0 && aligned16(x) && aligned16(y) ? abn8_apply_kernel<true> : abn8_apply_kernel<false>;
-  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, (hipStream_t)stream, x, sums, blocks, count, weight, bias, abs_eps, eps, momentum, running_mean,
-                     running_var, vec, y, (unsigned *)codes, (unsigned char *)scales, (unsigned *)signs, C, n, nb, (unsigned)chunks, slope);
-  return casmvs::check_launch("abn8_apply_kernel");
+extern "C" size_t casmvs_abn8_workspace_bytes(int N, int C, size_t n) {
+  if (N <= 0 || C <= 0 || n == 0) return 0;
+  return (size_t)C * parts_of(N, C, n) * 2 * sizeof(double);
 }
 
-extern "C" int casmvs_abn8_backward_sums_blocks(int N, size_t n) { return sums_blocks(N, n); }
-
-extern "C" int casmvs_abn8_backward_sums_f64(const float *grad_y, const void *codes, const void *scales, const void *signs, double *sums, int N, int C, size_t n,
-                                             float slope, void *stream) {
+extern "C" int casmvs_abn8_forward_f32(const float *x, const float *weight, const float *bias, float abs_eps, float eps, float momentum, float *running_mean,
+                                       float *running_var, float *vec, float *y, void *codes, void *scales, void *signs, void *workspace, int N, int C,
+                                       size_t n, float slope, void *stream) {
   casmvs::clear_error();
-  if (int rc = check_planes("abn8_backward_sums", N, C, n)) return rc;
-  CASMVS_REQUIRE(grad_y && codes && scales && signs && sums, "abn8_backward_sums: null pointer");
-  CASMVS_REQUIRE((((uintptr_t)codes | (uintptr_t)signs) & 3) == 0, "abn8_backward_sums: codes and signs are read as 4-byte words");
-  auto kernel = n % 4 == 0 && aligned16(grad_y) ? abn8_backward_sums_kernel<true> : abn8_backward_sums_kernel<false>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)sums_blocks(N, n), (unsigned)C), dim3(kThreads), 0, (hipStream_t)stream, grad_y, (const unsigned *)codes,
-                     (const unsigned char *)scales, (const unsigned *)signs, sums, N, C, n, blocks_of(n), slope);
-  return casmvs::check_launch("abn8_backward_sums_kernel");
+  if (int rc = check_planes("abn8_forward", N, C, n)) return rc;
+  CASMVS_REQUIRE(x && weight && bias && vec && y && codes && scales && signs && workspace, "abn8_forward: null pointer");
+  CASMVS_REQUIRE((running_mean == nullptr) == (running_var == nullptr), "abn8_forward: running_mean and running_var go together");
+  CASMVS_REQUIRE((((uintptr_t)codes | (uintptr_t)signs) & 3) == 0 && ((uintptr_t)workspace & 7) == 0,
+                 "abn8_forward: codes and signs are 4-byte words, the workspace 8-byte ones");
+  const size_t nb = blocks_of(n), chunks = (nb + kTurns * kGroups - 1) / (kTurns * kGroups);
+  const int parts = parts_of(N, C, n);
+  double *sums = (double *)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  const bool wide = n % 4 == 0 && aligned16(x) && aligned16(y);
+  hipLaunchKernelGGL(wide ? abn8_sums_kernel<true> : abn8_sums_kernel<false>, dim3((unsigned)parts, (unsigned)C), dim3(kThreads), 0, st, x, sums, N, C, n);
+  hipLaunchKernelGGL(wide ? abn8_apply_kernel<true> : abn8_apply_kernel<false>, dim3((unsigned)((size_t)N * C * chunks)), dim3(kThreads), 0, st, x, sums, parts,
+                     (double)N * (double)n, weight, bias, abs_eps, eps, momentum, running_mean, running_var, vec, y, (unsigned *)codes, (unsigned char *)scales,
+                     (unsigned *)signs, C, n, nb, (unsigned)chunks, slope);
+  return casmvs::check_launch("abn8_forward");
 }
 
-extern "C" int casmvs_abn8_backward_apply_f32(const float *grad_y, const void *codes, const void *scales, const void *signs, const double *sums, int blocks,
-                                              double count, const float *weight, float abs_eps, const float *vec, float *grad_weight, float *grad_bias,
-                                              float *grad_x, int N, int C, size_t n, float slope, void *stream) {
+extern "C" int casmvs_abn8_backward_f32(const float *grad_y, const void *codes, const void *scales, const void *signs, const float *weight, float abs_eps,
+                                        const float *vec, float *grad_weight, float *grad_bias, float *grad_x, void *workspace, int N, int C, size_t n,
+                                        float slope, void *stream) {
   casmvs::clear_error();
-  if (int rc = check_planes("abn8_backward_apply", N, C, n)) return rc;
-  CASMVS_REQUIRE(grad_y && codes && scales && signs && sums && weight && vec && grad_weight && grad_bias && blocks > 0 && count > 0.0,
-                 "abn8_backward_apply: bad arguments");
-  CASMVS_REQUIRE((((uintptr_t)codes | (uintptr_t)signs) & 3) == 0, "abn8_backward_apply: codes and signs are read as 4-byte words");
+  if (int rc = check_planes("abn8_backward", N, C, n)) return rc;
+  CASMVS_REQUIRE(grad_y && codes && scales && signs && weight && vec && grad_weight && grad_bias && workspace, "abn8_backward: null pointer");
+  CASMVS_REQUIRE((((uintptr_t)codes | (uintptr_t)signs) & 3) == 0 && ((uintptr_t)workspace & 7) == 0,
+                 "abn8_backward: codes and signs are 4-byte words, the workspace 8-byte ones");
   const size_t nb = blocks_of(n), chunks = (nb + kTurns * kGroups - 1) / (kTurns * kGroups);
-  const dim3 grid((unsigned)((size_t)N * C * chunks));
-  auto kernel = n % 4 == 0 && aligned16(grad_y) && (!grad_x || aligned16(grad_x)) ? abn8_backward_apply_kernel<true> : abn8_backward_apply_kernel<false>;
-  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, (hipStream_t)stream, grad_y, (const unsigned *)codes, (const unsigned char *)scales,
-                     (const unsigned *)signs, sums, blocks, count, weight, abs_eps, vec, grad_weight, grad_bias, grad_x, C, n, nb, (unsigned)chunks, slope);
-  return casmvs::check_launch("abn8_backward_apply_kernel");
+  const int parts = parts_of(N, C, n);
+  double *sums = (double *)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  const unsigned *cp = (const unsigned *)codes, *up = (const unsigned *)signs;
+  const unsigned char *sp = (const unsigned char *)scales;
+  const bool wide = n % 4 == 0 && aligned16(grad_y) && aligned16(grad_x);
+  hipLaunchKernelGGL(wide ? abn8_backward_sums_kernel<true> : abn8_backward_sums_kernel<false>, dim3((unsigned)parts, (unsigned)C), dim3(kThreads), 0, st, grad_y, cp,
+                     sp, up, sums, N, C, n, nb, slope);
+  // (without grad_x the workgroups of the channels' first chunks write the two vectors, and there are no others)
+  const dim3 grid((unsigned)(grad_x ? (size_t)N * C * chunks : (size_t)C * chunks));
+  hipLaunchKernelGGL(wide ? abn8_backward_apply_kernel<true> : abn8_backward_apply_kernel<false>, grid, dim3(kThreads), 0, st, grad_y, cp, sp, up, sums, parts,
+                     (double)N * (double)n, weight, abs_eps, vec, grad_weight, grad_bias, grad_x, C, n, nb, (unsigned)chunks, slope);
+  return casmvs::check_launch("abn8_backward");
 }

@@ -25,6 +25,25 @@ __device__ __forceinline__ void store(T *p, const Vec<T, V> &v) {
   *reinterpret_cast<Vec<T, V> *>(p) = v;
 }
 
+// The value of lane (own ^ d), d = 1, 2, 4 .. 32: inside a row of 16 lanes by data-parallel moves (quad permutes; 4 and 8 after the smaller steps of a sum, where
+// the mirror of 8 / 16 lanes holds the same value), beyond by the LDS crossbar.  For sums over lanes in the order 1, 2, 4, ..; all lanes active.
+__device__ __forceinline__ double lane_xor(double v, int d) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  int lo = (int)(unsigned)u, hi = (int)(unsigned)(u >> 32);
+  switch (d) {
+    case 1: lo = __builtin_amdgcn_update_dpp(0, lo, 0xB1, 0xF, 0xF, false); hi = __builtin_amdgcn_update_dpp(0, hi, 0xB1, 0xF, 0xF, false); break;
+    case 2: lo = __builtin_amdgcn_update_dpp(0, lo, 0x4E, 0xF, 0xF, false); hi = __builtin_amdgcn_update_dpp(0, hi, 0x4E, 0xF, 0xF, false); break;
+    case 4: lo = __builtin_amdgcn_update_dpp(0, lo, 0x141, 0xF, 0xF, false); hi = __builtin_amdgcn_update_dpp(0, hi, 0x141, 0xF, 0xF, false); break;
+    case 8: lo = __builtin_amdgcn_update_dpp(0, lo, 0x140, 0xF, 0xF, false); hi = __builtin_amdgcn_update_dpp(0, hi, 0x140, 0xF, 0xF, false); break;
+    default: {
+      const int from = (int)((threadIdx.x & 63) ^ d) * 4;
+      lo = __builtin_amdgcn_ds_bpermute(from, lo);
+      hi = __builtin_amdgcn_ds_bpermute(from, hi);
+    }
+  }
+  return __builtin_bit_cast(double, (unsigned long long)(unsigned)hi << 32 | (unsigned)lo);
+}
+
 }  // namespace elem
 }  // namespace casmvs
 

@@ -3,7 +3,9 @@ and the current HIP stream; every op below is one call into libcasmvs_hip.so.
 
 All inputs must be float32 tensors on a ROCm device ("cuda" in torch); nothing here runs on CPU.
 """
+import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -907,6 +909,8 @@ def selftest_mfma_rate(shape=1, blocks=2048, iters=4096):
 
 
 # ---- training-side operators: layer norm, 8-bit activation checkpoints, cross entropy over depth hypotheses ---------------------------------------------------
+# These are called on small tensors too, where the host's part of a call is all that counts: addresses go to the library as plain integers, the device is switched
+# only where it is not the current one, and a shape's workspace is asked for once.
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 
 
@@ -920,6 +924,23 @@ def _float_dev(t, name):
     if t.dtype not in _DTYPES:
         raise TypeError(f"{name}: expected float32, float16 or bfloat16, got {t.dtype}")
     return t.contiguous()
+
+
+_STAY = contextlib.nullcontext()
+
+
+def _on(t):
+    """The context in which t's device is the current one."""
+    return _STAY if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(name, *shape):
+    return getattr(_lib.load(), name)(*shape)
 
 
 def _same_device(ref, t, name):
@@ -959,8 +980,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, slope=1.0, channels_last=Fal
     No autograd graph: autograd.layer_norm is the differentiable form."""
     x, weight, bias, outer, C, inner = _layer_norm_args(x, weight, bias, eps, slope, channels_last)
     y = torch.empty_like(x)
-    with torch.cuda.device(x.device):
-        rc = _lib.load().casmvs_layer_norm_forward(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _DTYPES[x.dtype], outer, C, inner, float(eps), float(slope),
+    with _on(x):
+        rc = _lib.load().casmvs_layer_norm_forward(_at(x), _at(weight), _at(bias), _at(y), _DTYPES[x.dtype], outer, C, inner, float(eps), float(slope),
                                                    _stream(x))
     _lib.check(rc, "casmvs_layer_norm_forward")
     return y
@@ -974,10 +995,10 @@ def layer_norm_backward(x, grad_y, weight=None, bias=None, eps=1e-5, slope=1.0, 
         raise ValueError(f"layer_norm_backward: x {tuple(x.shape)} {x.dtype}, grad_y {tuple(grad_y.shape)} {grad_y.dtype}")
     lib, code = _lib.load(), _DTYPES[x.dtype]
     gx = torch.empty_like(x) if need_x else None
-    gw, gb = (torch.empty(C, dtype=torch.float32, device=x.device) for _ in range(2)) if need_affine else (None, None)
-    ws = torch.empty(lib.casmvs_layer_norm_backward_workspace_bytes(code, outer, C, inner), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = lib.casmvs_layer_norm_backward(_ptr(x), _ptr(grad_y), _ptr(weight), _ptr(bias), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), code, outer, C, inner,
+    gw, gb = torch.empty((2, C), dtype=torch.float32, device=x.device).unbind() if need_affine else (None, None)
+    ws = torch.empty(_workspace_bytes("casmvs_layer_norm_backward_workspace_bytes", code, outer, C, inner), dtype=torch.uint8, device=x.device)
+    with _on(x):
+        rc = lib.casmvs_layer_norm_backward(_at(x), _at(grad_y), _at(weight), _at(bias), _at(gx), _at(gw), _at(gb), _at(ws), code, outer, C, inner,
                                             float(eps), float(slope), _stream(x))
     _lib.check(rc, "casmvs_layer_norm_backward")
     return gx, gw, gb
@@ -1017,8 +1038,8 @@ def pack8(x):
     nb = (n + 31) // 32
     codes = torch.empty((rows, nb, 32), dtype=torch.uint8, device=x.device)
     scales = torch.empty((rows, nb), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = _lib.load().casmvs_pack8(_ptr(x), _DTYPES[x.dtype], rows, n, _ptr(codes), _ptr(scales), _stream(x))
+    with _on(x):
+        rc = _lib.load().casmvs_pack8(_at(x), _DTYPES[x.dtype], rows, n, _at(codes), _at(scales), _stream(x))
     _lib.check(rc, "casmvs_pack8")
     return Packed8(codes, scales, x.shape, x.dtype)
 
@@ -1047,8 +1068,8 @@ def unpack8(packed):
         if tuple(weight.shape) != (C,) or tuple(bias.shape) != (C,):
             raise ValueError(f"unpack8: affine {tuple(weight.shape)} {tuple(bias.shape)}, expected ({C},)")
     out = torch.empty(packed.shape, dtype=packed.dtype, device=codes.device)
-    with torch.cuda.device(codes.device):
-        rc = _lib.load().casmvs_unpack8(_ptr(codes), _ptr(scales), _ptr(weight), _ptr(bias), C, float(slope), _ptr(out), _DTYPES[packed.dtype], rows, n,
+    with _on(codes):
+        rc = _lib.load().casmvs_unpack8(_at(codes), _at(scales), _at(weight), _at(bias), C, float(slope), _at(out), _DTYPES[packed.dtype], rows, n,
                                         _stream(codes))
     _lib.check(rc, "casmvs_unpack8")
     return out

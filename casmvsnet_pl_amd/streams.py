@@ -116,4 +116,6 @@ def note_launch(device, f16=False, stream=None):
 
 def launch_stream(t, f16=False):
     """The hipStream_t (ctypes.c_void_p) a library call on tensor `t`'s device goes to: torch's current stream, after the guard."""
+    if not enabled():   # nothing to book: the stream's address alone, without building a Stream object (2 us of a call that may take 10)
+        return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(t.device.index))
     return ctypes.c_void_p(note_launch(t.device, f16).cuda_stream)

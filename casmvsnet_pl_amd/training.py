@@ -18,8 +18,8 @@ softmax + depth regression (mvsnet.py:175-177)         autograd.softmax_depth_re
 
 What a step keeps for its backward pass: float32 tensors (checkpoint="f32": the convolutions' inputs, ABN's input and output), or with checkpoint="8bit"
 (CascadeMVSNet.checkpoint_mode) 8-bit checkpoints: an ABN keeps 8 bits of its normalised input and one bit per element, the convolution behind it rebuilds its
-input from the same bytes, and a convolution whose input is anything else (a cost volume, a skip sum) packs that.  The forward pass is the same, bit for bit;
-the gradients carry the rounding of the 8 bits.
+input from the same bytes, and a convolution whose input is anything else (a cost volume, a skip sum) packs that.  The forward pass is the same to float32's
+rounding; the gradients carry the rounding of the 8 bits.
 
 torch is the autograd tape and the allocator; the skip additions of the U-Net and the gradient accumulation are torch adds.  Nothing here runs on CPU tensors.  DESIGN.md 2.6 has the kernels and the measured step
 times (18 ms per step at the reference's default training configuration, 15 ms captured as one hipGraph).
@@ -358,10 +358,7 @@ def conv(x, weight, bias, kind, checkpoint="f32"):
         raise RuntimeError("casmvsnet_pl_amd.training runs on the MI355X only; there is no CPU fallback")
     _check_checkpoint(checkpoint)
     if checkpoint == "8bit" and x.requires_grad and weight.requires_grad and torch.is_grad_enabled():
-        packed, version = getattr(x, "_casmvs_packed8", (None, None))
-        if packed is None or version != x._version:   # not an ABN's output, or written to since
-            packed = ops.pack8(x.detach().float())
-        return _Conv8.apply(x, weight, bias, kind, packed)
+        return _Conv8.apply(x, weight, bias, kind, packed_input(x))
     return _Conv.apply(x, weight, bias, kind)
 
 
@@ -386,7 +383,7 @@ class _Conv8(torch.autograd.Function):
         return _conv_raw(kind, weight, bias, x)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @A._once
     def backward(ctx, gy):
         weight, codes, scales, aff_w, aff_b = ctx.saved_tensors
         gy = gy.contiguous().float()
@@ -458,60 +455,69 @@ class _ABNTrain(torch.autograd.Function):
         return gx, out[0], out[1], None, None, None, None, None, None
 
 
+class _Kept8:
+    """The buffer that _ABNTrain8 keeps, as byte offsets: codes (planes, nb, 32), scales (planes, nb), signs (planes, nb) words, vec (4, C) floats."""
+
+    __slots__ = ("N", "C", "n", "scales", "signs", "vec", "bytes")
+
+    def __init__(self, N, C, n):
+        blocks = N * C * ((n + 31) // 32)
+        self.N, self.C, self.n = N, C, n
+        self.scales = 32 * blocks
+        self.signs = (33 * blocks + 15) // 16 * 16
+        self.vec = (self.signs + 4 * blocks + 15) // 16 * 16
+        self.bytes = self.vec + 16 * C
+
+    def packed(self, buffer, shape, slope):
+        """What the convolution behind takes as its checkpoint: y = lrelu(gamma xhat + beta)."""
+        planes, nb = self.N * self.C, (self.n + 31) // 32
+        vec = buffer[self.vec:].view(torch.float32).view(4, self.C)
+        return ops.Packed8(buffer[:self.scales].view(planes, nb, 32), buffer[self.scales:self.scales + planes * nb].view(planes, nb), shape, torch.float32,
+                           (vec[2], vec[3], slope))
+
+
 class _ABNTrain8(torch.autograd.Function):
-    """_ABNTrain that keeps 8 bits of the normalised input and one bit per element (casmvs_abn8_*): -> (y, codes, scales, vec), y as _ABNTrain's, bit for bit."""
+    """_ABNTrain that keeps 8 bits of the normalised input and one bit per element (casmvs_abn8_*): -> (y, the buffer it keeps)."""
 
     @staticmethod
     def forward(ctx, x, weight, beta, running_mean, running_var, momentum, eps, slope, abs_eps):
         x = x.contiguous().float()
         N, C = x.shape[:2]
         n = x.numel() // (N * C)
-        M, nb = N * n, (n + 31) // 32
-        lib = _lib.load()
-        blocks = lib.casmvs_channel_sums_blocks(N, n)
-        part = torch.empty((C, blocks, 2), dtype=torch.float64, device=x.device)
-        vec = torch.empty((4, C), dtype=torch.float32, device=x.device)   # scale, shift, gamma, beta
-        codes = torch.empty((N * C, nb, 32), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((N * C, nb), dtype=torch.uint8, device=x.device)
-        signs = torch.empty((N * C, nb), dtype=torch.int32, device=x.device)
+        kept = _Kept8(N, C, n)
+        buffer = torch.empty(kept.bytes, dtype=torch.uint8, device=x.device)
+        ws = torch.empty(ops._workspace_bytes("casmvs_abn8_workspace_bytes", N, C, n), dtype=torch.uint8, device=x.device)
         y = torch.empty_like(x)
         w, bta = weight.detach().contiguous().float(), beta.detach().contiguous().float()
         track = running_mean is not None and running_var is not None
-        with torch.cuda.device(x.device):
-            st = _stream(x)
-            rc = lib.casmvs_channel_sums_f64(_ptr(x), _ptr(part), N, C, n, st)
-            _lib.check(rc, "casmvs_channel_sums_f64")
-            rc = lib.casmvs_abn8_train_apply_f32(_ptr(x), _ptr(part), blocks, float(M), _ptr(w), _ptr(bta), float(abs_eps), float(eps), float(momentum),
-                                                 _ptr(running_mean) if track else None, _ptr(running_var) if track else None, _ptr(vec), _ptr(y),
-                                                 _ptr(codes), _ptr(scales), _ptr(signs), N, C, n, float(slope), st)
-            _lib.check(rc, "casmvs_abn8_train_apply_f32")
+        base = buffer.data_ptr()
+        with ops._on(x):
+            rc = _lib.load().casmvs_abn8_forward_f32(x.data_ptr(), w.data_ptr(), bta.data_ptr(), abs_eps, eps, momentum, running_mean.data_ptr() if track else None,
+                                                     running_var.data_ptr() if track else None, base + kept.vec, y.data_ptr(), base, base + kept.scales,
+                                                     base + kept.signs, ws.data_ptr(), N, C, n, slope, _stream(x))
+        _lib.check(rc, "casmvs_abn8_forward_f32")
         if track:   # the kernel wrote the buffers behind torch's back: bump their version counters (packed-weight caches key on them)
-            torch.autograd.graph.increment_version(running_mean)
-            torch.autograd.graph.increment_version(running_var)
-        ctx.save_for_backward(codes, scales, signs, w, vec)
-        ctx.slope, ctx.M, ctx.abs_eps, ctx.n = float(slope), M, float(abs_eps), n
-        ctx.mark_non_differentiable(codes, scales, vec)
-        return y, codes, scales, vec
+            torch.autograd.graph.increment_version((running_mean, running_var))
+        ctx.save_for_backward(buffer, w)
+        ctx.kept, ctx.slope, ctx.abs_eps = kept, slope, abs_eps
+        ctx.mark_non_differentiable(buffer)
+        return y, buffer
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy, *_):
-        codes, scales, signs, w, vec = ctx.saved_tensors
+    @A._once
+    def backward(ctx, gy, _):
+        buffer, w = ctx.saved_tensors
         gy = gy.contiguous().float()
-        N, C = gy.shape[:2]
-        lib = _lib.load()
-        blocks = lib.casmvs_abn8_backward_sums_blocks(N, ctx.n)
-        part = torch.empty((C, blocks, 2), dtype=torch.float64, device=gy.device)
-        out = torch.empty((2, C), dtype=torch.float32, device=gy.device)   # grad_weight, grad_bias
+        k = ctx.kept
+        gw, gb = torch.empty((2, k.C), dtype=torch.float32, device=gy.device).unbind()
         gx = torch.empty_like(gy) if ctx.needs_input_grad[0] else None
-        with torch.cuda.device(gy.device):
-            st = _stream(gy)
-            rc = lib.casmvs_abn8_backward_sums_f64(_ptr(gy), _ptr(codes), _ptr(scales), _ptr(signs), _ptr(part), N, C, ctx.n, ctx.slope, st)
-            _lib.check(rc, "casmvs_abn8_backward_sums_f64")
-            rc = lib.casmvs_abn8_backward_apply_f32(_ptr(gy), _ptr(codes), _ptr(scales), _ptr(signs), _ptr(part), blocks, float(ctx.M), _ptr(w), ctx.abs_eps,
-                                                    _ptr(vec), _ptr(out[0]), _ptr(out[1]), _ptr(gx), N, C, ctx.n, ctx.slope, st)
-            _lib.check(rc, "casmvs_abn8_backward_apply_f32")
-        return gx, out[0], out[1], None, None, None, None, None, None
+        ws = torch.empty(ops._workspace_bytes("casmvs_abn8_workspace_bytes", k.N, k.C, k.n), dtype=torch.uint8, device=gy.device)
+        base = buffer.data_ptr()
+        with ops._on(gy):
+            rc = _lib.load().casmvs_abn8_backward_f32(gy.data_ptr(), base, base + k.scales, base + k.signs, w.data_ptr(), ctx.abs_eps, base + k.vec, gw.data_ptr(),
+                                                      gb.data_ptr(), ops._at(gx), ws.data_ptr(), k.N, k.C, k.n, ctx.slope, _stream(gy))
+        _lib.check(rc, "casmvs_abn8_backward_f32")
+        return gx, gw, gb, None, None, None, None, None, None
 
 
 def abn_train(norm, x, checkpoint="f32"):
@@ -534,10 +540,23 @@ def abn_train(norm, x, checkpoint="f32"):
     args = (x, weight, norm.bias, norm.running_mean, norm.running_var, float(norm.momentum), float(norm.eps), slope, abs_eps)
     if checkpoint == "f32":
         return _ABNTrain.apply(*args)
-    y, codes, scales, vec = _ABNTrain8.apply(*args)
-    if y.dim() > 2:   # the convolution behind takes these as its own checkpoint: y = lrelu(gamma xhat + beta)
-        y._casmvs_packed8 = (ops.Packed8(codes, scales, y.shape, torch.float32, (vec[2], vec[3], slope)), y._version)
+    if not x.is_cuda:
+        raise RuntimeError("casmvsnet_pl_amd.training runs on the MI355X only; there is no CPU fallback")
+    if x.numel() == 0:
+        raise ValueError(f"abn_train: x {tuple(x.shape)} has no batch to normalise over")
+    y, buffer = _ABNTrain8.apply(*args)
+    if y.dim() > 2:
+        y._casmvs_packed8 = (buffer, slope, y._version)
     return y
+
+
+def packed_input(x):
+    """The 8-bit checkpoint of a convolution's input: the one that the ABN which made x keeps already, or a new one."""
+    buffer, slope, version = getattr(x, "_casmvs_packed8", (None, None, None))
+    if buffer is None or version != x._version:   # not an ABN's output, or written to since
+        return ops.pack8(x.detach().float())
+    N, C = x.shape[:2]
+    return _Kept8(N, C, x.numel() // (N * C)).packed(buffer, x.shape, slope)
 
 
 class _UpsampleAdd(torch.autograd.Function):

@@ -647,19 +647,18 @@ int casmvs_pack8(const void *x, int dtype, size_t rows, size_t n, void *codes, v
 int casmvs_unpack8(const void *codes, const void *scales, const float *weight, const float *bias, int C, float slope, void *out, int dtype, size_t rows,
                    size_t n, void *stream);
 
-/* Train-mode ABN (as casmvs_abn_train_apply_f32 from the sums of casmvs_channel_sums_f64; y is the same, bit for bit) that keeps for its backward pass the
- * 8-bit checkpoint of xhat = (x - mean) rstd over the planes (N C, n) - codes, scales - and signs (N C, nb) 32-bit words: bit i of a word = [z > 0] of the block's
- * value i.  vec (4, C): scale = gamma rstd, shift, gamma (|weight| + abs_eps where abs_eps >= 0), bias as the forward pass used them.
- * Backward: sums (C, casmvs_abn8_backward_sums_blocks, 2) doubles, then grad_weight / grad_bias / grad_x (may be NULL).  N * C <= 2^21. */
-int casmvs_abn8_train_apply_f32(const float *x, const double *sums, int blocks, double count, const float *weight, const float *bias, float abs_eps,
-                                float eps, float momentum, float *running_mean, float *running_var, float *vec, float *y, void *codes, void *scales,
-                                void *signs, int N, int C, size_t n, float slope, void *stream);
-int casmvs_abn8_backward_sums_blocks(int N, size_t n);
-int casmvs_abn8_backward_sums_f64(const float *grad_y, const void *codes, const void *scales, const void *signs, double *sums, int N, int C, size_t n,
-                                  float slope, void *stream);
-int casmvs_abn8_backward_apply_f32(const float *grad_y, const void *codes, const void *scales, const void *signs, const double *sums, int blocks,
-                                   double count, const float *weight, float abs_eps, const float *vec, float *grad_weight, float *grad_bias, float *grad_x,
-                                   int N, int C, size_t n, float slope, void *stream);
+/* Train-mode ABN (batch statistics, running statistics, leaky ReLU: casmvs_channel_sums_f64 + casmvs_abn_train_apply_f32, the sums in 64 bits from the first
+ * addition on) that keeps for its backward pass the 8-bit checkpoint of xhat = (x - mean) rstd over the planes (N C, n) - codes, scales - and signs
+ * (N C, nb) 32-bit words: bit i of a word = [z > 0] of the block's value i.  vec (4, C): scale = gamma rstd, shift, gamma (|weight| + abs_eps where
+ * abs_eps >= 0), bias as the forward pass used them; act(gamma * unpacked + bias) is y up to the rounding of the 8 bits.
+ * Backward: grad_weight, grad_bias, and grad_x (may be NULL).  workspace: casmvs_abn8_workspace_bytes, for either call on its own.  N * C <= 2^21. */
+size_t casmvs_abn8_workspace_bytes(int N, int C, size_t n);
+int casmvs_abn8_forward_f32(const float *x, const float *weight, const float *bias, float abs_eps, float eps, float momentum, float *running_mean,
+                            float *running_var, float *vec, float *y, void *codes, void *scales, void *signs, void *workspace, int N, int C, size_t n,
+                            float slope, void *stream);
+int casmvs_abn8_backward_f32(const float *grad_y, const void *codes, const void *scales, const void *signs, const float *weight, float abs_eps,
+                             const float *vec, float *grad_weight, float *grad_bias, float *grad_x, void *workspace, int N, int C, size_t n, float slope,
+                             void *stream);
 
 /* Softmax cross entropy over the depth hypotheses: cost (B, D, h*w) of `dtype`, depth_values (B, D, h*w) (per_pixel) or (B, D), depth_gt (B, h*w), mask (B, h*w)
  * bytes or NULL.  The class of a pixel is the hypothesis nearest to depth_gt (the lowest index on ties); a pixel counts if its mask is not 0, depth_gt

@@ -57,18 +57,21 @@ def ln_reference(x, w, b, gy, eps, slope, dim):
     gx = r * (gw - m1 - h * m2)
     terms = r * (gw.abs() + gw.abs().mean(-1, keepdim=True) + h.abs() * (gw * h).abs().mean(-1, keepdim=True))
     over = tuple(range(x.dim() - 1))
-    return (y.movedim(-1, dim), gx.movedim(-1, dim), (g * h).sum(over), g.sum(over), terms.movedim(-1, dim), (g * h).abs().sum(over), g.abs().sum(over))
+    # the mean's own rounding in 64 bits: at most 72 additions and the division, each 2^-53 of the sum of |x|; it moves z by its size times r |w|, which a row far from
+    # zero sees where z itself is small (an offset of 3e6: 3e6 * 2^-53 = 3e-10, against half a float32 step of 6e-10 at z = 0.01)
+    far = 80 * 2.0 ** -53 * x.abs().mean(-1, keepdim=True) * r * w.abs()
+    return (y.movedim(-1, dim), far.movedim(-1, dim), gx.movedim(-1, dim), (g * h).sum(over), g.sum(over), terms.movedim(-1, dim), (g * h).abs().sum(over), g.abs().sum(over))
 
 
 def ln_check(dev, x, w, b, gy, eps=1e-5, slope=0.01, channels_last=False):
     dim = -1 if channels_last else 1
-    y, gx, gw, gb, terms, aw, ab = ln_reference(x, w, b, gy, eps, slope, dim)
+    y, far, gx, gw, gb, terms, aw, ab = ln_reference(x, w, b, gy, eps, slope, dim)
     xd = x.to(dev).requires_grad_()
     wd, bd = (None if t is None else t.to(dev).requires_grad_() for t in (w, b))
     got = A.layer_norm(xd, wd, bd, eps, slope, channels_last)
     assert got.dtype == x.dtype and got.shape == x.shape
     assert torch.equal(got, ops.layer_norm(xd, wd, bd, eps, slope, channels_last))
-    within(got, y, rounding(y, x.dtype))
+    within(got, y, rounding(y, x.dtype) + far)
     got.backward(gy.to(dev))
     assert xd.grad.dtype == x.dtype
     within(xd.grad, gx, rounding(gx, x.dtype) + 16 * U * terms)
@@ -305,16 +308,19 @@ def test_abn8_against_float64(dev, shape, slope, inplace):
     y, gx, gw, gb, terms, aw, ab, mean, unbiased = abn8_reference(x, w, b, gy, slope, 1e-5, inplace)
     xd, xp = x.to(dev).requires_grad_(), x.to(dev).requires_grad_()
     got, same = T.abn_train(norm, xd, checkpoint="8bit"), T.abn_train(plain, xp)
-    assert torch.equal(got, same) and torch.equal(norm.running_mean, plain.running_mean) and torch.equal(norm.running_var, plain.running_var)
+    # y = fma(x, scale, shift) with scale and shift rounded to float32 once each, the slope once; the f32 mode's statistics are float32 sums of 64 on the way
+    r = 1 / torch.sqrt(x.double().transpose(0, 1).flatten(1).var(1, unbiased=False) + 1e-5)
+    scale = ((w.abs() + 1e-5 if inplace else w).double() * r).abs().view(1, C, 1)
+    size = x.double().abs().reshape(y.shape) * scale + mean.abs().view(1, C, 1) * scale + b.double().abs().view(1, C, 1)
+    within(got.reshape(y.shape), y, 6 * U * size)
+    within(got.reshape(y.shape), same.reshape(y.shape), 128 * U * size)
     got.backward(gy.to(dev))
     within(xd.grad.reshape(gx.shape), gx, rounding(gx, F32) + 16 * U * terms)
     within(norm.weight.grad, gw, 64 * U * aw + rounding(gw, F32) + 1e-12)
     within(norm.bias.grad, gb, 64 * U * ab + rounding(gb, F32))
     within(norm.running_mean, 0.1 * mean, 1e-6 * (1 + mean.abs()))
     # what the convolution behind rebuilds of y: one step of xhat times gamma away at most
-    packed, version = got._casmvs_packed8
-    assert version == got._version
-    again = ops.unpack8(packed)
+    again = ops.unpack8(T.packed_input(got))
     gamma = (w.abs() + 1e-5) if inplace else w
     N = shape[0]
     h = (x.double().reshape(N, C, -1) - mean.view(1, C, 1)) / torch.sqrt(x.double().reshape(N, C, -1).var((0, 2), unbiased=False) + 1e-5).view(1, C, 1)
@@ -355,7 +361,8 @@ def test_conv8_takes_its_weight_gradient_at_the_checkpoint(dev, source):
             x.mul_(1.5)
             want_x = ops.unpack8(ops.pack8(x.detach()))
         else:
-            want_x = ops.unpack8(x._casmvs_packed8[0])
+            want_x = ops.unpack8(T.packed_input(x))
+            assert not torch.equal(want_x, ops.unpack8(ops.pack8(x.detach())))   # its own, not a new one
     elif source == "sum":
         x = base + 1.0
         want_x = ops.unpack8(ops.pack8(x.detach()))
@@ -517,11 +524,13 @@ def _calls(dev):
         p = ops.pack8(x)
         return p.codes, p.scales, ops.unpack8(p)
 
+    norm = M.ABN(8).to(dev)
+    norm.running_mean = norm.running_var = None   # (they would differ from call to call)
+
     def abn():
-        norm = M.ABN(8).to(dev) if not hasattr(abn, "norm") else abn.norm
-        abn.norm = norm
-        y, codes, scales, vec = T._ABNTrain8.apply(x, norm.weight.detach(), norm.bias.detach(), None, None, 0.1, 1e-5, 0.01, -1.0)
-        return y, codes, scales, vec
+        xr = x.detach().requires_grad_()
+        y = T.abn_train(norm, xr, checkpoint="8bit")
+        return (y.detach(), ops.unpack8(T.packed_input(y)), *torch.autograd.grad(y, (xr, norm.weight, norm.bias), gy))
 
     def ce():
         c = cost.detach().requires_grad_()
@@ -592,10 +601,11 @@ def _step(dev, norm_act, mode, loss, seed=0, size=(64, 96), B=1):
 
 @pytest.mark.parametrize("norm_act", [M.ABN, M.InPlaceABN, M.LayerNormAct])
 def test_training_step_with_8_bit_checkpoints(dev, norm_act):
-    """The same forward bit for bit; gradients near the float32 ones: the direction of every layer's weight gradient within a few percent."""
+    """The same forward to float32's rounding; gradients near the float32 ones: within a few percent of their size."""
     _, res, value, want = _step(dev, norm_act, "f32", "sl1")
     _, res8, value8, got = _step(dev, norm_act, "8bit", "sl1")
-    assert all(torch.equal(res[k], res8[k]) for k in res) and torch.equal(value, value8)
+    assert all(float((res[f"depth_{l}"] - res8[f"depth_{l}"]).abs().max()) < 1e-3 * float(res[f"depth_{l}"].abs().max()) for l in range(3))
+    assert abs(float(value) - float(value8)) < 1e-3 * float(value)
     _, _, _, again = _step(dev, norm_act, "8bit", "sl1")
     assert all(torch.equal(got[k], again[k]) for k in got)   # bit-reproducible
     a = torch.cat([want[k].flatten() for k in sorted(want)]).double()

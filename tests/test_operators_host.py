@@ -72,12 +72,15 @@ def test_c_abi_refuses_bad_arguments():
     refused(lib.casmvs_unpack8(_p(), _p(), _p(), None, 8, 1.0, _p(), 0, 8, 32, None), b"go together")
     refused(lib.casmvs_unpack8(_p(), _p(), _p(), _p(), 0, 1.0, _p(), 0, 8, 32, None), b"go together")
     assert lib.casmvs_pack8(None, 0, 0, 32, None, None, None) == 0
-    args = [_p(), _p(), 1, 1.0, _p(), _p(), -1.0, 1e-5, 0.1, None, None, _p(), _p(), _p(), _p(), _p()]
-    refused(lib.casmvs_abn8_train_apply_f32(*args, 0, 8, 32, 0.01, None), b"N=0")
-    refused(lib.casmvs_abn8_train_apply_f32(*args, 1 << 20, 8, 32, 0.01, None), b"planes")
-    refused(lib.casmvs_abn8_train_apply_f32(*(args[:9] + [_p()] + args[10:]), 1, 8, 32, 0.01, None), b"go together")
-    refused(lib.casmvs_abn8_backward_sums_f64(_p(), _p(6), _p(), _p(), _p(), 1, 8, 32, 0.01, None), b"words")
-    refused(lib.casmvs_abn8_backward_apply_f32(_p(), _p(), _p(), _p(), _p(), 0, 1.0, _p(), -1.0, _p(), _p(), _p(), None, 1, 8, 32, 0.01, None), b"bad arguments")
+    args = [_p(), _p(), _p(), -1.0, 1e-5, 0.1, None, None] + [_p()] * 6
+    refused(lib.casmvs_abn8_forward_f32(*args, 0, 8, 32, 0.01, None), b"N=0")
+    refused(lib.casmvs_abn8_forward_f32(*args, 1 << 20, 8, 32, 0.01, None), b"planes")
+    refused(lib.casmvs_abn8_forward_f32(*args, 1, 8, 1 << 50, 0.01, None), b"planes")
+    refused(lib.casmvs_abn8_forward_f32(*(args[:6] + [_p()] + args[7:]), 1, 8, 32, 0.01, None), b"go together")
+    refused(lib.casmvs_abn8_forward_f32(*(args[:13] + [_p(12)]), 1, 8, 32, 0.01, None), b"words")
+    refused(lib.casmvs_abn8_backward_f32(_p(), _p(6), _p(), _p(), _p(), -1.0, _p(), _p(), _p(), _p(), _p(), 1, 8, 32, 0.01, None), b"words")
+    refused(lib.casmvs_abn8_backward_f32(_p(), _p(), _p(), _p(), _p(), -1.0, _p(), None, _p(), _p(), _p(), 1, 8, 32, 0.01, None), b"null pointer")
+    assert lib.casmvs_abn8_workspace_bytes(0, 8, 32) == 0 and lib.casmvs_abn8_workspace_bytes(1, 8, 32) == 128
     refused(lib.casmvs_depth_ce_forward(_p(), _p(), _p(), None, _p(), _p(), _p(), _p(), _p(), 0, 1, 0, 16, 1, None), b"D=0")
     refused(lib.casmvs_depth_ce_forward(_p(), None, _p(), None, _p(), _p(), _p(), _p(), _p(), 0, 1, 4, 16, 1, None), b"null pointer")
     refused(lib.casmvs_depth_ce_forward(_p(), _p(), _p(), None, _p(), _p(), _p(), None, _p(), 0, 1, 4, 16, 1, None), b"null pointer")
