@@ -110,18 +110,18 @@ def _once(backward):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, slope, channels_last):
-        x = x.contiguous()
+        x, weight, bias, *sizes = ops._layer_norm_args(x, weight, bias, eps, slope, channels_last)
         ctx.save_for_backward(x, weight, bias)
-        ctx.args = eps, slope, channels_last
-        return ops.layer_norm(x, weight, bias, eps, slope, channels_last)
+        ctx.args = (*sizes, eps, slope)
+        return ops._layer_norm_forward(x, weight, bias, *ctx.args)
 
     @staticmethod
     @_once
     def backward(ctx, gy):
         x, weight, bias = ctx.saved_tensors
-        gx, gw, gb = ops.layer_norm_backward(x, gy, weight, bias, *ctx.args, need_x=ctx.needs_input_grad[0],
-                                             need_affine=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
-        return gx, (gw if ctx.needs_input_grad[1] else None), (gb if ctx.needs_input_grad[2] else None), None, None, None
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        gx, gw, gb = ops._layer_norm_backward(x, gy.contiguous(), weight, bias, *ctx.args, need_x, need_w or need_b)
+        return gx, gw if need_w else None, gb if need_b else None, None, None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, slope=1.0, channels_last=False):

@@ -110,21 +110,26 @@ __global__ __launch_bounds__(kThreads) void unpack8_kernel(const unsigned *__res
 // of the pass behind: one partial sum per lane of a wave, in a fixed order.
 constexpr int kParts = 64;
 
-// sums of a workgroup's two values per thread, to thread 0
+// sums of two values per thread over a workgroup of THREADS, in every thread: lanes by exchange, then the waves' sums in their order
+template <int THREADS>
 __device__ __forceinline__ void workgroup_sums(double &s0, double &s1) {
-  __shared__ double red[2][kThreads];
-  red[0][threadIdx.x] = s0;
-  red[1][threadIdx.x] = s1;
-  __syncthreads();
-  for (int st = kThreads / 2; st > 0; st >>= 1) {
-    if ((int)threadIdx.x < st) {
-      red[0][threadIdx.x] += red[0][threadIdx.x + st];
-      red[1][threadIdx.x] += red[1][threadIdx.x + st];
-    }
-    __syncthreads();
+  __shared__ double red[2][THREADS / 64];
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    s0 += casmvs::elem::lane_xor(s0, d);
+    s1 += casmvs::elem::lane_xor(s1, d);
   }
-  s0 = red[0][0];
-  s1 = red[1][0];
+  if ((threadIdx.x & 63) == 0) {
+    red[0][threadIdx.x >> 6] = s0;
+    red[1][threadIdx.x >> 6] = s1;
+  }
+  __syncthreads();
+  s0 = s1 = 0.0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) {
+    s0 += red[0][i];
+    s1 += red[1][i];
+  }
 }
 
 // The channel's two totals from its partial sums (C, parts, 2), parts <= 64, in every wave.
@@ -139,19 +144,17 @@ __device__ __forceinline__ void channel_totals(const double *__restrict__ sums, 
   }
 }
 
-// sum x and sum x^2 of channel blockIdx.y, in 64 bits from the first addition on (x^2 is exact there): xhat's codes and the side of zero hang on the mean
-template <bool WIDE>
-__global__ __launch_bounds__(kThreads) void abn8_sums_kernel(const float *__restrict__ x, double *__restrict__ out, int N, int C, size_t n) {
-  const int c = blockIdx.y;
-  const size_t words = (n + 3) / 4, per = (words + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < words ? lo + per : words;
-  double s0 = 0.0, s1 = 0.0;
+// A workgroup's share [lo, hi) of a channel's planes, in words of four values, added to the sums of x and x^2: in 64 bits from the first addition on (x^2 is exact
+// there), because xhat's codes and the side of zero hang on the mean.
+template <bool WIDE, int THREADS>
+__device__ __forceinline__ void add_squares(const float *__restrict__ x, int N, int C, int c, size_t n, size_t lo, size_t hi, double &s0, double &s1) {
   for (int img = 0; img < N; ++img) {
     const float *xp = x + ((size_t)img * C + c) * n;
-    for (size_t e = lo + threadIdx.x; e < hi; e += 4 * kThreads) {
+    for (size_t e = lo + threadIdx.x; e < hi; e += 4 * THREADS) {
       float v[4][4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {   // four loads in flight
-        const size_t at = e + (size_t)k * kThreads;
+        const size_t at = e + (size_t)k * THREADS;
         load4<float, WIDE>(xp + 4 * at, at < hi ? left_of(n, 4 * at) : 0, v[k]);
       }
 #pragma unroll
@@ -164,7 +167,92 @@ __global__ __launch_bounds__(kThreads) void abn8_sums_kernel(const float *__rest
         }
     }
   }
-  workgroup_sums(s0, s1);
+}
+
+struct Channel {   // what the apply pass needs of a channel
+  double mean, rstd;
+  float gamma, beta, scale, shift;
+};
+struct Norm {      // arguments of either form of the forward pass
+  const float *weight, *bias;
+  float abs_eps, eps, momentum, slope;
+  float *rmean, *rvar, *vec;   // vec (4, C): scale = gamma rstd, shift, gamma, beta of the forward pass
+};
+__device__ __forceinline__ Channel finish(const Norm &p, double s0, double s1, double M, int c, int C, bool write) {
+  Channel k;
+  k.mean = s0 / M;
+  double var = s1 / M - k.mean * k.mean;   // biased
+  var = var > 0.0 ? var : (var != var ? var : 0.0);
+  k.rstd = 1.0 / sqrt(var + (double)p.eps);
+  k.gamma = p.abs_eps >= 0.0f ? fabsf(p.weight[c]) + p.abs_eps : p.weight[c];
+  k.beta = p.bias[c];
+  k.scale = (float)((double)k.gamma * k.rstd);
+  k.shift = (float)((double)k.beta - k.mean * (double)k.gamma * k.rstd);
+  if (write) {
+    p.vec[c] = k.scale;
+    p.vec[C + c] = k.shift;
+    p.vec[2 * C + c] = k.gamma;
+    p.vec[3 * C + c] = k.beta;
+    if (p.rmean) {   // F.batch_norm: running = (1 - momentum) * running + momentum * batch (running_var: unbiased)
+      const float keep = (float)(1.0 - (double)p.momentum);
+      p.rmean[c] = p.rmean[c] * keep + p.momentum * (float)k.mean;
+      p.rvar[c] = p.rvar[c] * keep + p.momentum * (float)(var * (M / (M > 1.0 ? M - 1.0 : 1.0)));
+    }
+  }
+  return k;
+}
+
+struct Store {     // the 8-bit checkpoint of the normalised input and the signs of z
+  unsigned *codes;
+  unsigned char *scales;
+  unsigned *signs;
+};
+// y and the checkpoint of the blocks blk0, blk0 + step, .. (kAhead of them, their loads issued together) of one plane.  Every lane of a wave comes here together.
+constexpr int kAhead = 4;
+template <bool WIDE>
+__device__ __forceinline__ void apply_blocks(const float *__restrict__ xp, float *__restrict__ yp, const Store &to, size_t base, size_t blk0, size_t step, size_t n,
+                                             size_t nb, int lane, const Channel &c, float slope) {
+  float v[kAhead][4];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const size_t first = (blk0 + k * step) * kBlock + 4 * lane;
+    load4<float, WIDE>(xp + first, left_of(n, first), v[k]);   // 0 past the plane's last block
+  }
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const size_t blk = blk0 + k * step, first = blk * kBlock + 4 * lane;
+    const int left = left_of(n, first);
+    float o[4];
+    double h[4];
+    unsigned up = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[i] = i < left ? ((double)v[k][i] - c.mean) * c.rstd : 0.0;
+      up |= (fma(h[i], (double)c.gamma, (double)c.beta) > 0.0 ? 1u : 0u) << i;
+      const float t = fmaf(v[k][i], c.scale, c.shift);
+      o[i] = t > 0.0f ? t : t * slope;
+    }
+    unsigned scale;
+    const unsigned q = casmvs::block8::quantise(h, scale);
+    const unsigned sign = casmvs::block8::over_block(up << (4 * lane), [](unsigned p, unsigned r) { return p | r; });
+    store4<float, WIDE>(yp + first, left, o);
+    if (blk < nb) {
+      to.codes[(base + blk) * kLanes + lane] = q;
+      if (lane == 0) {
+        to.scales[base + blk] = (unsigned char)scale;
+        to.signs[base + blk] = sign;
+      }
+    }
+  }
+}
+
+template <bool WIDE>
+__global__ __launch_bounds__(kThreads) void abn8_sums_kernel(const float *__restrict__ x, double *__restrict__ out, int N, int C, size_t n) {
+  const int c = blockIdx.y;
+  const size_t words = (n + 3) / 4, per = (words + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < words ? lo + per : words;
+  double s0 = 0.0, s1 = 0.0;
+  add_squares<WIDE, kThreads>(x, N, C, c, n, lo, hi, s0, s1);
+  workgroup_sums<kThreads>(s0, s1);
   if (threadIdx.x == 0) {
     out[((size_t)c * gridDim.x + blockIdx.x) * 2] = s0;
     out[((size_t)c * gridDim.x + blockIdx.x) * 2 + 1] = s1;
@@ -172,72 +260,36 @@ __global__ __launch_bounds__(kThreads) void abn8_sums_kernel(const float *__rest
 }
 
 constexpr int kTurns = 8;   // blocks per group of eight lanes and workgroup: 256 x 32 = 8192 elements share one read of the channel's partial sums
-constexpr int kAhead = 4;   // turns whose loads are issued together
 
-// blockIdx.x = (plane, chunk of kTurns * kGroups blocks); vec (4, C): scale = gamma rstd, shift, gamma, beta of the forward pass
+// blockIdx.x = (plane, chunk of kTurns * kGroups blocks)
 template <bool WIDE>
-__global__ __launch_bounds__(kThreads) void abn8_apply_kernel(const float *__restrict__ x, const double *__restrict__ sums, int parts, double M,
-                                                             const float *__restrict__ weight, const float *__restrict__ bias, float abs_eps, float eps,
-                                                             float momentum, float *__restrict__ rmean, float *__restrict__ rvar, float *__restrict__ vec,
-                                                             float *__restrict__ y, unsigned *__restrict__ codes, unsigned char *__restrict__ scales,
-                                                             unsigned *__restrict__ signs, int C, size_t n, size_t nb, unsigned chunks, float slope) {
+__global__ __launch_bounds__(kThreads) void abn8_apply_kernel(const float *__restrict__ x, const double *__restrict__ sums, int parts, double M, Norm norm,
+                                                             float *__restrict__ y, Store to, int C, size_t n, size_t nb, unsigned chunks) {
   const unsigned plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-  const int c = (int)(plane % C), lane = threadIdx.x & (kLanes - 1);
-  const float *xp = x + plane * n;
-  float *yp = y + plane * n;
-  const size_t base = plane * nb;
+  const int c = (int)(plane % C);
   double s0, s1;
   channel_totals(sums, parts, c, s0, s1);
-  const double mu = s0 / M;
-  double var = s1 / M - mu * mu;   // biased
-  var = var > 0.0 ? var : 0.0;
-  const double rs = 1.0 / sqrt(var + (double)eps);
-  const float gamma = abs_eps >= 0.0f ? fabsf(weight[c]) + abs_eps : weight[c], beta = bias[c];
-  const float a = (float)((double)gamma * rs), bq = (float)((double)beta - mu * (double)gamma * rs);
-  if (chunk == 0 && plane == (unsigned)c && threadIdx.x == 0) {
-    vec[c] = a;
-    vec[C + c] = bq;
-    vec[2 * C + c] = gamma;
-    vec[3 * C + c] = beta;
-    if (rmean) {   // F.batch_norm: running = (1 - momentum) * running + momentum * batch (running_var: unbiased)
-      const float keep = (float)(1.0 - (double)momentum);
-      rmean[c] = rmean[c] * keep + momentum * (float)mu;
-      rvar[c] = rvar[c] * keep + momentum * (float)(var * (M / (M > 1.0 ? M - 1.0 : 1.0)));
-    }
-  }
-  for (int ahead = 0; ahead < kTurns; ahead += kAhead) {
-    float v[kAhead][4];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const size_t first = (((size_t)chunk * kTurns + ahead + k) * kGroups + threadIdx.x / kLanes) * kBlock + 4 * lane;
-      load4<float, WIDE>(xp + first, left_of(n, first), v[k]);   // 0 past the plane's last block
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const size_t blk = ((size_t)chunk * kTurns + ahead + k) * kGroups + threadIdx.x / kLanes, first = blk * kBlock + 4 * lane;
-      const int left = left_of(n, first);
-      float o[4];
-      double h[4];
-      unsigned up = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        h[i] = i < left ? ((double)v[k][i] - mu) * rs : 0.0;
-        up |= (fma(h[i], (double)gamma, (double)beta) > 0.0 ? 1u : 0u) << i;
-        const float t = fmaf(v[k][i], a, bq);
-        o[i] = t > 0.0f ? t : t * slope;
-      }
-      unsigned scale;
-      const unsigned q = casmvs::block8::quantise(h, scale);
-      const unsigned sign = casmvs::block8::over_block(up << (4 * lane), [](unsigned p, unsigned r) { return p | r; });
-      store4<float, WIDE>(yp + first, left, o);
-      if (blk < nb) {
-        codes[(base + blk) * kLanes + lane] = q;
-        if (lane == 0) {
-          scales[base + blk] = (unsigned char)scale;
-          signs[base + blk] = sign;
-        }
-      }
-    }
+  const Channel k = finish(norm, s0, s1, M, c, C, chunk == 0 && plane == (unsigned)c && threadIdx.x == 0);
+  for (int turn = 0; turn < kTurns; turn += kAhead)
+    apply_blocks<WIDE>(x + plane * n, y + plane * n, to, plane * nb, ((size_t)chunk * kTurns + turn) * kGroups + threadIdx.x / kLanes, kGroups, n, nb,
+                       threadIdx.x & (kLanes - 1), k, norm.slope);
+}
+
+// A channel per workgroup, both passes: one launch where a channel is small (kOneLaunch)
+constexpr int kWide = 1024;   // threads of the one-launch forms
+template <bool WIDE>
+__global__ __launch_bounds__(kWide) void abn8_forward_one_kernel(const float *__restrict__ x, double M, Norm norm, float *__restrict__ y, Store to, int N, int C, size_t n,
+                                                                size_t nb) {
+  constexpr int groups = kWide / kLanes;
+  const int c = blockIdx.x;
+  double s0 = 0.0, s1 = 0.0;
+  add_squares<WIDE, kWide>(x, N, C, c, n, 0, (n + 3) / 4, s0, s1);
+  workgroup_sums<kWide>(s0, s1);
+  const Channel k = finish(norm, s0, s1, M, c, C, threadIdx.x == 0);
+  for (int img = 0; img < N; ++img) {
+    const size_t plane = (size_t)img * C + c;
+    for (size_t blk = 0; blk < nb; blk += kAhead * groups)
+      apply_blocks<WIDE>(x + plane * n, y + plane * n, to, plane * nb, blk + threadIdx.x / kLanes, groups, n, nb, threadIdx.x & (kLanes - 1), k, norm.slope);
   }
 }
 
@@ -247,37 +299,39 @@ struct Kept {
   unsigned q, up;
   float step;
 };
+struct Checkpoint {
+  const unsigned *codes;
+  const unsigned char *scales;
+  const unsigned *signs;
+};
 template <bool WIDE>
-__device__ __forceinline__ void load_kept(const float *__restrict__ gy, const unsigned *__restrict__ codes, const unsigned char *__restrict__ scales,
-                                          const unsigned *__restrict__ signs, size_t plane, size_t blk, size_t n, size_t nb, int lane, Kept &k) {
+__device__ __forceinline__ void load_kept(const float *__restrict__ gy, const Checkpoint &from, size_t plane, size_t blk, size_t n, size_t nb, int lane, Kept &k) {
   const size_t first = blk * kBlock + 4 * lane, at = plane * nb + (blk < nb ? blk : 0);
   load4<float, WIDE>(gy + plane * n + first, left_of(n, first), k.g);   // 0 past the plane's last block
-  k.q = codes[at * kLanes + lane];
-  k.up = signs[at] >> (4 * lane);
-  k.step = casmvs::block8::step_of(scales[at]);
+  k.q = from.codes[at * kLanes + lane];
+  k.up = from.signs[at] >> (4 * lane);
+  k.step = casmvs::block8::step_of(from.scales[at]);
 }
 __device__ __forceinline__ float behind_activation(const Kept &k, int i, float slope) { return k.g[i] * ((k.up >> i) & 1u ? 1.0f : slope); }
 
-// this workgroup's part of sum g and sum g Q of channel blockIdx.y
-template <bool WIDE>
-__global__ __launch_bounds__(kThreads) void abn8_backward_sums_kernel(const float *__restrict__ gy, const unsigned *__restrict__ codes,
-                                                                     const unsigned char *__restrict__ scales, const unsigned *__restrict__ signs,
-                                                                     double *__restrict__ out, int N, int C, size_t n, size_t nb, float slope) {
-  const int c = blockIdx.y, lane = threadIdx.x & (kLanes - 1);
-  const size_t per = (nb + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < nb ? lo + per : nb;
-  double s0 = 0.0, s1 = 0.0;
+// the blocks [lo, hi) of a channel's planes, added to sum g and sum g Q
+template <bool WIDE, int THREADS>
+__device__ __forceinline__ void add_gradients(const float *__restrict__ gy, const Checkpoint &from, int N, int C, int c, size_t n, size_t nb, size_t lo, size_t hi,
+                                              float slope, double &s0, double &s1) {
+  constexpr int groups = THREADS / kLanes;
+  const int lane = threadIdx.x & (kLanes - 1);
   for (int img = 0; img < N; ++img) {
     const size_t plane = (size_t)img * C + c;
-    for (size_t blk = lo + threadIdx.x / kLanes; blk < hi; blk += kAhead * kGroups) {
+    for (size_t blk = lo + threadIdx.x / kLanes; blk < hi; blk += kAhead * groups) {
       Kept k[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const size_t at = blk + (size_t)j * kGroups;
-        load_kept<WIDE>(gy, codes, scales, signs, plane, at < hi ? at : nb, n, nb, lane, k[j]);
+        const size_t at = blk + (size_t)j * groups;
+        load_kept<WIDE>(gy, from, plane, at < hi ? at : nb, n, nb, lane, k[j]);
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        if (blk + (size_t)j * kGroups >= hi) break;
+        if (blk + (size_t)j * groups >= hi) break;
         float p0 = 0.0f, p1 = 0.0f;   // four values in float32, then 64 bits
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -290,47 +344,85 @@ __global__ __launch_bounds__(kThreads) void abn8_backward_sums_kernel(const floa
       }
     }
   }
-  workgroup_sums(s0, s1);
+}
+
+template <bool WIDE>
+__global__ __launch_bounds__(kThreads) void abn8_backward_sums_kernel(const float *__restrict__ gy, Checkpoint from, double *__restrict__ out, int N, int C, size_t n,
+                                                                     size_t nb, float slope) {
+  const int c = blockIdx.y;
+  const size_t per = (nb + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < nb ? lo + per : nb;
+  double s0 = 0.0, s1 = 0.0;
+  add_gradients<WIDE, kThreads>(gy, from, N, C, c, n, nb, lo, hi, slope, s0, s1);
+  workgroup_sums<kThreads>(s0, s1);
   if (threadIdx.x == 0) {
     out[((size_t)c * gridDim.x + blockIdx.x) * 2] = s0;
     out[((size_t)c * gridDim.x + blockIdx.x) * 2 + 1] = s1;
   }
 }
 
-template <bool WIDE>
-__global__ __launch_bounds__(kThreads) void abn8_backward_apply_kernel(const float *__restrict__ gy, const unsigned *__restrict__ codes,
-                                                                      const unsigned char *__restrict__ scales, const unsigned *__restrict__ signs,
-                                                                      const double *__restrict__ sums, int parts, double M, const float *__restrict__ weight,
-                                                                      float abs_eps, const float *__restrict__ vec, float *__restrict__ gweight,
-                                                                      float *__restrict__ gbias, float *__restrict__ gx, int C, size_t n, size_t nb,
-                                                                      unsigned chunks, float slope) {
-  const unsigned plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-  const int c = (int)(plane % C), lane = threadIdx.x & (kLanes - 1);
-  double s0, s1;
-  channel_totals(sums, parts, c, s0, s1);
-  const float m1 = (float)(s0 / M), m2 = (float)(s1 / M), a = vec[c];
-  if (chunk == 0 && plane == (unsigned)c && threadIdx.x == 0) {
-    const float w = weight[c];
-    const float sgn = abs_eps >= 0.0f ? (w > 0.0f ? 1.0f : (w < 0.0f ? -1.0f : 0.0f)) : 1.0f;   // d|w| / dw
-    gweight[c] = (float)s1 * sgn;
-    gbias[c] = (float)s0;
+struct Gradients {
+  const float *weight, *vec;
+  float abs_eps, slope;
+  float *gweight, *gbias, *gx;   // gx may be null
+};
+struct Means {   // of g and g Q, and gamma rstd
+  float m1, m2, a;
+};
+__device__ __forceinline__ Means finish_gradients(const Gradients &p, double s0, double s1, double M, int c, bool write) {
+  if (write) {
+    const float w = p.weight[c];
+    const float sgn = p.abs_eps >= 0.0f ? (w > 0.0f ? 1.0f : (w < 0.0f ? -1.0f : 0.0f)) : 1.0f;   // d|w| / dw
+    p.gweight[c] = (float)s1 * sgn;
+    p.gbias[c] = (float)s0;
   }
-  if (!gx) return;
-  for (int ahead = 0; ahead < kTurns; ahead += kAhead) {
-    const size_t blk = ((size_t)chunk * kTurns + ahead) * kGroups + threadIdx.x / kLanes;
-    Kept k[kAhead];
+  return Means{(float)(s0 / M), (float)(s1 / M), p.vec[c]};
+}
+template <bool WIDE>
+__device__ __forceinline__ void gradient_blocks(const float *__restrict__ gy, const Checkpoint &from, float *__restrict__ gx, size_t plane, size_t blk0, size_t step, size_t n,
+                                                size_t nb, const Means &m, float slope) {
+  const int lane = threadIdx.x & (kLanes - 1);
+  Kept k[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) load_kept<WIDE>(gy, codes, scales, signs, plane, blk + (size_t)j * kGroups, n, nb, lane, k[j]);
+  for (int j = 0; j < kAhead; ++j) load_kept<WIDE>(gy, from, plane, blk0 + j * step, n, nb, lane, k[j]);
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const size_t first = (blk + (size_t)j * kGroups) * kBlock + 4 * lane;
-      float o[4];
+  for (int j = 0; j < kAhead; ++j) {
+    const size_t first = (blk0 + j * step) * kBlock + 4 * lane;
+    float o[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = a * (behind_activation(k[j], i, slope) - m1 - casmvs::block8::value_of(k[j].q, i, k[j].step) * m2);
-      store4<float, WIDE>(gx + plane * n + first, left_of(n, first), o);
-    }
+    for (int i = 0; i < 4; ++i) o[i] = m.a * (behind_activation(k[j], i, slope) - m.m1 - casmvs::block8::value_of(k[j].q, i, k[j].step) * m.m2);
+    store4<float, WIDE>(gx + plane * n + first, left_of(n, first), o);
   }
 }
+
+template <bool WIDE>
+__global__ __launch_bounds__(kThreads) void abn8_backward_apply_kernel(const float *__restrict__ gy, Checkpoint from, const double *__restrict__ sums, int parts, double M,
+                                                                      Gradients p, int C, size_t n, size_t nb, unsigned chunks) {
+  const unsigned plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const int c = (int)(plane % C);
+  double s0, s1;
+  channel_totals(sums, parts, c, s0, s1);
+  const Means m = finish_gradients(p, s0, s1, M, c, chunk == 0 && plane == (unsigned)c && threadIdx.x == 0);
+  if (!p.gx) return;
+  for (int turn = 0; turn < kTurns; turn += kAhead)
+    gradient_blocks<WIDE>(gy, from, p.gx, plane, ((size_t)chunk * kTurns + turn) * kGroups + threadIdx.x / kLanes, kGroups, n, nb, m, p.slope);
+}
+
+template <bool WIDE>
+__global__ __launch_bounds__(kWide) void abn8_backward_one_kernel(const float *__restrict__ gy, Checkpoint from, double M, Gradients p, int N, int C, size_t n, size_t nb) {
+  constexpr int groups = kWide / kLanes;
+  const int c = blockIdx.x;
+  double s0 = 0.0, s1 = 0.0;
+  add_gradients<WIDE, kWide>(gy, from, N, C, c, n, nb, 0, nb, p.slope, s0, s1);
+  workgroup_sums<kWide>(s0, s1);
+  const Means m = finish_gradients(p, s0, s1, M, c, threadIdx.x == 0);
+  if (!p.gx) return;
+  for (int img = 0; img < N; ++img)
+    for (size_t blk = 0; blk < nb; blk += kAhead * groups)
+      gradient_blocks<WIDE>(gy, from, p.gx, (size_t)img * C + c, blk + threadIdx.x / kLanes, groups, n, nb, m, p.slope);
+}
+
+// Elements of a channel up to which one workgroup does both passes over it: one launch less, on as many CUs as there are channels
+constexpr size_t kOneLaunch = 16384;
 
 // Workgroups that form a channel's sums: at least 4096 elements each, at most 1024 workgroups in all (four per CU)
 int parts_of(int N, int C, size_t n) {
@@ -414,13 +506,19 @@ extern "C" int casmvs_abn8_forward_f32(const float *x, const float *weight, cons
                  "abn8_forward: codes and signs are 4-byte words, the workspace 8-byte ones");
   const size_t nb = blocks_of(n), chunks = (nb + kTurns * kGroups - 1) / (kTurns * kGroups);
   const int parts = parts_of(N, C, n);
+  const double count = (double)N * (double)n;
   double *sums = (double *)workspace;
   hipStream_t st = (hipStream_t)stream;
   const bool wide = n % 4 == 0 && aligned16(x) && aligned16(y);
+  const Norm norm{weight, bias, abs_eps, eps, momentum, slope, running_mean, running_var, vec};
+  const Store to{(unsigned *)codes, (unsigned char *)scales, (unsigned *)signs};
+  if ((size_t)N * n <= kOneLaunch) {
+    hipLaunchKernelGGL(wide ? abn8_forward_one_kernel<true> : abn8_forward_one_kernel<false>, dim3((unsigned)C), dim3(kWide), 0, st, x, count, norm, y, to, N, C, n, nb);
+    return casmvs::check_launch("abn8_forward_one_kernel");
+  }
   hipLaunchKernelGGL(wide ? abn8_sums_kernel<true> : abn8_sums_kernel<false>, dim3((unsigned)parts, (unsigned)C), dim3(kThreads), 0, st, x, sums, N, C, n);
-  hipLaunchKernelGGL(wide ? abn8_apply_kernel<true> : abn8_apply_kernel<false>, dim3((unsigned)((size_t)N * C * chunks)), dim3(kThreads), 0, st, x, sums, parts,
-                     (double)N * (double)n, weight, bias, abs_eps, eps, momentum, running_mean, running_var, vec, y, (unsigned *)codes, (unsigned char *)scales,
-                     (unsigned *)signs, C, n, nb, (unsigned)chunks, slope);
+  hipLaunchKernelGGL(wide ? abn8_apply_kernel<true> : abn8_apply_kernel<false>, dim3((unsigned)((size_t)N * C * chunks)), dim3(kThreads), 0, st, x, sums, parts, count, norm,
+                     y, to, C, n, nb, (unsigned)chunks);
   return casmvs::check_launch("abn8_forward");
 }
 
@@ -434,16 +532,21 @@ extern "C" int casmvs_abn8_backward_f32(const float *grad_y, const void *codes, 
                  "abn8_backward: codes and signs are 4-byte words, the workspace 8-byte ones");
   const size_t nb = blocks_of(n), chunks = (nb + kTurns * kGroups - 1) / (kTurns * kGroups);
   const int parts = parts_of(N, C, n);
+  const double count = (double)N * (double)n;
   double *sums = (double *)workspace;
   hipStream_t st = (hipStream_t)stream;
-  const unsigned *cp = (const unsigned *)codes, *up = (const unsigned *)signs;
-  const unsigned char *sp = (const unsigned char *)scales;
   const bool wide = n % 4 == 0 && aligned16(grad_y) && aligned16(grad_x);
-  hipLaunchKernelGGL(wide ? abn8_backward_sums_kernel<true> : abn8_backward_sums_kernel<false>, dim3((unsigned)parts, (unsigned)C), dim3(kThreads), 0, st, grad_y, cp,
-                     sp, up, sums, N, C, n, nb, slope);
+  const Checkpoint from{(const unsigned *)codes, (const unsigned char *)scales, (const unsigned *)signs};
+  const Gradients to{weight, vec, abs_eps, slope, grad_weight, grad_bias, grad_x};
+  if ((size_t)N * n <= kOneLaunch) {
+    hipLaunchKernelGGL(wide ? abn8_backward_one_kernel<true> : abn8_backward_one_kernel<false>, dim3((unsigned)C), dim3(kWide), 0, st, grad_y, from, count, to, N, C, n, nb);
+    return casmvs::check_launch("abn8_backward_one_kernel");
+  }
+  hipLaunchKernelGGL(wide ? abn8_backward_sums_kernel<true> : abn8_backward_sums_kernel<false>, dim3((unsigned)parts, (unsigned)C), dim3(kThreads), 0, st, grad_y, from, sums,
+                     N, C, n, nb, slope);
   // (without grad_x the workgroups of the channels' first chunks write the two vectors, and there are no others)
   const dim3 grid((unsigned)(grad_x ? (size_t)N * C * chunks : (size_t)C * chunks));
-  hipLaunchKernelGGL(wide ? abn8_backward_apply_kernel<true> : abn8_backward_apply_kernel<false>, grid, dim3(kThreads), 0, st, grad_y, cp, sp, up, sums, parts,
-                     (double)N * (double)n, weight, abs_eps, vec, grad_weight, grad_bias, grad_x, C, n, nb, (unsigned)chunks, slope);
+  hipLaunchKernelGGL(wide ? abn8_backward_apply_kernel<true> : abn8_backward_apply_kernel<false>, grid, dim3(kThreads), 0, st, grad_y, from, sums, parts, count, to, C, n, nb,
+                     (unsigned)chunks);
   return casmvs::check_launch("abn8_backward");
 }

@@ -632,11 +632,18 @@ struct Call {   // arguments of either direction
   const float *w, *b;
   void *out;        // y, or gx (may be null)
   float *partial;   // null: no weight gradient
+  float *gw, *gb;   // where it goes
   size_t outer, inner;
   int C;
   float eps, slope;
   hipStream_t stream;
   size_t positions() const { return outer * inner; }
+  // One workgroup's sums are the gradients themselves, where grad_bias lies behind grad_weight: nothing is left to add up (parts = 0)
+  float *sums(int &parts) const {
+    if (!partial || parts != 1 || gb != gw + C) return partial;
+    parts = 0;
+    return gw;
+  }
 };
 
 template <class T, int CG, int V>
@@ -647,9 +654,11 @@ void planes(const Call &a, int &parts) {
                        a.inner, 1.0 / a.C, a.eps, a.slope);
     return;
   }
-  parts = (int)(tiles < kBackwardBlocks ? tiles : kBackwardBlocks);
+  const unsigned grid = (unsigned)(tiles < kBackwardBlocks ? tiles : kBackwardBlocks);
+  parts = (int)grid;
+  float *sums = a.sums(parts);
   auto kernel = a.partial ? ln_backward_planes_kernel<T, CG, V, true> : ln_backward_planes_kernel<T, CG, V, false>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)parts), dim3(kThreads), 0, a.stream, (const T *)a.x, (const T *)a.gy, a.w, a.b, (T *)a.out, a.partial, a.positions(), tiles,
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0, a.stream, (const T *)a.x, (const T *)a.gy, a.w, a.b, (T *)a.out, sums, a.positions(), tiles,
                      a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
 }
 template <class T, int V>
@@ -672,9 +681,11 @@ void rows(const Call &a, int &parts) {
                        1.0 / a.C, a.eps, a.slope);
     return;
   }
-  parts = (int)(blocks < kBackwardBlocks ? blocks : kBackwardBlocks);
+  const unsigned grid = (unsigned)(blocks < kBackwardBlocks ? blocks : kBackwardBlocks);
+  parts = (int)grid;
+  float *sums = a.sums(parts);
   auto kernel = a.partial ? ln_backward_rows_kernel<T, L, V, K, true> : ln_backward_rows_kernel<T, L, V, K, false>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)parts), dim3(threads), 0, a.stream, (const T *)a.x, (const T *)a.gy, a.w, a.b, (T *)a.out, a.partial, a.outer, a.C,
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, a.stream, (const T *)a.x, (const T *)a.gy, a.w, a.b, (T *)a.out, sums, a.outer, a.C,
                      1.0 / a.C, a.eps, a.slope);
 }
 template <class T, int V>
@@ -692,7 +703,7 @@ void rows_by_width(const Call &a, int &parts) {
   else rows<T, 512, V, k16>(a, parts);
 }
 
-// Either direction in the planes / rows form; `parts`: rows of partial sums that the backward pass wrote.
+// Either direction in the planes / rows form; `parts`: rows of partial sums that the backward pass wrote and are still to be added up.
 void run_form(Form form, int dtype, const Call &a, int &parts) {
   CASMVS_WITH_DTYPE(dtype, {
     // four elements at a time where rows / planes keep their alignment
@@ -717,7 +728,7 @@ extern "C" int casmvs_layer_norm_forward(const void *x, const float *weight, con
   hipStream_t st = (hipStream_t)stream;
   if (form != kAny) {
     int parts = 0;
-    run_form(form, dtype, Call{x, nullptr, weight, bias, y, nullptr, outer, inner, C, eps, slope, st}, parts);
+    run_form(form, dtype, Call{x, nullptr, weight, bias, y, nullptr, nullptr, nullptr, outer, inner, C, eps, slope, st}, parts);
     return casmvs::check_launch("layer_norm_forward");
   }
   const size_t positions = outer * inner;
@@ -750,8 +761,8 @@ extern "C" int casmvs_layer_norm_backward(const void *x, const void *grad_y, con
   const Form form = form_of(C, inner);
   if (form != kAny || !positions) {
     int parts = 0;
-    if (positions) run_form(form, dtype, Call{x, grad_y, weight, bias, grad_x, grad_weight ? (float *)workspace : nullptr, outer, inner, C, eps, slope, st}, parts);
-    if (grad_weight) {
+    if (positions) run_form(form, dtype, Call{x, grad_y, weight, bias, grad_x, grad_weight ? (float *)workspace : nullptr, grad_weight, grad_bias, outer, inner, C, eps, slope, st}, parts);
+    if (grad_weight && (parts || !positions)) {
       if (C <= 32)
         hipLaunchKernelGGL(ln_finish_parts_kernel<16>, dim3((unsigned)((2 * C + 15) / 16)), dim3(1024), 0, st, (const float *)workspace, grad_weight, grad_bias, parts, C);
       else

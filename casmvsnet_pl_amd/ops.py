@@ -966,42 +966,45 @@ def _layer_norm_args(x, weight, bias, eps, slope, channels_last):
             if tuple(t.shape) != (C,):
                 raise ValueError(f"layer_norm: {name} {tuple(t.shape)}, expected ({C},)")
         affine.append(t)
-    inner = 1
-    if not channels_last:
-        for s in x.shape[2:]:
-            inner *= s
-    outer = x.numel() // (C * inner) if x.numel() else 0
-    return x, affine[0], affine[1], outer, C, inner
+    numel = x.numel()
+    inner = 1 if channels_last or not numel else numel // (x.shape[0] * C)
+    return x, affine[0], affine[1], numel // (C * inner), C, inner
+
+
+def _layer_norm_forward(x, weight, bias, outer, C, inner, eps, slope):
+    y = torch.empty_like(x)
+    with _on(x):
+        rc = _lib.load().casmvs_layer_norm_forward(x.data_ptr(), _at(weight), _at(bias), y.data_ptr(), _DTYPES[x.dtype], outer, C, inner, eps, slope, _stream(x))
+    _lib.check(rc, "casmvs_layer_norm_forward")
+    return y
+
+
+def _layer_norm_backward(x, grad_y, weight, bias, outer, C, inner, eps, slope, need_x, need_affine):
+    code = _DTYPES[x.dtype]
+    gx = torch.empty_like(x) if need_x else None
+    gw, gb = torch.empty((2, C), dtype=torch.float32, device=x.device).unbind() if need_affine else (None, None)   # (one behind the other: a small pass writes both itself)
+    ws = torch.empty(_workspace_bytes("casmvs_layer_norm_backward_workspace_bytes", code, outer, C, inner), dtype=torch.uint8, device=x.device)
+    with _on(x):
+        rc = _lib.load().casmvs_layer_norm_backward(x.data_ptr(), grad_y.data_ptr(), _at(weight), _at(bias), _at(gx), _at(gw), _at(gb), ws.data_ptr(), code, outer, C,
+                                                    inner, eps, slope, _stream(x))
+    _lib.check(rc, "casmvs_layer_norm_backward")
+    return gx, gw, gb
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, slope=1.0, channels_last=False):
     """Layer norm over the channel axis + leaky ReLU (casmvs_layer_norm_forward): x (N,C,*spatial) - or (..,C) with channels_last=True, the layout of the
     pixel-major feature maps -, float32 / float16 / bfloat16; weight, bias (C,) float32 or None -> x's shape and type.  slope 1: no activation.
     No autograd graph: autograd.layer_norm is the differentiable form."""
-    x, weight, bias, outer, C, inner = _layer_norm_args(x, weight, bias, eps, slope, channels_last)
-    y = torch.empty_like(x)
-    with _on(x):
-        rc = _lib.load().casmvs_layer_norm_forward(_at(x), _at(weight), _at(bias), _at(y), _DTYPES[x.dtype], outer, C, inner, float(eps), float(slope),
-                                                   _stream(x))
-    _lib.check(rc, "casmvs_layer_norm_forward")
-    return y
+    return _layer_norm_forward(*_layer_norm_args(x, weight, bias, eps, slope, channels_last), float(eps), float(slope))
 
 
 def layer_norm_backward(x, grad_y, weight=None, bias=None, eps=1e-5, slope=1.0, channels_last=False, need_x=True, need_affine=True):
     """The gradients of layer_norm at x (casmvs_layer_norm_backward; the statistics are recomputed) -> (grad_x or None, grad_weight, grad_bias or None)."""
-    x, weight, bias, outer, C, inner = _layer_norm_args(x, weight, bias, eps, slope, channels_last)
+    x, weight, bias, *sizes = _layer_norm_args(x, weight, bias, eps, slope, channels_last)
     grad_y = _same_device(x, _float_dev(grad_y, "grad_y"), "grad_y")
     if grad_y.shape != x.shape or grad_y.dtype != x.dtype:
         raise ValueError(f"layer_norm_backward: x {tuple(x.shape)} {x.dtype}, grad_y {tuple(grad_y.shape)} {grad_y.dtype}")
-    lib, code = _lib.load(), _DTYPES[x.dtype]
-    gx = torch.empty_like(x) if need_x else None
-    gw, gb = torch.empty((2, C), dtype=torch.float32, device=x.device).unbind() if need_affine else (None, None)
-    ws = torch.empty(_workspace_bytes("casmvs_layer_norm_backward_workspace_bytes", code, outer, C, inner), dtype=torch.uint8, device=x.device)
-    with _on(x):
-        rc = lib.casmvs_layer_norm_backward(_at(x), _at(grad_y), _at(weight), _at(bias), _at(gx), _at(gw), _at(gb), _at(ws), code, outer, C, inner,
-                                            float(eps), float(slope), _stream(x))
-    _lib.check(rc, "casmvs_layer_norm_backward")
-    return gx, gw, gb
+    return _layer_norm_backward(x, grad_y, weight, bias, *sizes, float(eps), float(slope), need_x, need_affine)
 
 
 class Packed8:

@@ -471,7 +471,7 @@ class _Kept8:
     def packed(self, buffer, shape, slope):
         """What the convolution behind takes as its checkpoint: y = lrelu(gamma xhat + beta)."""
         planes, nb = self.N * self.C, (self.n + 31) // 32
-        vec = buffer[self.vec:].view(torch.float32).view(4, self.C)
+        vec = buffer[self.vec:self.bytes].view(torch.float32).view(4, self.C)
         return ops.Packed8(buffer[:self.scales].view(planes, nb, 32), buffer[self.scales:self.scales + planes * nb].view(planes, nb), shape, torch.float32,
                            (vec[2], vec[3], slope))
 
@@ -485,8 +485,8 @@ class _ABNTrain8(torch.autograd.Function):
         N, C = x.shape[:2]
         n = x.numel() // (N * C)
         kept = _Kept8(N, C, n)
-        buffer = torch.empty(kept.bytes, dtype=torch.uint8, device=x.device)
-        ws = torch.empty(ops._workspace_bytes("casmvs_abn8_workspace_bytes", N, C, n), dtype=torch.uint8, device=x.device)
+        # (the forward's workspace, at most 16 KB, lies behind what is kept)
+        buffer = torch.empty(kept.bytes + ops._workspace_bytes("casmvs_abn8_workspace_bytes", N, C, n), dtype=torch.uint8, device=x.device)
         y = torch.empty_like(x)
         w, bta = weight.detach().contiguous().float(), beta.detach().contiguous().float()
         track = running_mean is not None and running_var is not None
@@ -494,7 +494,7 @@ class _ABNTrain8(torch.autograd.Function):
         with ops._on(x):
             rc = _lib.load().casmvs_abn8_forward_f32(x.data_ptr(), w.data_ptr(), bta.data_ptr(), abs_eps, eps, momentum, running_mean.data_ptr() if track else None,
                                                      running_var.data_ptr() if track else None, base + kept.vec, y.data_ptr(), base, base + kept.scales,
-                                                     base + kept.signs, ws.data_ptr(), N, C, n, slope, _stream(x))
+                                                     base + kept.signs, base + kept.bytes, N, C, n, slope, _stream(x))
         _lib.check(rc, "casmvs_abn8_forward_f32")
         if track:   # the kernel wrote the buffers behind torch's back: bump their version counters (packed-weight caches key on them)
             torch.autograd.graph.increment_version((running_mean, running_var))
