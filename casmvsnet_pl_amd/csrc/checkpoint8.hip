@@ -56,25 +56,41 @@ __device__ __forceinline__ void store4(T *p, int left, const float (&v)[4]) {
 __device__ __forceinline__ int left_of(size_t n, size_t first) { return first >= n ? 0 : n - first < 4 ? (int)(n - first) : 4; }
 
 // ---- pack / unpack ------------------------------------------------------------------------------------------------------------------------------------
+constexpr int kAhead = 4;   // blocks per group of eight lanes whose loads are issued together
+
+// Row and first value of a lane's four in block `blk` of (rows, nb); n % 32 == 0 came in as one long row.
+__device__ __forceinline__ void place_of(size_t blk, size_t rows, size_t nb, int lane, size_t &row, size_t &first) {
+  size_t in_row = blk;
+  row = 0;
+  if (rows > 1) casmvs::elem::divide(blk, nb, row, in_row);
+  first = in_row * kBlock + 4 * lane;
+}
+
 template <class T, bool WIDE>
 __global__ __launch_bounds__(kThreads) void pack8_kernel(const T *__restrict__ x, unsigned *__restrict__ codes, unsigned char *__restrict__ scales, size_t rows,
                                                         size_t n, size_t nb) {
-  const size_t total = rows * nb;
+  const size_t total = rows * nb, step = (size_t)gridDim.x * kGroups;
   const int lane = threadIdx.x & (kLanes - 1);
-  // every lane of a wave takes the same number of turns (the exchanges inside a block need its eight lanes); a turn past the end works on nothing
-  const size_t turns = (total + (size_t)gridDim.x * kGroups - 1) / ((size_t)gridDim.x * kGroups);
-  for (size_t turn = 0; turn < turns; ++turn) {
-    const size_t blk = (turn * gridDim.x + blockIdx.x) * kGroups + threadIdx.x / kLanes;
-    const bool live = blk < total;
-    const size_t row = live ? blk / nb : 0, first = (live ? blk % nb : 0) * kBlock + 4 * lane;
-    float v[4];
-    load4<T, WIDE>(x + row * n + first, live ? left_of(n, first) : 0, v);
-    const double d[4] = {v[0], v[1], v[2], v[3]};
-    unsigned scale;
-    const unsigned q = casmvs::block8::quantise(d, scale);
-    if (live) {
-      codes[blk * kLanes + lane] = q;
-      if (lane == 0) scales[blk] = (unsigned char)scale;
+  // every lane of a wave takes the same number of turns (the exchanges inside a block need its eight lanes); a block past the end is empty
+  for (size_t start = (size_t)blockIdx.x * kGroups; start < total; start += kAhead * step) {
+    float v[kAhead][4];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const size_t blk = start + k * step + threadIdx.x / kLanes;
+      size_t row, first;
+      place_of(blk < total ? blk : 0, rows, nb, lane, row, first);
+      load4<T, WIDE>(x + row * n + first, blk < total ? left_of(n, first) : 0, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const size_t blk = start + k * step + threadIdx.x / kLanes;
+      const double d[4] = {v[k][0], v[k][1], v[k][2], v[k][3]};
+      unsigned scale;
+      const unsigned q = casmvs::block8::quantise(d, scale);
+      if (blk < total) {
+        codes[blk * kLanes + lane] = q;
+        if (lane == 0) scales[blk] = (unsigned char)scale;
+      }
     }
   }
 }
@@ -84,24 +100,37 @@ template <class T, bool WIDE, bool AFFINE>
 __global__ __launch_bounds__(kThreads) void unpack8_kernel(const unsigned *__restrict__ codes, const unsigned char *__restrict__ scales, T *__restrict__ out,
                                                           const float *__restrict__ weight, const float *__restrict__ bias, int C, float slope, size_t rows,
                                                           size_t n, size_t nb) {
-  const size_t total = rows * nb, step_blocks = (size_t)gridDim.x * kGroups;
+  const size_t total = rows * nb, step = (size_t)gridDim.x * kGroups;
   const int lane = threadIdx.x & (kLanes - 1);
-  for (size_t blk = (size_t)blockIdx.x * kGroups + threadIdx.x / kLanes; blk < total; blk += step_blocks) {
-    const size_t row = blk / nb, first = (blk % nb) * kBlock + 4 * lane;
-    const float step = casmvs::block8::step_of(scales[blk]);
-    const unsigned q = codes[blk * kLanes + lane];
-    float v[4];
+  for (size_t start = (size_t)blockIdx.x * kGroups + threadIdx.x / kLanes; start < total; start += kAhead * step) {
+    unsigned q[kAhead], scale[kAhead];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = casmvs::block8::value_of(q, i, step);
-    if (AFFINE) {
-      const float w = weight[row % C], b = bias[row % C];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float z = fmaf(v[i], w, b);
-        v[i] = z > 0.0f ? z : z * slope;
-      }
+    for (int k = 0; k < kAhead; ++k) {
+      const size_t blk = start + k * step < total ? start + k * step : start;
+      q[k] = codes[blk * kLanes + lane];
+      scale[k] = scales[blk];
     }
-    store4<T, WIDE>(out + row * n + first, left_of(n, first), v);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const size_t blk = start + k * step;
+      if (blk >= total) break;
+      size_t row, first;
+      place_of(blk, rows, nb, lane, row, first);
+      const float per = casmvs::block8::step_of(scale[k]);
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = casmvs::block8::value_of(q[k], i, per);
+      if (AFFINE) {
+        const int c = rows <= 0xFFFFFFFFu ? (int)((unsigned)row % (unsigned)C) : (int)(row % C);
+        const float w = weight[c], b = bias[c];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float z = fmaf(v[i], w, b);
+          v[i] = z > 0.0f ? z : z * slope;
+        }
+      }
+      store4<T, WIDE>(out + row * n + first, left_of(n, first), v);
+    }
   }
 }
 
@@ -208,7 +237,6 @@ struct Store {     // the 8-bit checkpoint of the normalised input and the signs
   unsigned *signs;
 };
 // y and the checkpoint of the blocks blk0, blk0 + step, .. (kAhead of them, their loads issued together) of one plane.  Every lane of a wave comes here together.
-constexpr int kAhead = 4;
 template <bool WIDE>
 __device__ __forceinline__ void apply_blocks(const float *__restrict__ xp, float *__restrict__ yp, const Store &to, size_t base, size_t blk0, size_t step, size_t n,
                                              size_t nb, int lane, const Channel &c, float slope) {
@@ -246,13 +274,15 @@ __device__ __forceinline__ void apply_blocks(const float *__restrict__ xp, float
   }
 }
 
+// 512 threads: a pass that only reads needs more waves per CU than one that writes too (2 x 8 x 32 x 256 x 320 forward 111 us, with 256 threads 124; small maps lose with 1024)
+constexpr int kSumThreads = 512;
 template <bool WIDE>
-__global__ __launch_bounds__(kThreads) void abn8_sums_kernel(const float *__restrict__ x, double *__restrict__ out, int N, int C, size_t n) {
+__global__ __launch_bounds__(kSumThreads) void abn8_sums_kernel(const float *__restrict__ x, double *__restrict__ out, int N, int C, size_t n) {
   const int c = blockIdx.y;
   const size_t words = (n + 3) / 4, per = (words + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < words ? lo + per : words;
   double s0 = 0.0, s1 = 0.0;
-  add_squares<WIDE, kThreads>(x, N, C, c, n, lo, hi, s0, s1);
-  workgroup_sums<kThreads>(s0, s1);
+  add_squares<WIDE, kSumThreads>(x, N, C, c, n, lo, hi, s0, s1);
+  workgroup_sums<kSumThreads>(s0, s1);
   if (threadIdx.x == 0) {
     out[((size_t)c * gridDim.x + blockIdx.x) * 2] = s0;
     out[((size_t)c * gridDim.x + blockIdx.x) * 2 + 1] = s1;
@@ -347,13 +377,13 @@ __device__ __forceinline__ void add_gradients(const float *__restrict__ gy, cons
 }
 
 template <bool WIDE>
-__global__ __launch_bounds__(kThreads) void abn8_backward_sums_kernel(const float *__restrict__ gy, Checkpoint from, double *__restrict__ out, int N, int C, size_t n,
+__global__ __launch_bounds__(kSumThreads) void abn8_backward_sums_kernel(const float *__restrict__ gy, Checkpoint from, double *__restrict__ out, int N, int C, size_t n,
                                                                      size_t nb, float slope) {
   const int c = blockIdx.y;
   const size_t per = (nb + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < nb ? lo + per : nb;
   double s0 = 0.0, s1 = 0.0;
-  add_gradients<WIDE, kThreads>(gy, from, N, C, c, n, nb, lo, hi, slope, s0, s1);
-  workgroup_sums<kThreads>(s0, s1);
+  add_gradients<WIDE, kSumThreads>(gy, from, N, C, c, n, nb, lo, hi, slope, s0, s1);
+  workgroup_sums<kSumThreads>(s0, s1);
   if (threadIdx.x == 0) {
     out[((size_t)c * gridDim.x + blockIdx.x) * 2] = s0;
     out[((size_t)c * gridDim.x + blockIdx.x) * 2 + 1] = s1;
@@ -516,7 +546,7 @@ extern "C" int casmvs_abn8_forward_f32(const float *x, const float *weight, cons
     hipLaunchKernelGGL(wide ? abn8_forward_one_kernel<true> : abn8_forward_one_kernel<false>, dim3((unsigned)C), dim3(kWide), 0, st, x, count, norm, y, to, N, C, n, nb);
     return casmvs::check_launch("abn8_forward_one_kernel");
   }
-  hipLaunchKernelGGL(wide ? abn8_sums_kernel<true> : abn8_sums_kernel<false>, dim3((unsigned)parts, (unsigned)C), dim3(kThreads), 0, st, x, sums, N, C, n);
+  hipLaunchKernelGGL(wide ? abn8_sums_kernel<true> : abn8_sums_kernel<false>, dim3((unsigned)parts, (unsigned)C), dim3(kSumThreads), 0, st, x, sums, N, C, n);
   hipLaunchKernelGGL(wide ? abn8_apply_kernel<true> : abn8_apply_kernel<false>, dim3((unsigned)((size_t)N * C * chunks)), dim3(kThreads), 0, st, x, sums, parts, count, norm,
                      y, to, C, n, nb, (unsigned)chunks);
   return casmvs::check_launch("abn8_forward");
@@ -542,7 +572,7 @@ extern "C" int casmvs_abn8_backward_f32(const float *grad_y, const void *codes, 
     hipLaunchKernelGGL(wide ? abn8_backward_one_kernel<true> : abn8_backward_one_kernel<false>, dim3((unsigned)C), dim3(kWide), 0, st, grad_y, from, count, to, N, C, n, nb);
     return casmvs::check_launch("abn8_backward_one_kernel");
   }
-  hipLaunchKernelGGL(wide ? abn8_backward_sums_kernel<true> : abn8_backward_sums_kernel<false>, dim3((unsigned)parts, (unsigned)C), dim3(kThreads), 0, st, grad_y, from, sums,
+  hipLaunchKernelGGL(wide ? abn8_backward_sums_kernel<true> : abn8_backward_sums_kernel<false>, dim3((unsigned)parts, (unsigned)C), dim3(kSumThreads), 0, st, grad_y, from, sums,
                      N, C, n, nb, slope);
   // (without grad_x the workgroups of the channels' first chunks write the two vectors, and there are no others)
   const dim3 grid((unsigned)(grad_x ? (size_t)N * C * chunks : (size_t)C * chunks));

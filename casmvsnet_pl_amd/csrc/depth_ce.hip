@@ -25,8 +25,8 @@ struct Running {   // of one pixel over some of its hypotheses
   float cost_at, low, high;   // smallest / largest depth
 };
 
-// exp(a - m) where m may be -inf (then a is, too): 0
-__device__ __forceinline__ float exp_below(float a, float m) { return m == -INFINITY ? (a == -INFINITY ? 0.0f : expf(a)) : expf(a - m); }
+// exp(a - m) for a <= m by the hardware's 2^x, the argument rounded once more (2^-24 of at most 127, for a probability of 2^-127).  m may be -inf (then a is, too): 0.
+__device__ __forceinline__ float exp_below(float a, float m) { return __builtin_amdgcn_exp2f((a - (m == -INFINITY ? 0.0f : m)) * 1.44269504088896341f); }
 
 __device__ __forceinline__ void join(Running &r, const Running &o) {   // o: the hypotheses behind r's
   const float m = fmaxf(r.m, o.m);

@@ -25,6 +25,23 @@ __device__ __forceinline__ void store(T *p, const Vec<T, V> &v) {
   *reinterpret_cast<Vec<T, V> *>(p) = v;
 }
 
+// V consecutive floats on any 4-byte boundary, still as one access
+template <int V>
+struct __attribute__((packed, aligned(4))) Floats {
+  float v[V];
+};
+
+// a / b and a % b; in 32 bits where both fit (a 64-bit division is some 100 instructions)
+__device__ __forceinline__ void divide(size_t a, size_t b, size_t &quotient, size_t &rest) {
+  if (((a | b) >> 32) == 0) {
+    quotient = (unsigned)a / (unsigned)b;
+    rest = (unsigned)a - (unsigned)quotient * (unsigned)b;
+  } else {
+    quotient = a / b;
+    rest = a - quotient * b;
+  }
+}
+
 // The value of lane (own ^ d), d = 1, 2, 4 .. 32: inside a row of 16 lanes by data-parallel moves (quad permutes; 4 and 8 after the smaller steps of a sum, where
 // the mirror of 8 / 16 lanes holds the same value), beyond by the LDS crossbar.  For sums over lanes in the order 1, 2, 4, ..; all lanes active.
 __device__ __forceinline__ double lane_xor(double v, int d) {

@@ -5,17 +5,21 @@
 //   g = gy (z > 0 ? 1 : slope),  m1 = mean_c (g w),  m2 = mean_c (g w h):   gx = r (g w - m1 - h m2),  gw_c = sum_p g h,  gb_c = sum_p g
 //
 // The backward pass takes x and recomputes mu, r and the side of zero that z lies on: x has to be read for h anyway, and two stored floats per position
-// would be a quarter of the traffic at 8 channels.  Statistics, z and gx are held in 64 bits.  An element whose z is within float32's rounding of zero would
-// otherwise get the slope in one computation and 1 in another, an error of the size of the gradient itself, and at two or three channels gx is what is left
-// after cancellation.  The vector ALU does 64-bit multiply-adds at the rate of scalar float32 ones, and these kernels wait for memory.
+// would be a quarter of the traffic at 8 channels.
+//
+// What is 64 bits wide: the statistics and x - mu (a row far from zero keeps its spread), and the side of zero of a z that float32 cannot tell - an element
+// within its rounding of zero would otherwise get the slope in one computation and 1 in another, an error of the size of the gradient itself.  Those are
+// found by |z| <= 2^-18 |b| (near zero h w is about -b, and the float32 z is off by at most 4 * 2^-24 of it) and decided again from x; they are one in 10^5.
+// Everything else is float32 from the rounded x - mu on, but at fewer than 8 channels (FEW), where gx is what is left after cancellation: all 64 bits there.
 //
 // Three forms, by where a position's channels lie and how many there are:
-//   planes  (inner > 1, C <= 512)   a thread holds 8 channels of 4 (or 1) consecutive positions in registers, up to 64 threads share a position;
+//   planes  (inner > 1, C <= 512)   a thread holds 8 channels of 2 (or 1) consecutive positions in registers, up to 64 threads share a position;
 //   rows    (inner = 1, C <= 8192)  up to 64 lanes of a wave, or a workgroup, hold a row in registers;
 //   any     everything else: x is read once per use.
 #include "elem_types.h"
 
 namespace {
+using casmvs::elem::Floats;
 using casmvs::elem::lane_xor;
 using casmvs::elem::Vec;
 
@@ -70,25 +74,34 @@ struct PlaneTile {
 template <int CG, int V>
 constexpr int plane_lds(int most) { return CG == 1 ? 1 : most * kThreads * V + most * kThreads / CG * V; }
 
+// What a thread loads of a tile, as loaded; 0 for a channel or position that is not there
 template <class T, int V>
-__device__ __forceinline__ void load_planes(const T *__restrict__ x, size_t base, size_t inner, int first, int step, int C, bool live, float (&v)[kHeld][V]) {
+struct PlaneLoads {
+  Vec<T, V> t[kHeld];
+  template <bool FULL>
+  __device__ __forceinline__ void load(const T *__restrict__ x, size_t base, size_t inner, int first, int step, int C, bool live) {
 #pragma unroll
-  for (int r = 0; r < kHeld; ++r) {
-    const int c = first + r * step;
-    if (live && c < C) {
-      const Vec<T, V> t = casmvs::elem::load<T, V>(x + base + c * inner);
+    for (int r = 0; r < kHeld; ++r) {
+      const int c = first + r * step;
+      if (live && (FULL || c < C)) {
+        t[r] = casmvs::elem::load<T, V>(x + base + c * inner);
+      } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[r][i] = (float)t.v[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[r][i] = 0.0f;
+        for (int i = 0; i < V; ++i) t[r].v[i] = (T)0.0f;
+      }
     }
   }
-}
+  __device__ __forceinline__ void widen(float (&v)[kHeld][V]) const {
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r)
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[r][i] = (float)t[r].v[i];
+  }
+};
 
-// mean and 1 / sqrt(var + eps) of the thread's positions
-template <int MOST, int CG, int V>
-__device__ __forceinline__ void plane_statistics(const PlaneTile<CG, V> &tile, const float (&v)[kHeld][V], int C, double per_c, float eps, double *lds, double (&mean)[V],
+// mean and 1 / sqrt(var + eps) of the thread's positions; CENTRE: v becomes x - mean
+template <int MOST, bool CENTRE, bool FULL, int CG, int V>
+__device__ __forceinline__ void plane_statistics(const PlaneTile<CG, V> &tile, float (&v)[kHeld][V], int C, double per_c, float eps, double *lds, double (&mean)[V],
                                                  double (&rstd)[V]) {
   double s[1][V];
 #pragma unroll
@@ -105,11 +118,12 @@ __device__ __forceinline__ void plane_statistics(const PlaneTile<CG, V> &tile, c
   }
 #pragma unroll
   for (int r = 0; r < kHeld; ++r)
-    if (tile.cg + r * CG < C) {
+    if (FULL || tile.cg + r * CG < C) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const double d = (double)v[r][i] - mean[i];
         s[0][i] = fma(d, d, s[0][i]);
+        if (CENTRE) v[r][i] = (float)d;
       }
     }
   tile.template over_groups<1, MOST>(s, lds);
@@ -117,7 +131,25 @@ __device__ __forceinline__ void plane_statistics(const PlaneTile<CG, V> &tile, c
   for (int i = 0; i < V; ++i) rstd[i] = inverse_sqrt(s[0][i] * per_c + (double)eps);
 }
 
-template <class T, int CG, int V>
+// A float32 z of magnitude up to this cannot tell its side of zero.  slope 1: the side does not matter.
+__device__ __forceinline__ float near_zero(float bias, float slope) { return slope == 1.0f ? -1.0f : 0x1p-18f * fabsf(bias); }
+__device__ __forceinline__ double z_of(float x, double mean, double rstd, float w, float b) { return fma(((double)x - mean) * rstd, (double)w, (double)b); }
+
+// The thread's weights: kept over its tiles; 1 and 0 for what is missing
+template <int CG>
+struct PlaneWeights {
+  float w[kHeld], b[kHeld];
+  __device__ __forceinline__ PlaneWeights(const float *__restrict__ wp, const float *__restrict__ bp, int cg, int C) {
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) {
+      const int c = cg + r * CG < C ? cg + r * CG : C - 1;
+      w[r] = wp ? wp[c] : 1.0f;
+      b[r] = bp ? bp[c] : 0.0f;
+    }
+  }
+};
+
+template <class T, int CG, int V, bool FEW>
 __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__restrict__ x, const float *__restrict__ w, const float *__restrict__ b,
                                                                     T *__restrict__ y, size_t positions, int C, size_t inner, double per_c, float eps,
                                                                     float slope) {
@@ -125,67 +157,141 @@ __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__
   const PlaneTile<CG, V> tile;
   const size_t p = ((size_t)blockIdx.x * PlaneTile<CG, V>::PL + tile.pl) * V;
   const bool live = p < positions;   // (V divides inner: all V positions or none, in one plane)
-  const size_t n = live ? p / inner : 0, base = n * C * inner + (live ? p - n * inner : 0);
+  size_t n, at;
+  casmvs::elem::divide(live ? p : 0, inner, n, at);
+  const size_t base = n * C * inner + at;
+  PlaneLoads<T, V> xs;
+  xs.template load<false>(x, base, inner, tile.cg, CG, C, live);
+  const PlaneWeights<CG> a(w, b, tile.cg, C);
   float v[kHeld][V];
-  load_planes<T, V>(x, base, inner, tile.cg, CG, C, live, v);
+  xs.widen(v);
   double mean[V], rstd[V];
-  plane_statistics<1, CG, V>(tile, v, C, per_c, eps, lds, mean, rstd);
+  plane_statistics<1, !FEW, false, CG, V>(tile, v, C, per_c, eps, lds, mean, rstd);
   if (!live) return;
 #pragma unroll
   for (int r = 0; r < kHeld; ++r) {
     const int c = tile.cg + r * CG;
     if (c >= C) break;
-    const double wc = w ? (double)w[c] : 1.0, bc = b ? (double)b[c] : 0.0;
     Vec<T, V> t;
+    bool near = FEW;   // (a channel's store leaves as soon as its z are known: one test for all of them holds every store back, 62 -> 70 us at 2 x 8 x 32 x 256 x 320)
+    if (!FEW) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const double z = fma(((double)v[r][i] - mean[i]) * rstd[i], wc, bc);
-      t.v[i] = (T)(float)(z > 0.0 ? z : z * slope);
+      for (int i = 0; i < V; ++i) {
+        const float z = v[r][i] * (float)rstd[i] * a.w[r] + a.b[r];
+        near |= fabsf(z) <= near_zero(a.b[r], slope);
+        t.v[i] = (T)(z > 0.0f ? z : z * slope);
+      }
+    }
+    if (near) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const double z = z_of(FEW ? v[r][i] : (float)x[base + c * inner + i], mean[i], rstd[i], a.w[r], a.b[r]);
+        t.v[i] = (T)(float)(z > 0.0 ? z : z * slope);
+      }
     }
     casmvs::elem::store<T, V>(y + base + c * inner, t);
   }
 }
 
+// How the backward pass counts its channels: fewer than 8 (all in 64 bits), any number, or exactly 8 per group (no test at a channel).  The forward pass has no
+// form of the last kind: without the tests the compiler holds every channel's values at once, 88 registers instead of 56, and the pass is 15 % slower.
+enum Channels { kFew, kSome, kFull };
+
 // gx, and of every workgroup the sums over its tiles of g h and g per channel: partial[workgroup][0 / 1][c].  AFFINE: the weight gradient is wanted.
-template <class T, int CG, int V, bool AFFINE>
+template <class T, int CG, int V, bool AFFINE, Channels CH>
 __global__ __launch_bounds__(kThreads) void ln_backward_planes_kernel(const T *__restrict__ x, const T *__restrict__ gy, const float *__restrict__ w,
                                                                      const float *__restrict__ b, T *__restrict__ gx, float *__restrict__ partial,
                                                                      size_t positions, size_t tiles, int C, size_t inner, double per_c, float eps, float slope) {
   using Tile = PlaneTile<CG, V>;
+  constexpr bool FEW = CH == kFew, FULL = CH == kFull;
   constexpr int kSums = plane_lds<CG, V>(2) > 2 * kHeld * kThreads / 2 ? plane_lds<CG, V>(2) : 2 * kHeld * kThreads / 2;
   __shared__ double lds[kSums];   // (the groups' sums; at the end 2 * kHeld * 256 floats)
   const Tile tile;
+  const PlaneWeights<CG> a(w, b, tile.cg, C);
   float sw[kHeld], sb[kHeld];   // this thread's share of sum g h and sum g: positions / (workgroups * PL) values each
 #pragma unroll
   for (int r = 0; r < kHeld; ++r) sw[r] = sb[r] = 0.0f;
-  for (size_t k = blockIdx.x; k < tiles; k += gridDim.x) {
+  // The next tile's loads are issued before this one is worked on: with two waves per SIMD three quarters of the time went by waiting for them
+  PlaneLoads<T, V> xs, gs;
+  size_t base_ahead;
+  bool live_ahead;
+  auto load_ahead = [&](size_t k) {
     const size_t p = (k * Tile::PL + tile.pl) * V;
-    const bool live = p < positions;
-    const size_t n = live ? p / inner : 0, base = n * C * inner + (live ? p - n * inner : 0);
+    live_ahead = k < tiles && p < positions;
+    size_t n, at;
+    casmvs::elem::divide(live_ahead ? p : 0, inner, n, at);
+    base_ahead = n * C * inner + at;
+    xs.template load<FULL>(x, base_ahead, inner, tile.cg, CG, C, live_ahead);
+    gs.template load<FULL>(gy, base_ahead, inner, tile.cg, CG, C, live_ahead);
+  };
+  load_ahead(blockIdx.x);
+  for (size_t k = blockIdx.x; k < tiles; k += gridDim.x) {
+    const size_t base = base_ahead;
+    const bool live = live_ahead;
     float v[kHeld][V], g[kHeld][V];
-    load_planes<T, V>(x, base, inner, tile.cg, CG, C, live, v);
-    load_planes<T, V>(gy, base, inner, tile.cg, CG, C, live, g);
+    xs.widen(v);
+    gs.widen(g);
+    if (k + gridDim.x < tiles) load_ahead(k + gridDim.x);
     double mean[V], rstd[V], m[2][V];
-    plane_statistics<2, CG, V>(tile, v, C, per_c, eps, lds, mean, rstd);
+    plane_statistics<2, !FEW, FULL, CG, V>(tile, v, C, per_c, eps, lds, mean, rstd);
+    if (FEW) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) m[0][i] = m[1][i] = 0.0;
+      for (int i = 0; i < V; ++i) m[0][i] = m[1][i] = 0.0;
 #pragma unroll
-    for (int r = 0; r < kHeld; ++r) {
-      const int c = tile.cg + r * CG;
-      if (c < C) {
-        const double wc = w ? (double)w[c] : 1.0, bc = b ? (double)b[c] : 0.0;
+      for (int r = 0; r < kHeld; ++r)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const double h = ((double)v[r][i] - mean[i]) * rstd[i];
-          g[r][i] *= fma(h, wc, bc) > 0.0 ? 1.0f : slope;
-          const double gw = (double)g[r][i] * wc;
+          g[r][i] *= fma(h, (double)a.w[r], (double)a.b[r]) > 0.0 ? 1.0f : slope;
+          const double gw = (double)g[r][i] * (double)a.w[r];
           m[0][i] += gw;
           m[1][i] = fma(gw, h, m[1][i]);
           if (AFFINE) {
-            sb[r] += g[r][i];
             sw[r] = fmaf(g[r][i], (float)h, sw[r]);
+            sb[r] += g[r][i];
           }
         }
+    } else {
+      bool near = false;
+#pragma unroll
+      for (int r = 0; r < kHeld; ++r)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          v[r][i] *= (float)rstd[i];   // h from here on
+          const float z = v[r][i] * a.w[r] + a.b[r];
+          near |= fabsf(z) <= near_zero(a.b[r], slope);
+          g[r][i] *= z > 0.0f ? 1.0f : slope;
+        }
+      if (near && live) {
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) {
+          const int c = tile.cg + r * CG;
+          if (FULL || c < C) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+              g[r][i] = (float)gy[base + c * inner + i] * (z_of((float)x[base + c * inner + i], mean[i], rstd[i], a.w[r], a.b[r]) > 0.0 ? 1.0f : slope);
+          }
+        }
+      }
+      float f[2][V];   // sum g w and sum g w h over this thread's 8 channels; in 64 bits over the groups
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[0][i] = f[1][i] = 0.0f;
+#pragma unroll
+      for (int r = 0; r < kHeld; ++r)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float gw = g[r][i] * a.w[r];
+          f[0][i] += gw;
+          f[1][i] = fmaf(gw, v[r][i], f[1][i]);
+          if (AFFINE) {
+            sw[r] = fmaf(g[r][i], v[r][i], sw[r]);
+            sb[r] += g[r][i];
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        m[0][i] = f[0][i];
+        m[1][i] = f[1][i];
       }
     }
     if (gx) {
@@ -199,13 +305,16 @@ __global__ __launch_bounds__(kThreads) void ln_backward_planes_kernel(const T *_
 #pragma unroll
         for (int r = 0; r < kHeld; ++r) {
           const int c = tile.cg + r * CG;
-          if (c >= C) break;
-          const double wc = w ? (double)w[c] : 1.0;
+          if (!FULL && c >= C) break;
           Vec<T, V> t;
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const double h = ((double)v[r][i] - mean[i]) * rstd[i];
-            t.v[i] = (T)(float)(rstd[i] * ((double)g[r][i] * wc - m[0][i] - h * m[1][i]));
+            if (FEW) {
+              const double h = ((double)v[r][i] - mean[i]) * rstd[i];
+              t.v[i] = (T)(float)(rstd[i] * ((double)g[r][i] * (double)a.w[r] - m[0][i] - h * m[1][i]));
+            } else {
+              t.v[i] = (T)((float)rstd[i] * (g[r][i] * a.w[r] - (float)m[0][i] - v[r][i] * (float)m[1][i]));
+            }
           }
           casmvs::elem::store<T, V>(gx + base + c * inner, t);
         }
@@ -248,17 +357,18 @@ __device__ __forceinline__ void over_row(double (&v)[N], double *lds) {
 #pragma unroll
     for (int d = 1; d < (L < 64 ? L : 64); d <<= 1) v[k] += lane_xor(v[k], d);
   if (L > 64) {
-    constexpr int W = L / 64;
+    constexpr int W = L / 64, waves = row_threads<L>() / 64;
+    const int wave = threadIdx.x >> 6, first = wave / W * W;   // the row's first wave
     __syncthreads();   // (lds may still be read from the last use)
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int k = 0; k < N; ++k) lds[k * W + (threadIdx.x >> 6)] = v[k];
+      for (int k = 0; k < N; ++k) lds[k * waves + wave] = v[k];
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      v[k] = lds[k * W];
+      v[k] = lds[k * waves + first];
 #pragma unroll
-      for (int i = 1; i < W; ++i) v[k] += lds[k * W + i];
+      for (int i = 1; i < W; ++i) v[k] += lds[k * waves + first + i];
     }
   }
 }
@@ -279,8 +389,9 @@ __device__ __forceinline__ void load_row(const T *__restrict__ x, size_t base, i
   }
 }
 
-template <int L, int V, int K>
-__device__ __forceinline__ void row_statistics(const float (&v)[K][V], int t, int C, double per_c, float eps, double *lds, double &mean, double &rstd) {
+// (as plane_statistics)
+template <int L, int V, int K, bool CENTRE>
+__device__ __forceinline__ void row_statistics(float (&v)[K][V], int t, int C, double per_c, float eps, double *lds, double &mean, double &rstd) {
   double s[1] = {0.0};
 #pragma unroll
   for (int j = 0; j < K; ++j)
@@ -296,15 +407,16 @@ __device__ __forceinline__ void row_statistics(const float (&v)[K][V], int t, in
       for (int i = 0; i < V; ++i) {
         const double d = (double)v[j][i] - mean;
         s[0] = fma(d, d, s[0]);
+        if (CENTRE) v[j][i] = (float)d;
       }
     }
   over_row<L, 1>(s, lds);
   rstd = inverse_sqrt(s[0] * per_c + (double)eps);
 }
 
-template <class T, int L, int V, int K>
+template <class T, int L, int V, int K, bool FEW>
 __global__ __launch_bounds__(row_threads<L>()) void ln_forward_rows_kernel(const T *__restrict__ x, const float *__restrict__ w, const float *__restrict__ b, T *__restrict__ y,
-                                                                  size_t rows, int C, double per_c, float eps, float slope) {
+                                                                          size_t rows, int C, double per_c, float eps, float slope) {
   __shared__ double lds[row_threads<L>() / 64];
   const int t = threadIdx.x % L;
   const size_t row = (size_t)blockIdx.x * (row_threads<L>() / L) + threadIdx.x / L;
@@ -313,27 +425,46 @@ __global__ __launch_bounds__(row_threads<L>()) void ln_forward_rows_kernel(const
   float v[K][V];
   load_row<T, L, V, K>(x, base, t, C, live, v);
   double mean, rstd;
-  row_statistics<L, V, K>(v, t, C, per_c, eps, lds, mean, rstd);
+  row_statistics<L, V, K, !FEW>(v, t, C, per_c, eps, lds, mean, rstd);
   if (!live) return;
 #pragma unroll
   for (int j = 0; j < K; ++j) {
     const int c = (j * L + t) * V;
     if (c >= C) break;
-    Vec<T, V> u;
+    Floats<V> wc, bc;   // (V divides C)
+    if (w) wc = *reinterpret_cast<const Floats<V> *>(w + c);
+    if (b) bc = *reinterpret_cast<const Floats<V> *>(b + c);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const double z = fma(((double)v[j][i] - mean) * rstd, w ? (double)w[c + i] : 1.0, b ? (double)b[c + i] : 0.0);
-      u.v[i] = (T)(float)(z > 0.0 ? z : z * slope);
+      if (!w) wc.v[i] = 1.0f;
+      if (!b) bc.v[i] = 0.0f;
+    }
+    Vec<T, V> u;
+    bool near = FEW;
+    if (!FEW) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float z = v[j][i] * (float)rstd * wc.v[i] + bc.v[i];
+        near |= fabsf(z) <= near_zero(bc.v[i], slope);
+        u.v[i] = (T)(z > 0.0f ? z : z * slope);
+      }
+    }
+    if (near) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const double z = z_of(FEW ? v[j][i] : (float)x[base + c + i], mean, rstd, wc.v[i], bc.v[i]);
+        u.v[i] = (T)(float)(z > 0.0 ? z : z * slope);
+      }
     }
     casmvs::elem::store<T, V>(y + base + c, u);
   }
 }
 
 // gx, and of every workgroup the sums over its rows of g h and g: a thread keeps its channels for all of them.  partial[workgroup][0 / 1][c].
-template <class T, int L, int V, int K, bool AFFINE>
+template <class T, int L, int V, int K, bool AFFINE, bool FEW>
 __global__ __launch_bounds__(row_threads<L>()) void ln_backward_rows_kernel(const T *__restrict__ x, const T *__restrict__ gy, const float *__restrict__ w,
-                                                                   const float *__restrict__ b, T *__restrict__ gx, float *__restrict__ partial, size_t rows,
-                                                                   int C, double per_c, float eps, float slope) {
+                                                                           const float *__restrict__ b, T *__restrict__ gx, float *__restrict__ partial, size_t rows,
+                                                                           int C, double per_c, float eps, float slope) {
   constexpr int BT = row_threads<L>(), G = BT / L;   // rows at a time
   __shared__ double lds[2 * BT / 64];
   __shared__ float red[AFFINE && G > 1 ? K * V * BT : 1];
@@ -355,25 +486,59 @@ __global__ __launch_bounds__(row_threads<L>()) void ln_backward_rows_kernel(cons
     const size_t base = live ? row * C : 0;
     float v[K][V], g[K][V];
     load_row<T, L, V, K>(x, base, t, C, live, v);
-    load_row<T, L, V, K>(gy, base, t, C, live, g);
+    load_row<T, L, V, K>(gy, base, t, C, live, g);   // (g of a missing channel or row is 0)
     double mean, rstd, m[2] = {0.0, 0.0};
-    row_statistics<L, V, K>(v, t, C, per_c, eps, lds, mean, rstd);
+    row_statistics<L, V, K, !FEW>(v, t, C, per_c, eps, lds, mean, rstd);
+    const float r32 = (float)rstd;
+    float f0 = 0.0f, f1 = 0.0f;   // sum g w and sum g w h over this thread's channels; in 64 bits over the row
 #pragma unroll
-    for (int j = 0; j < K; ++j)
+    for (int j = 0; j < K; ++j) {
+      if (FEW) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {   // (g of a missing channel is 0)
-        const double h = ((double)v[j][i] - mean) * rstd;
-        g[j][i] *= fma(h, (double)wc[j][i], (double)bc[j][i]) > 0.0 ? 1.0f : slope;
-        const double gw = (double)g[j][i] * (double)wc[j][i];
-        m[0] += gw;
-        m[1] = fma(gw, h, m[1]);
-        if (AFFINE && live) {
-          sb[j][i] += g[j][i];
-          sw[j][i] = fmaf(g[j][i], (float)h, sw[j][i]);
+        for (int i = 0; i < V; ++i) {
+          const double h = ((double)v[j][i] - mean) * rstd;
+          g[j][i] *= fma(h, (double)wc[j][i], (double)bc[j][i]) > 0.0 ? 1.0f : slope;
+          const double gw = (double)g[j][i] * (double)wc[j][i];
+          m[0] += gw;
+          m[1] = fma(gw, h, m[1]);
+          if (AFFINE && live) sw[j][i] = fmaf(g[j][i], (float)h, sw[j][i]);
+        }
+      } else {
+        bool near = false;
+        float factor[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          v[j][i] *= r32;   // h from here on
+          const float z = v[j][i] * wc[j][i] + bc[j][i];
+          near |= fabsf(z) <= near_zero(bc[j][i], slope);
+          factor[i] = z > 0.0f ? 1.0f : slope;
+        }
+        const int c = (j * L + t) * V;
+        if (near && live && c < C) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) factor[i] = z_of((float)x[base + c + i], mean, rstd, wc[j][i], bc[j][i]) > 0.0 ? 1.0f : slope;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          g[j][i] *= factor[i];
+          const float gw = g[j][i] * wc[j][i];
+          f0 += gw;
+          f1 = fmaf(gw, v[j][i], f1);
+          if (AFFINE && live) sw[j][i] = fmaf(g[j][i], v[j][i], sw[j][i]);
         }
       }
+      if (AFFINE && live) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sb[j][i] += g[j][i];
+      }
+    }
     if (gx) {
+      if (!FEW) {
+        m[0] = f0;
+        m[1] = f1;
+      }
       over_row<L, 2>(m, lds);
+      const float m0 = (float)(m[0] * per_c), m1 = (float)(m[1] * per_c);
       if (live) {
 #pragma unroll
         for (int j = 0; j < K; ++j) {
@@ -382,8 +547,12 @@ __global__ __launch_bounds__(row_threads<L>()) void ln_backward_rows_kernel(cons
           Vec<T, V> u;
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const double h = ((double)v[j][i] - mean) * rstd;
-            u.v[i] = (T)(float)(rstd * ((double)g[j][i] * (double)wc[j][i] - m[0] * per_c - h * (m[1] * per_c)));
+            if (FEW) {
+              const double h = ((double)v[j][i] - mean) * rstd;
+              u.v[i] = (T)(float)(rstd * ((double)g[j][i] * (double)wc[j][i] - m[0] * per_c - h * (m[1] * per_c)));
+            } else {
+              u.v[i] = (T)(r32 * (g[j][i] * wc[j][i] - m0 - v[j][i] * m1));
+            }
           }
           casmvs::elem::store<T, V>(gx + base + c, u);
         }
@@ -612,9 +781,10 @@ int slices_of(size_t positions) {
 enum Form { kAny, kPlanes, kRows };
 Form form_of(int C, size_t inner) { return inner == 1 ? (C <= 8192 ? kRows : kAny) : (C <= 64 * kHeld ? kPlanes : kAny); }
 
-// workgroups of the fused backward pass = rows of its partial sums: two per CU keep the memory busy (every thread has 16 loads in flight), and the finishing
-// kernel reads few of them
-constexpr size_t kBackwardBlocks = 512;
+// Workgroups of the fused backward pass = rows of its partial sums.  Three per CU are resident (registers) and keep the memory busiest: bf16 2 x 8 x 32 x 256 x 320
+// 49 us with 768, 54 with 512, 57 with 1024.  Past 256 channels a row of sums is as long as a row of data and there are few rows: 8191 x 1000 bf16 30 us
+// with 512, 39 with 768 (rows 983040 x 32: 83 and 72).
+size_t backward_blocks(int C) { return C > 256 ? 512 : 768; }
 
 bool fits(const void *p, size_t bytes) { return p == nullptr || ((uintptr_t)p & (bytes - 1)) == 0; }
 
@@ -646,53 +816,59 @@ struct Call {   // arguments of either direction
   }
 };
 
-template <class T, int CG, int V>
+template <class T, int CG, int V, Channels CH>
 void planes(const Call &a, int &parts) {
   const size_t tile = (size_t)(kThreads / CG) * V, tiles = (a.positions() + tile - 1) / tile;
   if (!a.gy) {
-    hipLaunchKernelGGL((ln_forward_planes_kernel<T, CG, V>), dim3((unsigned)tiles), dim3(kThreads), 0, a.stream, (const T *)a.x, a.w, a.b, (T *)a.out, a.positions(), a.C,
-                       a.inner, 1.0 / a.C, a.eps, a.slope);
+    hipLaunchKernelGGL((ln_forward_planes_kernel<T, CG, V, CH == kFew>), dim3((unsigned)tiles), dim3(kThreads), 0, a.stream, (const T *)a.x, a.w, a.b, (T *)a.out, a.positions(),
+                       a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
     return;
   }
-  const unsigned grid = (unsigned)(tiles < kBackwardBlocks ? tiles : kBackwardBlocks);
+  const unsigned grid = (unsigned)(tiles < backward_blocks(a.C) ? tiles : backward_blocks(a.C));
   parts = (int)grid;
   float *sums = a.sums(parts);
-  auto kernel = a.partial ? ln_backward_planes_kernel<T, CG, V, true> : ln_backward_planes_kernel<T, CG, V, false>;
+  auto kernel = a.partial ? ln_backward_planes_kernel<T, CG, V, true, CH> : ln_backward_planes_kernel<T, CG, V, false, CH>;
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0, a.stream, (const T *)a.x, (const T *)a.gy, a.w, a.b, (T *)a.out, sums, a.positions(), tiles,
                      a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
 }
 template <class T, int V>
 void planes_by_groups(const Call &a, int &parts) {
-  const int groups = (a.C + kHeld - 1) / kHeld;
-  if (groups <= 1) planes<T, 1, V>(a, parts);
-  else if (groups <= 2) planes<T, 2, V>(a, parts);
-  else if (groups <= 4) planes<T, 4, V>(a, parts);
-  else if (groups <= 8) planes<T, 8, V>(a, parts);
-  else if (groups <= 16) planes<T, 16, V>(a, parts);
-  else planes<T, 64, V>(a, parts);
+  switch (a.C) {
+    case kHeld: return planes<T, 1, V, kFull>(a, parts);
+    case 2 * kHeld: return planes<T, 2, V, kFull>(a, parts);
+    case 4 * kHeld: return planes<T, 4, V, kFull>(a, parts);
+    case 8 * kHeld: return planes<T, 8, V, kFull>(a, parts);
+    default: break;
+  }
+  if (a.C < kHeld) planes<T, 1, V, kFew>(a, parts);
+  else if (a.C <= 2 * kHeld) planes<T, 2, V, kSome>(a, parts);
+  else if (a.C <= 4 * kHeld) planes<T, 4, V, kSome>(a, parts);
+  else if (a.C <= 8 * kHeld) planes<T, 8, V, kSome>(a, parts);
+  else if (a.C <= 16 * kHeld) planes<T, 16, V, kSome>(a, parts);
+  else planes<T, 64, V, kSome>(a, parts);
 }
 
-template <class T, int L, int V, int K>
+template <class T, int L, int V, int K, bool FEW = false>
 void rows(const Call &a, int &parts) {
   constexpr int threads = row_threads<L>();
   const size_t blocks = (a.outer + threads / L - 1) / (threads / L);
   if (!a.gy) {
-    hipLaunchKernelGGL((ln_forward_rows_kernel<T, L, V, K>), dim3((unsigned)blocks), dim3(threads), 0, a.stream, (const T *)a.x, a.w, a.b, (T *)a.out, a.outer, a.C,
+    hipLaunchKernelGGL((ln_forward_rows_kernel<T, L, V, K, FEW>), dim3((unsigned)blocks), dim3(threads), 0, a.stream, (const T *)a.x, a.w, a.b, (T *)a.out, a.outer, a.C,
                        1.0 / a.C, a.eps, a.slope);
     return;
   }
-  const unsigned grid = (unsigned)(blocks < kBackwardBlocks ? blocks : kBackwardBlocks);
+  const unsigned grid = (unsigned)(blocks < backward_blocks(a.C) ? blocks : backward_blocks(a.C));
   parts = (int)grid;
   float *sums = a.sums(parts);
-  auto kernel = a.partial ? ln_backward_rows_kernel<T, L, V, K, true> : ln_backward_rows_kernel<T, L, V, K, false>;
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, a.stream, (const T *)a.x, (const T *)a.gy, a.w, a.b, (T *)a.out, sums, a.outer, a.C,
-                     1.0 / a.C, a.eps, a.slope);
+  auto kernel = a.partial ? ln_backward_rows_kernel<T, L, V, K, true, FEW> : ln_backward_rows_kernel<T, L, V, K, false, FEW>;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, a.stream, (const T *)a.x, (const T *)a.gy, a.w, a.b, (T *)a.out, sums, a.outer, a.C, 1.0 / a.C, a.eps, a.slope);
 }
 template <class T, int V>
 void rows_by_width(const Call &a, int &parts) {
   const int vectors = (a.C + V - 1) / V;
   constexpr int k16 = 16 / V;   // 16 channels per lane
-  if (vectors <= 4) rows<T, 4, V, 1>(a, parts);
+  if (a.C < kHeld) rows<T, 8 / V, V, 1, true>(a, parts);
+  else if (vectors <= 4) rows<T, 4, V, 1>(a, parts);
   else if (vectors <= 8) rows<T, 8, V, 1>(a, parts);
   else if (vectors <= 16) rows<T, 16, V, 1>(a, parts);
   else if (vectors <= 64) rows<T, 64, V, 1>(a, parts);
@@ -710,7 +886,7 @@ void run_form(Form form, int dtype, const Call &a, int &parts) {
     const size_t bytes = 4 * sizeof(T);
     const bool wide = (form == kRows ? a.C : a.inner) % 4 == 0 && fits(a.x, bytes) && fits(a.gy, bytes) && fits(a.out, bytes);
     if (form == kPlanes) {
-      if (wide) planes_by_groups<T, 4>(a, parts); else planes_by_groups<T, 1>(a, parts);
+      if (wide) planes_by_groups<T, 2>(a, parts); else planes_by_groups<T, 1>(a, parts);
     } else {
       if (wide) rows_by_width<T, 4>(a, parts); else rows_by_width<T, 1>(a, parts);
     }
@@ -744,7 +920,7 @@ extern "C" int casmvs_layer_norm_forward(const void *x, const float *weight, con
 extern "C" size_t casmvs_layer_norm_backward_workspace_bytes(int dtype, size_t outer, int C, size_t inner) {
   if (!casmvs::elem::known(dtype) || C <= 0) return 0;
   const size_t positions = outer * inner;
-  if (form_of(C, inner) != kAny) return (positions < kBackwardBlocks ? positions : kBackwardBlocks) * 2 * C * sizeof(float) + 16;
+  if (form_of(C, inner) != kAny) return (positions < backward_blocks(C) ? positions : backward_blocks(C)) * 2 * C * sizeof(float) + 16;
   return positions * 16 + (size_t)slices_of(positions) * 2 * C * 8 + 16;
 }
 

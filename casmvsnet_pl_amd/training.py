@@ -32,6 +32,8 @@ import torch
 from . import _lib, ops
 from . import autograd as A
 from ._lib import CONV_S1, CONV_S2, CONV_T2, CONV2D_K3, CONV2D_K5S2, CONV2D_K1
+from .inplace_abn import InPlaceABN
+from .norm import LayerNormAct
 
 _3D = (CONV_S1, CONV_S2, CONV_T2)
 
@@ -488,8 +490,11 @@ class _ABNTrain8(torch.autograd.Function):
         # (the forward's workspace, at most 16 KB, lies behind what is kept)
         buffer = torch.empty(kept.bytes + ops._workspace_bytes("casmvs_abn8_workspace_bytes", N, C, n), dtype=torch.uint8, device=x.device)
         y = torch.empty_like(x)
-        w, bta = weight.detach().contiguous().float(), beta.detach().contiguous().float()
+        w, bta = weight.contiguous().float(), beta.contiguous().float()   # (themselves, as a rule)
         track = running_mean is not None and running_var is not None
+        for t in (w, bta, running_mean, running_var) if track else (w, bta):
+            if t.shape != (C,) or t.dtype != torch.float32 or t.device != x.device or not t.is_contiguous():
+                raise ValueError(f"abn_train: x {tuple(x.shape)} on {x.device}, a parameter or running statistic is {tuple(t.shape)} {t.dtype} on {t.device}")
         base = buffer.data_ptr()
         with ops._on(x):
             rc = _lib.load().casmvs_abn8_forward_f32(x.data_ptr(), w.data_ptr(), bta.data_ptr(), abs_eps, eps, momentum, running_mean.data_ptr() if track else None,
@@ -525,8 +530,6 @@ def abn_train(norm, x, checkpoint="f32"):
     leaky-relu slope): inplace_abn.ABN (gamma = weight) or InPlaceABN (gamma = |weight| + eps, see inplace_abn.py); of a norm.LayerNormAct: layer norm.
     checkpoint "8bit": what is kept for the backward pass is 8 bits of the normalised input + one bit per element (x and y in float32 otherwise).  Layer
     norm keeps its float32 input in either case."""
-    from .inplace_abn import InPlaceABN
-    from .norm import LayerNormAct
     _check_checkpoint(checkpoint)
     if isinstance(norm, LayerNormAct):
         return norm(x.float())

@@ -7,6 +7,7 @@
 // what these sources use beyond the emulated subset
 inline double hipemu_rsq(double a) { return (double)(float)(1.0 / std::sqrt(a)); }   // an estimate of 24 bits
 #define __builtin_amdgcn_rsq hipemu_rsq
+#define __builtin_amdgcn_exp2f(x) exp2f(x)
 inline int hipemu_bpermute(int from, int v) { return hipemu_lane_exchange(v, (from >> 2) & 63); }
 #define __builtin_amdgcn_ds_bpermute hipemu_bpermute
 
@@ -59,7 +60,7 @@ static void layer_norm_check(const char *name, int dtype, double half_step, size
     for (int c = 0; c < C; ++c) {
       const double h = (value(x[base + c * inner]) - mean) * r, wc = affine ? w[c] : 1.0, z = h * wc + (affine ? b[c] : 0.0);
       const double want = z > 0 ? z : z * slope, g = value(gy[base + c * inner]) * (z > 0 ? 1.0 : slope);
-      ey = std::fmax(ey, std::fabs(value(y[base + c * inner]) - want) / (std::fabs(want) * half_step + 1e-7));
+      ey = std::fmax(ey, std::fabs(value(y[base + c * inner]) - want) / (std::fabs(want) * half_step + 0x1p-24 * (4 * std::fabs(h * wc) + 2 * std::fabs(z)) + 1e-12));
       m1 += g * wc / C;
       m2 += g * wc * h / C;
       sw[c] += g * h;
