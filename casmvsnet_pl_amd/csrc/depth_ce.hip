@@ -5,8 +5,9 @@
 //
 // One pass over the hypothesis axis with the running maximum m and the sum s of exp(c_k - m); what the backward pass needs beside the costs is m, 1 / s and
 // t (12 bytes per pixel), never a volume of probabilities.  m and 1 / s are kept apart: their sum m + log s, rounded to float32, would move every
-// probability by the rounding of a number as large as the costs.  The distances to gt are formed in 64 bits, where the differences of float32 depths are exact, so
-// which of two planes is the nearer one does not depend on a rounding.
+// probability by the rounding of a number as large as the costs.  The distances to gt are compared in float32; rounding keeps their order or makes two of them
+// equal, and only where equal ones were met they are compared again in 64 bits, where differences of float32 depths are exact: which of two planes is the nearer one does not
+// depend on a rounding.
 // Both passes wait for memory: forward cost + depth value per hypothesis, backward cost in and gradient out.  A pixel whose mask is not set reads nothing.
 #include "elem_types.h"
 
@@ -14,56 +15,65 @@ namespace {
 using casmvs::elem::Vec;
 
 constexpr int kThreads = 256;
-constexpr int kPixels = 64;               // pixels per workgroup
-constexpr int kPieces = kThreads / kPixels;   // pieces of the hypothesis axis, joined at the end
-constexpr int kChunk = 8;                 // hypotheses loaded before they are used
+constexpr int kChunk = 8;   // hypotheses loaded before they are used
 
 struct Running {   // of one pixel over some of its hypotheses
-  float m, s;              // the largest cost, sum of exp(cost - m)
-  double near;             // the smallest distance to gt, where it is and the cost there
+  float m, s;         // the largest cost, sum of exp(cost - m)
+  float near;         // the smallest distance to gt, rounded to float32, and where it is first
   int at;
-  float cost_at, low, high;   // smallest / largest depth
+  float low, high;    // smallest / largest depth
 };
 
 // exp(a - m) for a <= m by the hardware's 2^x, the argument rounded once more (2^-24 of at most 127, for a probability of 2^-127).  m may be -inf (then a is, too): 0.
 __device__ __forceinline__ float exp_below(float a, float m) { return __builtin_amdgcn_exp2f((a - (m == -INFINITY ? 0.0f : m)) * 1.44269504088896341f); }
 
-__device__ __forceinline__ void join(Running &r, const Running &o) {   // o: the hypotheses behind r's
+// Is depth `a` nearer to `gt` than `b`, whose rounded distances are equal?
+__device__ __forceinline__ bool nearer(float a, float b, float gt) { return __builtin_fabs((double)a - (double)gt) < __builtin_fabs((double)b - (double)gt); }
+
+// o: the hypotheses behind r's; dp, dstep: the pixel's depths
+__device__ __forceinline__ void join(Running &r, const Running &o, const float *__restrict__ dp, size_t dstep, float gt) {
   const float m = fmaxf(r.m, o.m);
   r.s = r.s * exp_below(r.m, m) + o.s * exp_below(o.m, m);
   r.m = m;
-  if (o.near < r.near) {
-    r.near = o.near;
-    r.at = o.at;
-    r.cost_at = o.cost_at;
-  }
+  bool take = o.near < r.near;
+  if (o.near == r.near) take = nearer(dp[o.at * dstep], dp[r.at * dstep], gt);
+  r.at = take ? o.at : r.at;
+  r.near = fminf(r.near, o.near);
   r.low = fminf(r.low, o.low);
   r.high = fmaxf(r.high, o.high);
 }
 
-template <class T, bool PER_PIXEL>
+// PIECES threads share a pixel: each takes its piece of the hypothesis axis, joined at the end
+template <class T, bool PER_PIXEL, int PIECES>
 __global__ __launch_bounds__(kThreads) void depth_ce_forward_kernel(const T *__restrict__ cost, const float *__restrict__ depth, const float *__restrict__ gt,
                                                                    const unsigned char *__restrict__ mask, float2 *__restrict__ stats, int *__restrict__ target,
                                                                    double *__restrict__ partial, size_t pixels, int D, size_t hw) {
+  constexpr int kPixels = kThreads / PIECES;
   const int lane = threadIdx.x % kPixels, piece = threadIdx.x / kPixels;
   const size_t p = (size_t)blockIdx.x * kPixels + lane;
   const bool live = p < pixels && (!mask || mask[p]);
-  const size_t b = live ? p / hw : 0, s = live ? p % hw : 0;
-  Running r = {-INFINITY, 0.0f, INFINITY, 0, 0.0f, INFINITY, -INFINITY};
+  size_t b, s;
+  casmvs::elem::divide(live ? p : 0, hw, b, s);
+  Running r = {-INFINITY, 0.0f, INFINITY, 0, INFINITY, -INFINITY};
+  float true_depth = 0.0f;
+  const T *cp = cost + (b * D) * hw + s;
+  const float *dp = PER_PIXEL ? depth + (b * D) * hw + s : depth + b * D;
+  const size_t dstep = PER_PIXEL ? hw : 1;
   if (live) {
-    const int per = (D + kPieces - 1) / kPieces, lo = piece * per, hi = lo + per < D ? lo + per : D;
-    const double true_depth = gt[p];
-    const T *cp = cost + (b * D) * hw + s;
-    const float *dp = PER_PIXEL ? depth + (b * D) * hw + s : depth + b * D;
+    const int per = (D + PIECES - 1) / PIECES, lo = piece * per, hi = lo + per < D ? lo + per : D;
+    true_depth = gt[p];
     for (int k0 = lo; k0 < hi; k0 += kChunk) {
       float c[kChunk], d[kChunk];
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) {
         const int k = k0 + i < hi ? k0 + i : hi - 1;
         c[i] = (float)cp[(size_t)k * hw];
-        d[i] = dp[PER_PIXEL ? (size_t)k * hw : (size_t)k];
+        d[i] = dp[k * dstep];
       }
       float m = r.m;
+      const float near = r.near;
+      const int at = r.at;
+      bool tied = false;
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) m = fmaxf(m, c[i]);
       r.s *= exp_below(r.m, m);
@@ -72,33 +82,48 @@ __global__ __launch_bounds__(kThreads) void depth_ce_forward_kernel(const T *__r
       for (int i = 0; i < kChunk; ++i)
         if (k0 + i < hi) {
           r.s += exp_below(c[i], m);
-          const double far = __builtin_fabs((double)d[i] - true_depth);
-          if (far < r.near) {
-            r.near = far;
-            r.at = k0 + i;
-            r.cost_at = c[i];
-          }
+          const float far = fabsf(d[i] - true_depth);
+          tied |= far == r.near;
+          r.at = far < r.near ? k0 + i : r.at;
+          r.near = fminf(r.near, far);
           r.low = fminf(r.low, d[i]);
           r.high = fmaxf(r.high, d[i]);
         }
+      if (tied) {   // two roundings were equal (a lane in thousands): the chunk again, in 64 bits where they are
+        r.near = near;
+        r.at = at;
+        float depth_at = dp[at * dstep];
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+          const float far = fabsf(d[i] - true_depth);
+          if (k0 + i < hi && (far < r.near || (far == r.near && nearer(d[i], depth_at, true_depth)))) {
+            r.near = far;
+            r.at = k0 + i;
+            depth_at = d[i];
+          }
+        }
+      }
     }
   }
-  __shared__ Running joined[kPieces][kPixels];
+  __shared__ Running joined[PIECES > 1 ? kThreads : 1];
   __shared__ double red[2][kPixels];
-  joined[piece][lane] = r;
-  __syncthreads();
+  if (PIECES > 1) {
+    joined[piece * kPixels + lane] = r;
+    __syncthreads();
+  }
   if (piece == 0) {
-    for (int q = 1; q < kPieces; ++q) join(r, joined[q][lane]);
+    for (int q = 1; q < PIECES; ++q) join(r, joined[q * kPixels + lane], dp, dstep, true_depth);
     bool counted = false;
+    float cost_at = 0.0f;
     if (live) {
-      const float g = gt[p];
-      counted = g >= r.low && g <= r.high && !(r.m == -INFINITY && r.s == 0.0f);
+      counted = true_depth >= r.low && true_depth <= r.high && !(r.m == -INFINITY && r.s == 0.0f);
+      cost_at = (float)cp[(size_t)r.at * hw];
     }
     if (p < pixels) {
       stats[p] = float2{counted ? r.m : 0.0f, counted ? 1.0f / r.s : 0.0f};
       target[p] = counted ? r.at : -1;
     }
-    red[0][lane] = counted ? (double)(logf(r.s) + (r.m - r.cost_at)) : 0.0;
+    red[0][lane] = counted ? (double)(logf(r.s) + (r.m - cost_at)) : 0.0;
     red[1][lane] = counted ? 1.0 : 0.0;
   }
   __syncthreads();
@@ -146,14 +171,15 @@ __global__ __launch_bounds__(kThreads) void depth_ce_backward_kernel(const T *__
                                                                     T *__restrict__ grad, size_t pixels, int D, size_t hw) {
   const size_t p = (size_t)blockIdx.x * kThreads + threadIdx.x;
   if (p >= pixels) return;
-  const size_t b = p / hw, s = p % hw;
+  size_t b, s;
+  casmvs::elem::divide(p, hw, b, s);
   const int t = target[p];
   const float2 st = stats[p];
   const float share = *share_of_one * *gloss;
   const int per = (D + (int)gridDim.y - 1) / (int)gridDim.y, lo = (int)blockIdx.y * per, hi = lo + per < D ? lo + per : D;
   const T *cp = cost + (b * D) * hw + s;
   T *gp = grad + (b * D) * hw + s;
-#pragma unroll 4
+#pragma unroll 8
   for (int k = lo; k < hi; ++k) {
     const float q = t < 0 ? 0.0f : (exp_below((float)cp[(size_t)k * hw], st.x) * st.y - (k == t ? 1.0f : 0.0f)) * share;
     gp[(size_t)k * hw] = (T)q;
@@ -165,12 +191,15 @@ int check_sizes(const char *what, int dtype, int B, int D, size_t hw) {
   CASMVS_REQUIRE(B > 0 && D > 0 && D <= 65536 && hw < ((size_t)1 << 36) / (size_t)B, "%s: B=%d D=%d h*w=%zu", what, B, D, hw);
   return CASMVS_OK;
 }
-size_t forward_blocks(size_t pixels) { return (pixels + kPixels - 1) / kPixels; }
+// Pieces of the hypothesis axis: few pixels with many hypotheses would leave CUs idle, each thread walking its axis alone.  1 or 4 pieces, us: 32 hypotheses of
+// 163840 pixels 14.3 / 15.8, 48 of 40960 10.9 / 9.4, 192 of 118400 38 / 30, 256 of 20480 42 / 17.
+int pieces_of(size_t pixels, int D) { return D < 16 || pixels >= (D <= 32 ? 65536u : 524288u) ? 1 : pixels >= 2048 || D < 64 ? 4 : 16; }
+size_t forward_blocks(size_t pixels, int D) { return (pixels * pieces_of(pixels, D) + kThreads - 1) / kThreads; }
 }  // namespace
 
 extern "C" size_t casmvs_depth_ce_workspace_bytes(int B, int D, size_t hw) {
   if (B <= 0 || D <= 0) return 0;
-  return forward_blocks((size_t)B * hw) * 16 + 16;
+  return forward_blocks((size_t)B * hw, D) * 16 + 16;
 }
 
 extern "C" int casmvs_depth_ce_forward(const void *cost, const float *depth_values, const float *depth_gt, const void *mask, float *stats, int *target,
@@ -178,13 +207,16 @@ extern "C" int casmvs_depth_ce_forward(const void *cost, const float *depth_valu
   casmvs::clear_error();
   if (int rc = check_sizes("depth_ce_forward", dtype, B, D, hw)) return rc;
   CASMVS_REQUIRE(loss && share && workspace, "depth_ce_forward: null pointer");
-  const size_t pixels = (size_t)B * hw, blocks = pixels ? forward_blocks(pixels) : 0;
+  const size_t pixels = (size_t)B * hw, blocks = pixels ? forward_blocks(pixels, D) : 0;
   CASMVS_REQUIRE(!pixels || (cost && depth_values && depth_gt && stats && target), "depth_ce_forward: null pointer");
   hipStream_t st = (hipStream_t)stream;
   double *partial = (double *)workspace;
   if (pixels) {
     CASMVS_WITH_DTYPE(dtype, {
-      auto kernel = per_pixel ? depth_ce_forward_kernel<T, true> : depth_ce_forward_kernel<T, false>;
+      const int pieces = pieces_of(pixels, D);
+      auto kernel = pieces == 1   ? (per_pixel ? depth_ce_forward_kernel<T, true, 1> : depth_ce_forward_kernel<T, false, 1>)
+                    : pieces == 4 ? (per_pixel ? depth_ce_forward_kernel<T, true, 4> : depth_ce_forward_kernel<T, false, 4>)
+                                  : (per_pixel ? depth_ce_forward_kernel<T, true, 16> : depth_ce_forward_kernel<T, false, 16>);
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, (const T *)cost, depth_values, depth_gt, (const unsigned char *)mask,
                          (float2 *)stats, target, partial, pixels, D, hw);
     });
