@@ -466,7 +466,8 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 int check_planes(const char *what, int N, int C, size_t n) {
   CASMVS_REQUIRE(N > 0 && C > 0 && C <= 65535 && n > 0, "%s: N=%d C=%d n=%zu", what, N, C, n);
   const size_t chunks = (blocks_of(n) + kTurns * kGroups - 1) / (kTurns * kGroups);
-  CASMVS_REQUIRE((size_t)N * C <= ((size_t)1 << 31) / 1024 && chunks < ((size_t)1 << 31) / ((size_t)N * C), "%s: %d x %d planes of %zu elements", what, N, C, n);
+  // (a launch has fewer than 2^32 threads)
+  CASMVS_REQUIRE((size_t)N * C <= ((size_t)1 << 21) && chunks < ((size_t)1 << 24) / ((size_t)N * C), "%s: %d x %d planes of %zu elements", what, N, C, n);
   return CASMVS_OK;
 }
 }  // namespace

@@ -188,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void depth_ce_backward_kernel(const T *__
 
 int check_sizes(const char *what, int dtype, int B, int D, size_t hw) {
   CASMVS_REQUIRE(casmvs::elem::known(dtype), "%s: dtype %d", what, dtype);
-  CASMVS_REQUIRE(B > 0 && D > 0 && D <= 65536 && hw < ((size_t)1 << 36) / (size_t)B, "%s: B=%d D=%d h*w=%zu", what, B, D, hw);
+  CASMVS_REQUIRE(B > 0 && D > 0 && D <= 65536 && hw < ((size_t)1 << 31) / (size_t)B, "%s: B=%d D=%d h*w=%zu (B h w < 2^31)", what, B, D, hw);
   return CASMVS_OK;
 }
 // Pieces of the hypothesis axis: few pixels with many hypotheses would leave CUs idle, each thread walking its axis alone.  1 or 4 pieces, us: 32 hypotheses of

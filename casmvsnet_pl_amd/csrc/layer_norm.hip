@@ -151,11 +151,11 @@ struct PlaneWeights {
 
 template <class T, int CG, int V, bool FEW>
 __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__restrict__ x, const float *__restrict__ w, const float *__restrict__ b,
-                                                                    T *__restrict__ y, size_t positions, int C, size_t inner, double per_c, float eps,
-                                                                    float slope) {
+                                                                    T *__restrict__ y, size_t first, size_t positions, int C, size_t inner, double per_c,
+                                                                    float eps, float slope) {
   __shared__ double lds[plane_lds<CG, V>(1)];
   const PlaneTile<CG, V> tile;
-  const size_t p = ((size_t)blockIdx.x * PlaneTile<CG, V>::PL + tile.pl) * V;
+  const size_t p = ((first + blockIdx.x) * PlaneTile<CG, V>::PL + tile.pl) * V;
   const bool live = p < positions;   // (V divides inner: all V positions or none, in one plane)
   size_t n, at;
   casmvs::elem::divide(live ? p : 0, inner, n, at);
@@ -416,10 +416,10 @@ __device__ __forceinline__ void row_statistics(float (&v)[K][V], int t, int C, d
 
 template <class T, int L, int V, int K, bool FEW>
 __global__ __launch_bounds__(row_threads<L>()) void ln_forward_rows_kernel(const T *__restrict__ x, const float *__restrict__ w, const float *__restrict__ b, T *__restrict__ y,
-                                                                          size_t rows, int C, double per_c, float eps, float slope) {
+                                                                          size_t first, size_t rows, int C, double per_c, float eps, float slope) {
   __shared__ double lds[row_threads<L>() / 64];
   const int t = threadIdx.x % L;
-  const size_t row = (size_t)blockIdx.x * (row_threads<L>() / L) + threadIdx.x / L;
+  const size_t row = (first + blockIdx.x) * (row_threads<L>() / L) + threadIdx.x / L;
   const bool live = row < rows;
   const size_t base = live ? row * C : 0;
   float v[K][V];
@@ -786,14 +786,19 @@ Form form_of(int C, size_t inner) { return inner == 1 ? (C <= 8192 ? kRows : kAn
 // with 512, 39 with 768 (rows 983040 x 32: 83 and 72).
 size_t backward_blocks(int C) { return C > 256 ? 512 : 768; }
 
+// A launch has fewer than 2^32 threads: a larger forward pass (more than 2^31 elements and up) goes in several
+constexpr size_t kLaunchBlocks = (size_t)1 << 22;
+unsigned launch_blocks(size_t left) { return (unsigned)(left < kLaunchBlocks ? left : kLaunchBlocks); }
+
 bool fits(const void *p, size_t bytes) { return p == nullptr || ((uintptr_t)p & (bytes - 1)) == 0; }
 
 int check_sizes(const char *what, int dtype, size_t outer, int C, size_t inner) {
   CASMVS_REQUIRE(casmvs::elem::known(dtype), "%s: dtype %d", what, dtype);
   CASMVS_REQUIRE(C > 0 && C <= 65535, "%s: C=%d (1 .. 65535)", what, C);
-  // (launches are at least one workgroup per row / per 64 positions)
-  CASMVS_REQUIRE(inner == 0 || outer <= ((size_t)1 << 36) / inner, "%s: %zu x %zu positions", what, outer, inner);
-  CASMVS_REQUIRE(inner != 1 || outer < ((size_t)1 << 31), "%s: %zu rows", what, outer);
+  // rows / planes: what a launch's block count holds; any: 256 threads per row / per 64 positions in one launch
+  const Form form = form_of(C, inner);
+  const size_t most = form == kRows ? ((size_t)1 << 31) - 1 : form == kPlanes ? (size_t)1 << 36 : inner == 1 ? ((size_t)1 << 24) - 1 : ((size_t)1 << 30) - 64;
+  CASMVS_REQUIRE(inner == 0 || outer <= most / inner, "%s: %zu x %zu positions of %d channels (at most %zu)", what, outer, inner, C, most);
   return CASMVS_OK;
 }
 
@@ -820,8 +825,9 @@ template <class T, int CG, int V, Channels CH>
 void planes(const Call &a, int &parts) {
   const size_t tile = (size_t)(kThreads / CG) * V, tiles = (a.positions() + tile - 1) / tile;
   if (!a.gy) {
-    hipLaunchKernelGGL((ln_forward_planes_kernel<T, CG, V, CH == kFew>), dim3((unsigned)tiles), dim3(kThreads), 0, a.stream, (const T *)a.x, a.w, a.b, (T *)a.out, a.positions(),
-                       a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
+    for (size_t first = 0; first < tiles; first += kLaunchBlocks)
+      hipLaunchKernelGGL((ln_forward_planes_kernel<T, CG, V, CH == kFew>), dim3(launch_blocks(tiles - first)), dim3(kThreads), 0, a.stream, (const T *)a.x, a.w, a.b,
+                         (T *)a.out, first, a.positions(), a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
     return;
   }
   const unsigned grid = (unsigned)(tiles < backward_blocks(a.C) ? tiles : backward_blocks(a.C));
@@ -853,8 +859,9 @@ void rows(const Call &a, int &parts) {
   constexpr int threads = row_threads<L>();
   const size_t blocks = (a.outer + threads / L - 1) / (threads / L);
   if (!a.gy) {
-    hipLaunchKernelGGL((ln_forward_rows_kernel<T, L, V, K, FEW>), dim3((unsigned)blocks), dim3(threads), 0, a.stream, (const T *)a.x, a.w, a.b, (T *)a.out, a.outer, a.C,
-                       1.0 / a.C, a.eps, a.slope);
+    for (size_t first = 0; first < blocks; first += kLaunchBlocks)
+      hipLaunchKernelGGL((ln_forward_rows_kernel<T, L, V, K, FEW>), dim3(launch_blocks(blocks - first)), dim3(threads), 0, a.stream, (const T *)a.x, a.w, a.b, (T *)a.out,
+                         first, a.outer, a.C, 1.0 / a.C, a.eps, a.slope);
     return;
   }
   const unsigned grid = (unsigned)(blocks < backward_blocks(a.C) ? blocks : backward_blocks(a.C));

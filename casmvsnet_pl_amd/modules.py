@@ -33,10 +33,12 @@ class ConvBnReLU(nn.Module):
     def forward(self, x):
         if not x.is_cuda:
             raise RuntimeError("casmvsnet_pl_amd.ConvBnReLU runs on the MI355X only; there is no CPU fallback")
-        if self.training or isinstance(self.bn, LayerNormAct):   # batch statistics / layer norm (training.py); an autograd graph in train mode
+        if self.training:   # batch statistics, autograd graph (training.py)
             from .training import conv_bn_relu_2d
-            with torch.set_grad_enabled(self.training and torch.is_grad_enabled()):
-                return conv_bn_relu_2d(self, x.float())
+            return conv_bn_relu_2d(self, x.float())
+        if isinstance(self.bn, LayerNormAct):   # it does not fold into the convolution
+            from .training import conv_bn_relu_2d, without_graph
+            return without_graph(conv_bn_relu_2d, self, x.float())
         kind = self._KINDS.get(self._geometry)
         if kind is None:
             raise RuntimeError(f"ConvBnReLU: (kernel, stride, pad) = {self._geometry} is not one of the layer shapes of "
@@ -80,10 +82,12 @@ class ConvBnReLU3D(nn.Module):
     def forward(self, x):
         if not x.is_cuda:
             raise RuntimeError("casmvsnet_pl_amd.ConvBnReLU3D runs on the MI355X only; there is no CPU fallback")
-        if self.training or isinstance(self.bn, LayerNormAct):   # batch statistics / layer norm (training.py); an autograd graph in train mode
+        if self.training:   # batch statistics, autograd graph (training.py)
             from .training import conv_bn_relu_3d
-            with torch.set_grad_enabled(self.training and torch.is_grad_enabled()):
-                return conv_bn_relu_3d(self, x.float())
+            return conv_bn_relu_3d(self, x.float())
+        if isinstance(self.bn, LayerNormAct):   # it does not fold into the convolution
+            from .training import conv_bn_relu_3d, without_graph
+            return without_graph(conv_bn_relu_3d, self, x.float())
         kind = {(3, 1, 1): ops.CONV_S1, (3, 2, 1): ops.CONV_S2}.get(self._geometry)
         if kind is None:
             raise RuntimeError(f"ConvBnReLU3D: (kernel, stride, pad) = {self._geometry} is not a CostRegNet layer shape "

@@ -226,9 +226,8 @@ class FeatureNet(_PackedWeights, nn.Module):
             from .training import feature_net_train
             return feature_net_train(self, x.float())
         if not self.foldable:   # layer norm: the layer-by-layer forward, without a graph
-            from .training import feature_net_train
-            with torch.no_grad():
-                return feature_net_train(self, x.float())
+            from .training import feature_net_train, without_graph
+            return without_graph(feature_net_train, self, x.float())
         N, _, H, W = x.shape
         if self.tail_mode not in ("splitf16", "f32"):
             raise ValueError(f"FeatureNet.tail_mode={self.tail_mode!r} (splitf16 or f32)")
@@ -383,9 +382,8 @@ class CostRegNet(_PackedWeights, nn.Module):
             from .training import cost_reg_net_train
             return cost_reg_net_train(self, x)
         if not self.foldable:   # layer norm: the layer-by-layer forward, without a graph
-            from .training import cost_reg_net_train
-            with torch.no_grad():
-                return cost_reg_net_train(self, x.float())
+            from .training import cost_reg_net_train, without_graph
+            return without_graph(cost_reg_net_train, self, x.float())
         B, _, D, h, w = x.shape
         packed = self.packed_layers(x.device)
         need = ops.costreg_workspace_bytes(B, D, h, w)

@@ -18,8 +18,9 @@ softmax + depth regression (mvsnet.py:175-177)         autograd.softmax_depth_re
 
 What a step keeps for its backward pass: float32 tensors (checkpoint="f32": the convolutions' inputs, ABN's input and output), or with checkpoint="8bit"
 (CascadeMVSNet.checkpoint_mode) 8-bit checkpoints: an ABN keeps 8 bits of its normalised input and one bit per element, the convolution behind it rebuilds its
-input from the same bytes, and a convolution whose input is anything else (a cost volume, a skip sum) packs that.  The forward pass is the same to float32's
-rounding; the gradients carry the rounding of the 8 bits.
+input from the same bytes (behind a layer norm: from the norm's input, exactly), and a convolution whose input is anything else (a cost volume, a skip sum)
+packs that.  The forward pass is the same to float32's rounding; the gradients carry the rounding of the 8 bits.  One step at 640x512, 3 views: peak memory
+2.31 -> 0.84 GiB with ABN, 2.06 -> 1.32 GiB with layer norm; 1 % and 6 % more time.
 
 torch is the autograd tape and the allocator; the skip additions of the U-Net and the gradient accumulation are torch adds.  Nothing here runs on CPU tensors.  DESIGN.md 2.6 has the kernels and the measured step
 times (18 ms per step at the reference's default training configuration, 15 ms captured as one hipGraph).
@@ -354,13 +355,13 @@ class _Conv(torch.autograd.Function):
 
 def conv(x, weight, bias, kind, checkpoint="f32"):
     """Differentiable convolution of one of the model's layer kinds (forward, input, weight and bias gradients in HIP).
-    checkpoint "8bit": the weight gradient is taken at an 8-bit checkpoint of x - the one that the ABN which made x keeps already, or a new one.  An x that no
-    gradient goes to (the images) is kept as it is: its owner holds it anyway."""
+    checkpoint "8bit": x is not kept.  The weight gradient is taken at what the norm that made x keeps already - an ABN's 8 bits; the input of a layer norm, which
+    forms x again exactly - or at a new 8-bit checkpoint of x.  An x that no gradient goes to (the images) is kept as it is: its owner holds it anyway."""
     if not x.is_cuda:
         raise RuntimeError("casmvsnet_pl_amd.training runs on the MI355X only; there is no CPU fallback")
     _check_checkpoint(checkpoint)
     if checkpoint == "8bit" and x.requires_grad and weight.requires_grad and torch.is_grad_enabled():
-        return _Conv8.apply(x, weight, bias, kind, packed_input(x))
+        return _Conv8.apply(x, weight, bias, kind, kept_input(x))
     return _Conv.apply(x, weight, bias, kind)
 
 
@@ -373,27 +374,23 @@ def _check_checkpoint(checkpoint):
 
 
 class _Conv8(torch.autograd.Function):
-    """_Conv that keeps its input as a Packed8: the weight gradient is taken at the unpacked values (one more pass over them, 33/32 + 4 bytes per element)."""
+    """_Conv that keeps, instead of its input, `kept` = (tensors, rebuild): the weight gradient is taken at rebuild(*tensors), one more pass over the input."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, kind, packed):
+    def forward(ctx, x, weight, bias, kind, kept):
         x = x.contiguous().float()
         ctx.kind, ctx.has_bias, ctx.shape = kind, bias is not None, tuple(x.shape)
-        affine = packed.affine or (None, None, 1.0)
-        ctx.slope = affine[2]
-        ctx.save_for_backward(weight, packed.codes, packed.scales, affine[0], affine[1])
+        tensors, ctx.rebuild = kept
+        ctx.save_for_backward(weight, *tensors)
         return _conv_raw(kind, weight, bias, x)
 
     @staticmethod
     @A._once
     def backward(ctx, gy):
-        weight, codes, scales, aff_w, aff_b = ctx.saved_tensors
+        weight, *tensors = ctx.saved_tensors
         gy = gy.contiguous().float()
         gx = conv_dgrad(ctx.kind, weight, gy, ctx.shape) if ctx.needs_input_grad[0] else None
-        gw = None
-        if ctx.needs_input_grad[1]:
-            x = ops.unpack8(ops.Packed8(codes, scales, ctx.shape, torch.float32, None if aff_w is None else (aff_w, aff_b, ctx.slope)))
-            gw = conv_wgrad(ctx.kind, x, gy, tuple(weight.shape))
+        gw = conv_wgrad(ctx.kind, ctx.rebuild(*tensors), gy, tuple(weight.shape)) if ctx.needs_input_grad[1] else None
         gb = channel_sums(gy)[0].float() if (ctx.has_bias and ctx.needs_input_grad[2]) else None
         return gx, gw, gb, None, None
 
@@ -470,12 +467,11 @@ class _Kept8:
         self.vec = (self.signs + 4 * blocks + 15) // 16 * 16
         self.bytes = self.vec + 16 * C
 
-    def packed(self, buffer, shape, slope):
-        """What the convolution behind takes as its checkpoint: y = lrelu(gamma xhat + beta)."""
+    def packed(self, buffer):
+        """codes, scales, gamma, beta: y = lrelu(gamma xhat + beta)."""
         planes, nb = self.N * self.C, (self.n + 31) // 32
         vec = buffer[self.vec:self.bytes].view(torch.float32).view(4, self.C)
-        return ops.Packed8(buffer[:self.scales].view(planes, nb, 32), buffer[self.scales:self.scales + planes * nb].view(planes, nb), shape, torch.float32,
-                           (vec[2], vec[3], slope))
+        return buffer[:self.scales].view(planes, nb, 32), buffer[self.scales:self.scales + planes * nb].view(planes, nb), vec[2], vec[3]
 
 
 class _ABNTrain8(torch.autograd.Function):
@@ -514,9 +510,8 @@ class _ABNTrain8(torch.autograd.Function):
         buffer, w = ctx.saved_tensors
         gy = gy.contiguous().float()
         k = ctx.kept
-        gw, gb = torch.empty((2, k.C), dtype=torch.float32, device=gy.device).unbind()
+        gw, gb, ws = ops._affine_gradients(k.C, ops._workspace_bytes("casmvs_abn8_workspace_bytes", k.N, k.C, k.n), gy.device)
         gx = torch.empty_like(gy) if ctx.needs_input_grad[0] else None
-        ws = torch.empty(ops._workspace_bytes("casmvs_abn8_workspace_bytes", k.N, k.C, k.n), dtype=torch.uint8, device=gy.device)
         base = buffer.data_ptr()
         with ops._on(gy):
             rc = _lib.load().casmvs_abn8_backward_f32(gy.data_ptr(), base, base + k.scales, base + k.signs, w.data_ptr(), ctx.abs_eps, base + k.vec, gw.data_ptr(),
@@ -528,11 +523,15 @@ class _ABNTrain8(torch.autograd.Function):
 def abn_train(norm, x, checkpoint="f32"):
     """Train-mode forward of an ABN-like module (`weight`, `bias`, `running_mean`, `running_var`, `eps`, `momentum`,
     leaky-relu slope): inplace_abn.ABN (gamma = weight) or InPlaceABN (gamma = |weight| + eps, see inplace_abn.py); of a norm.LayerNormAct: layer norm.
-    checkpoint "8bit": what is kept for the backward pass is 8 bits of the normalised input + one bit per element (x and y in float32 otherwise).  Layer
-    norm keeps its float32 input in either case."""
+    checkpoint "8bit": what ABN keeps for the backward pass is 8 bits of the normalised input + one bit per element (x and y in float32 otherwise).  Layer
+    norm keeps its float32 input in either case; with "8bit" the convolution behind it keeps nothing of its own."""
     _check_checkpoint(checkpoint)
     if isinstance(norm, LayerNormAct):
-        return norm(x.float())
+        x = x.contiguous().float()
+        y = norm(x)
+        if checkpoint == "8bit":
+            y._casmvs_made_by = (y._version, norm, x)
+        return y
     if not getattr(norm, "affine", True) or norm.weight is None:
         raise RuntimeError("training: ABN without affine parameters is not supported")
     if isinstance(norm, InPlaceABN):
@@ -541,7 +540,7 @@ def abn_train(norm, x, checkpoint="f32"):
         weight, abs_eps = (norm._gamma() if hasattr(norm, "_gamma") else norm.weight), -1.0
     slope = norm.leaky_slope() if hasattr(norm, "leaky_slope") else float(getattr(norm, "activation_param", 0.01))
     args = (x, weight, norm.bias, norm.running_mean, norm.running_var, float(norm.momentum), float(norm.eps), slope, abs_eps)
-    if checkpoint == "f32":
+    if checkpoint == "f32" or not torch.is_grad_enabled():
         return _ABNTrain.apply(*args)
     if not x.is_cuda:
         raise RuntimeError("casmvsnet_pl_amd.training runs on the MI355X only; there is no CPU fallback")
@@ -549,17 +548,30 @@ def abn_train(norm, x, checkpoint="f32"):
         raise ValueError(f"abn_train: x {tuple(x.shape)} has no batch to normalise over")
     y, buffer = _ABNTrain8.apply(*args)
     if y.dim() > 2:
-        y._casmvs_packed8 = (buffer, slope, y._version)
+        y._casmvs_made_by = (y._version, buffer, slope)
     return y
 
 
-def packed_input(x):
-    """The 8-bit checkpoint of a convolution's input: the one that the ABN which made x keeps already, or a new one."""
-    buffer, slope, version = getattr(x, "_casmvs_packed8", (None, None, None))
-    if buffer is None or version != x._version:   # not an ABN's output, or written to since
-        return ops.pack8(x.detach().float())
+def _unpack(shape, slope):
+    return lambda codes, scales, *affine: ops.unpack8(ops.Packed8(codes, scales, shape, torch.float32, (*affine, slope) if affine else None))
+
+
+def kept_input(x):
+    """What a convolution keeps of its input x under checkpoint "8bit": (tensors, the function that makes x of them, to 8 bits or exactly)."""
+    version, *made_by = getattr(x, "_casmvs_made_by", (None,))
+    if version is None or version != x._version:   # not a norm's output, or written to since
+        packed = ops.pack8(x.detach().float())
+        return (packed.codes, packed.scales), _unpack(tuple(x.shape), 1.0)
+    if isinstance(made_by[0], LayerNormAct):
+        norm, source = made_by
+        eps, slope = norm.eps, norm.leaky_slope()
+        if norm.affine:
+            return (source.detach(), norm.weight.detach(), norm.bias.detach()), lambda t, w, b: ops.layer_norm(t, w, b, eps, slope)
+        return (source.detach(),), lambda t: ops.layer_norm(t, eps=eps, slope=slope)
+    buffer, slope = made_by
     N, C = x.shape[:2]
-    return _Kept8(N, C, x.numel() // (N * C)).packed(buffer, x.shape, slope)
+    codes, scales, weight, bias = _Kept8(N, C, x.numel() // (N * C)).packed(buffer)
+    return (codes, scales, weight, bias), _unpack(tuple(x.shape), slope)
 
 
 class _UpsampleAdd(torch.autograd.Function):
@@ -707,6 +719,18 @@ def conv_bn_relu_3d(m, x, checkpoint="f32"):
     if kind is None:
         raise RuntimeError(f"training: ConvBnReLU3D geometry {m._geometry} is not a CostRegNet layer shape")
     return abn_train(m.bn, conv(x, m.conv.weight, None, kind, checkpoint), checkpoint)
+
+
+def without_graph(forward, m, x):
+    """`forward` (one of the layer-by-layer forwards here) in eval mode: no graph, and no images of a training step's PackPlan - a captured hipGraph packs the weights
+    that it finds at each replay."""
+    global _ACTIVE_PLAN
+    plan, _ACTIVE_PLAN = _ACTIVE_PLAN, None
+    try:
+        with torch.no_grad():
+            return forward(m, x)
+    finally:
+        _ACTIVE_PLAN = plan
 
 
 def feature_net_train(net, x, checkpoint="f32"):

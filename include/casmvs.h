@@ -630,7 +630,8 @@ int casmvs_costvol_gwc_backward_f32(const float *feats, const float *proj, const
 
 /* Layer norm over the channel axis of a contiguous (outer, C, inner) tensor - inner = 1: rows of C - followed by the leaky ReLU of `slope` (1: none):
  *   y = lrelu((x - mean) / sqrt(var + eps) * weight[c] + bias[c]), mean and biased variance over the C channels of a position.
- * weight / bias may be NULL (1 / 0).  Statistics and the side of zero are computed in 64 bits.  C <= 65535; outer or inner may be 0.
+ * weight / bias may be NULL (1 / 0).  Statistics and the side of zero are computed in 64 bits; |x| below 1e37 (the rest is float32).  C <= 65535; outer or
+ * inner may be 0.
  * The backward pass takes the forward's x (no statistics are kept).  grad_x may be NULL; grad_weight / grad_bias are both given or both NULL; the sums are formed in
  * a fixed order (the same bits run to run).  workspace: casmvs_layer_norm_backward_workspace_bytes, 8-byte aligned. */
 int casmvs_layer_norm_forward(const void *x, const float *weight, const float *bias, void *y, int dtype, size_t outer, int C, size_t inner, float eps,
@@ -651,7 +652,8 @@ int casmvs_unpack8(const void *codes, const void *scales, const float *weight, c
  * addition on) that keeps for its backward pass the 8-bit checkpoint of xhat = (x - mean) rstd over the planes (N C, n) - codes, scales - and signs
  * (N C, nb) 32-bit words: bit i of a word = [z > 0] of the block's value i.  vec (4, C): scale = gamma rstd, shift, gamma (|weight| + abs_eps where
  * abs_eps >= 0), bias as the forward pass used them; act(gamma * unpacked + bias) is y up to the rounding of the 8 bits.
- * Backward: grad_weight, grad_bias, and grad_x (may be NULL).  workspace: casmvs_abn8_workspace_bytes, for either call on its own.  N * C <= 2^21. */
+ * Backward: grad_weight, grad_bias, and grad_x (may be NULL).  workspace: casmvs_abn8_workspace_bytes, for either call on its own.  N * C <= 2^21,
+ * planes of up to 2^37 / (N C) elements. */
 size_t casmvs_abn8_workspace_bytes(int N, int C, size_t n);
 int casmvs_abn8_forward_f32(const float *x, const float *weight, const float *bias, float abs_eps, float eps, float momentum, float *running_mean,
                             float *running_var, float *vec, float *y, void *codes, void *scales, void *signs, void *workspace, int N, int C, size_t n,
@@ -664,7 +666,7 @@ int casmvs_abn8_backward_f32(const float *grad_y, const void *codes, const void 
  * bytes or NULL.  The class of a pixel is the hypothesis nearest to depth_gt (the lowest index on ties); a pixel counts if its mask is not 0, depth_gt
  * lies inside [min, max] of its hypotheses and some cost is above -inf.  loss = mean over the counted pixels of -log softmax(cost)[class], share = 1 / count
  * (one float each); both 0 where no pixel counts.  stats (B, h*w, 2) floats (8-byte aligned), target (B, h*w): what the backward pass takes beside cost.
- * grad_loss: one device float; grad_cost has cost's type, 0 at every pixel that does not count.  workspace: casmvs_depth_ce_workspace_bytes. */
+ * B h w < 2^31, D <= 65536.  grad_loss: one device float; grad_cost has cost's type, 0 at every pixel that does not count.  workspace: casmvs_depth_ce_workspace_bytes. */
 size_t casmvs_depth_ce_workspace_bytes(int B, int D, size_t hw);
 int casmvs_depth_ce_forward(const void *cost, const float *depth_values, const float *depth_gt, const void *mask, float *stats, int *target, float *loss,
                             float *share, void *workspace, int dtype, int B, int D, size_t hw, int per_pixel, void *stream);

@@ -31,6 +31,12 @@ def rounding(want, dtype):
     return want.abs() * (f.eps / 2 + (U if dtype != F32 else 0.0)) + f.smallest_normal * f.eps / 2
 
 
+def rebuilt(x):
+    """The input that a convolution with 8-bit checkpoints takes its weight gradient at."""
+    tensors, rebuild = T.kept_input(x)
+    return rebuild(*tensors)
+
+
 def within(got, want, limit):
     got, want = got.detach().double().cpu(), want.detach().double().cpu()
     limit = limit.cpu() if isinstance(limit, torch.Tensor) else limit
@@ -323,7 +329,7 @@ def test_abn8_against_float64(dev, shape, slope, inplace):
     within(norm.bias.grad, gb, 64 * U * ab + rounding(gb, F32))
     within(norm.running_mean, 0.1 * mean, 1e-6 * (1 + mean.abs()))
     # what the convolution behind rebuilds of y: one step of xhat times gamma away at most
-    again = ops.unpack8(T.packed_input(got))
+    again = rebuilt(got)
     gamma = (w.abs() + 1e-5) if inplace else w
     N = shape[0]
     h = (x.double().reshape(N, C, -1) - mean.view(1, C, 1)) / torch.sqrt(x.double().reshape(N, C, -1).var((0, 2), unbiased=False) + 1e-5).view(1, C, 1)
@@ -352,7 +358,7 @@ def test_abn8_keeps_less_and_carries_non_finite_input(dev):
     assert bool(torch.isnan(bad.grad[:, 3]).all()) and bool(torch.isfinite(bad.grad[:, :3]).all()) and bool(torch.isfinite(bad.grad[:, 4:]).all())
 
 
-@pytest.mark.parametrize("source", ["abn", "abn written to", "sum", "leaf"])
+@pytest.mark.parametrize("source", ["abn", "abn written to", "layer norm", "plain layer norm", "layer norm written to", "sum", "leaf"])
 def test_conv8_takes_its_weight_gradient_at_the_checkpoint(dev, source):
     g = torch.Generator().manual_seed(7)
     w = (torch.randn(16, 8, 3, 3, 3, generator=g) * 0.2).to(dev).requires_grad_()
@@ -364,8 +370,13 @@ def test_conv8_takes_its_weight_gradient_at_the_checkpoint(dev, source):
             x.mul_(1.5)
             want_x = ops.unpack8(ops.pack8(x.detach()))
         else:
-            want_x = ops.unpack8(T.packed_input(x))
+            want_x = rebuilt(x)
             assert not torch.equal(want_x, ops.unpack8(ops.pack8(x.detach())))   # its own, not a new one
+    elif "layer norm" in source:
+        x = T.abn_train(M.LayerNormAct(8, affine=not source.startswith("plain")).to(dev), base, checkpoint="8bit")
+        if source.endswith("written to"):
+            x.add_(0.5)
+        want_x = ops.unpack8(ops.pack8(x.detach())) if source.endswith("written to") else x   # formed again exactly
     elif source == "sum":
         x = base + 1.0
         want_x = ops.unpack8(ops.pack8(x.detach()))
@@ -454,7 +465,7 @@ def test_depth_cross_entropy_edges(dev):
         c = wild.to(dev).requires_grad_()
         loss = A.depth_cross_entropy(c, values.to(dev), t.to(dev), None if m is None else m.to(dev))
         loss.backward()
-        assert float(loss) == 0.0 and not c.grad.any()
+        assert float(loss.detach()) == 0.0 and not c.grad.any()
     # -inf and the type's lowest value mask hypotheses out; a pixel with nothing left does not count
     for low in (-math.inf, torch.finfo(F32).min):
         c = cost.clone()
@@ -533,7 +544,7 @@ def _calls(dev):
     def abn():
         xr = x.detach().requires_grad_()
         y = T.abn_train(norm, xr, checkpoint="8bit")
-        return (y.detach(), ops.unpack8(T.packed_input(y)), *torch.autograd.grad(y, (xr, norm.weight, norm.bias), gy))
+        return (y.detach(), rebuilt(y), *torch.autograd.grad(y, (xr, norm.weight, norm.bias), gy))
 
     def ce():
         c = cost.detach().requires_grad_()
@@ -684,3 +695,55 @@ def test_layer_norm_model_in_eval_mode(dev):
         assert float((got[f"depth_{l}"] - want[f"depth_{l}"]).abs().max()) <= 1e-3 * float(want[f"depth_{l}"].abs().max())
     layer = model.feature.conv0[0]
     assert not layer(imgs[0]).requires_grad
+
+
+def test_layer_norm_model_follows_its_weights_in_a_captured_forward(dev):
+    """GraphedForward of a layer-norm model: its replays equal the eager forward, before and after a training step has changed the weights."""
+    from casmvsnet_pl_amd.graph import GraphedForward
+    from casmvsnet_pl_amd.synthetic import make_inputs
+    model, *_ = _step(dev, M.LayerNormAct, "8bit", "sl1")   # (its PackPlan is warm)
+    model.eval()
+    imgs, proj, dmin, dint = make_inputs(1, 3, 64, 96, seed=5)
+    imgs, proj = imgs.to(dev), proj.to(dev)
+    graphed = GraphedForward(model, imgs, proj, dmin, dint)
+    for round_ in range(3):
+        want = {k: v.clone() for k, v in model(imgs, proj, dmin, dint).items()}
+        got = graphed(imgs, proj)
+        torch.cuda.synchronize()
+        assert all(torch.equal(got[k], want[k]) for k in want), round_
+        with torch.no_grad():
+            for p in model.parameters():
+                p.mul_(1.01)
+
+
+def test_a_training_step_of_all_of_them_in_a_graph(dev):
+    """Layer norm, 8-bit checkpoints and the cross entropy in one captured step (forward, loss, backward to the parameters' gradients): every replay equals eager."""
+    g = torch.Generator().manual_seed(12)
+    x = torch.randn(2, 8, 8, 16, 24, generator=g).to(dev)
+    values = (400 + 2.65 * torch.arange(8, dtype=F32).view(1, 8, 1, 1) + torch.rand(2, 1, 16, 24, generator=g)).expand(2, 8, 16, 24).contiguous().to(dev)
+    gt, mask = (values[:, 3] + 1.0).contiguous(), (torch.rand(2, 16, 24, generator=g) < 0.7).to(dev)
+    for norm_act in (M.LayerNormAct, M.ABN):
+        torch.manual_seed(3)
+        net = M.CostRegNet(8, norm_act).to(dev).train()
+        for m in net.modules():
+            if hasattr(m, "running_mean"):
+                m.running_mean = m.running_var = None
+        params = list(net.parameters())
+
+        def step():
+            cost = T.cost_reg_net_train(net, x, "8bit").squeeze(1)
+            loss = A.depth_cross_entropy(cost, values, gt, mask)
+            return (loss.detach(), *torch.autograd.grad(loss, params))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = [t.clone() for t in step()]
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            captured = step()
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(captured, want))
+            assert all(torch.equal(p, q) for p, q in zip(step(), want))

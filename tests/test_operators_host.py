@@ -59,7 +59,9 @@ def test_c_abi_refuses_bad_arguments():
     refused(lib.casmvs_layer_norm_forward(_p(), None, None, _p(), 0, 1, 0, 4, 1e-5, 1.0, None), b"C=0")
     refused(lib.casmvs_layer_norm_forward(_p(), None, None, _p(), 0, 1, 65536, 4, 1e-5, 1.0, None), b"C=65536")
     refused(lib.casmvs_layer_norm_forward(None, None, None, _p(), 0, 1, 8, 4, 1e-5, 1.0, None), b"null pointer")
-    refused(lib.casmvs_layer_norm_forward(_p(), None, None, _p(), 0, 1 << 31, 8, 1, 1e-5, 1.0, None), b"rows")
+    refused(lib.casmvs_layer_norm_forward(_p(), None, None, _p(), 0, 1 << 31, 8, 1, 1e-5, 1.0, None), b"positions of 8 channels")
+    refused(lib.casmvs_layer_norm_forward(_p(), None, None, _p(), 0, 1 << 24, 9000, 1, 1e-5, 1.0, None), b"positions of 9000 channels")
+    refused(lib.casmvs_layer_norm_forward(_p(), None, None, _p(), 0, 1 << 15, 600, 1 << 15, 1e-5, 1.0, None), b"positions of 600 channels")
     refused(lib.casmvs_layer_norm_forward(_p(), None, None, _p(), 0, 1 << 62, 8, 16, 1e-5, 1.0, None), b"positions")
     refused(lib.casmvs_layer_norm_backward(_p(), _p(), None, None, _p(), _p(), None, _p(), 0, 1, 8, 4, 1e-5, 1.0, None), b"go together")
     refused(lib.casmvs_layer_norm_backward(_p(), _p(), None, None, _p(), None, None, None, 0, 1, 8, 4, 1e-5, 1.0, None), b"workspace")
@@ -75,6 +77,7 @@ def test_c_abi_refuses_bad_arguments():
     args = [_p(), _p(), _p(), -1.0, 1e-5, 0.1, None, None] + [_p()] * 6
     refused(lib.casmvs_abn8_forward_f32(*args, 0, 8, 32, 0.01, None), b"N=0")
     refused(lib.casmvs_abn8_forward_f32(*args, 1 << 20, 8, 32, 0.01, None), b"planes")
+    refused(lib.casmvs_abn8_forward_f32(*args, 1, 8, 1 << 35, 0.01, None), b"planes")
     refused(lib.casmvs_abn8_forward_f32(*args, 1, 8, 1 << 50, 0.01, None), b"planes")
     refused(lib.casmvs_abn8_forward_f32(*(args[:6] + [_p()] + args[7:]), 1, 8, 32, 0.01, None), b"go together")
     refused(lib.casmvs_abn8_forward_f32(*(args[:13] + [_p(12)]), 1, 8, 32, 0.01, None), b"words")
@@ -82,6 +85,7 @@ def test_c_abi_refuses_bad_arguments():
     refused(lib.casmvs_abn8_backward_f32(_p(), _p(), _p(), _p(), _p(), -1.0, _p(), None, _p(), _p(), _p(), 1, 8, 32, 0.01, None), b"null pointer")
     assert lib.casmvs_abn8_workspace_bytes(0, 8, 32) == 0 and lib.casmvs_abn8_workspace_bytes(1, 8, 32) == 128
     refused(lib.casmvs_depth_ce_forward(_p(), _p(), _p(), None, _p(), _p(), _p(), _p(), _p(), 0, 1, 0, 16, 1, None), b"D=0")
+    refused(lib.casmvs_depth_ce_forward(_p(), _p(), _p(), None, _p(), _p(), _p(), _p(), _p(), 0, 2, 4, 1 << 30, 1, None), b"2^31")
     refused(lib.casmvs_depth_ce_forward(_p(), None, _p(), None, _p(), _p(), _p(), _p(), _p(), 0, 1, 4, 16, 1, None), b"null pointer")
     refused(lib.casmvs_depth_ce_forward(_p(), _p(), _p(), None, _p(), _p(), _p(), None, _p(), 0, 1, 4, 16, 1, None), b"null pointer")
     refused(lib.casmvs_depth_ce_backward(_p(), _p(), _p(), _p(), None, _p(), 0, 1, 4, 16, None), b"null pointer")
