@@ -148,17 +148,15 @@ class _DepthCrossEntropy(torch.autograd.Function):
             mask = ops._same_device(cost, mask, "mask").contiguous()
         if B * D == 0:
             raise ValueError(f"depth_cross_entropy: cost {tuple(cost.shape)} has no hypotheses")
-        lib, code, pixels = _lib.load(), ops._DTYPES[cost.dtype], B * h * w
+        code, pixels = ops._DTYPES[cost.dtype], B * h * w
         loss = torch.empty((), dtype=torch.float32, device=cost.device)
         # one buffer: per pixel the running maximum and 1 / sum (two floats) and the class (an int), 1 / count, and (8-byte aligned) the forward's workspace
         at_target, at_share = 8 * pixels, 12 * pixels
         at_ws = at_share + 4 + (at_share + 4) % 8
         kept = torch.empty(at_ws + ops._workspace_bytes("casmvs_depth_ce_workspace_bytes", B, D, h * w), dtype=torch.uint8, device=cost.device)
         base = kept.data_ptr()
-        with ops._on(cost):
-            rc = lib.casmvs_depth_ce_forward(cost.data_ptr(), depth_values.data_ptr(), depth_gt.data_ptr(), ops._at(mask), base, base + at_target, loss.data_ptr(),
-                                             base + at_share, base + at_ws, code, B, D, h * w, int(depth_values.dim() == 4), _stream(cost))
-        _lib.check(rc, "casmvs_depth_ce_forward")
+        ops._launch("casmvs_depth_ce_forward", cost, cost.data_ptr(), depth_values.data_ptr(), depth_gt.data_ptr(), ops._at(mask), base, base + at_target, loss.data_ptr(),
+                    base + at_share, base + at_ws, code, B, D, h * w, int(depth_values.dim() == 4))
         ctx.save_for_backward(cost, kept)
         return loss
 
@@ -169,10 +167,8 @@ class _DepthCrossEntropy(torch.autograd.Function):
         B, D, h, w = cost.shape
         gcost = torch.empty_like(cost)
         base, pixels = kept.data_ptr(), B * h * w
-        with ops._on(cost):
-            rc = _lib.load().casmvs_depth_ce_backward(cost.data_ptr(), base, base + 8 * pixels, base + 12 * pixels, gloss.contiguous().data_ptr(), gcost.data_ptr(),
-                                                      ops._DTYPES[cost.dtype], B, D, h * w, _stream(cost))
-        _lib.check(rc, "casmvs_depth_ce_backward")
+        ops._launch("casmvs_depth_ce_backward", cost, cost.data_ptr(), base, base + 8 * pixels, base + 12 * pixels, gloss.contiguous().data_ptr(), gcost.data_ptr(),
+                    ops._DTYPES[cost.dtype], B, D, h * w)
         return gcost, None, None, None
 
 

@@ -3,7 +3,6 @@ and the current HIP stream; every op below is one call into libcasmvs_hip.so.
 
 All inputs must be float32 tensors on a ROCm device ("cuda" in torch); nothing here runs on CPU.
 """
-import contextlib
 import ctypes
 import functools
 
@@ -926,12 +925,18 @@ def _float_dev(t, name):
     return t.contiguous()
 
 
-_STAY = contextlib.nullcontext()
-
-
-def _on(t):
-    """The context in which t's device is the current one."""
-    return _STAY if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _launch(name, t, *args):
+    """lib.<name>(*args, stream) on t's device, in its current stream (streams.launch_stream); raises where the library refuses."""
+    index = t.device.index
+    stream = torch._C._cuda_getCurrentRawStream(index) if streams._enabled is False else _stream(t)
+    fn = getattr(_lib.load(), name)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, name)
 
 
 def _at(t):
@@ -982,9 +987,7 @@ def _layer_norm_args(x, weight, bias, eps, slope, channels_last):
 
 def _layer_norm_forward(x, weight, bias, outer, C, inner, eps, slope):
     y = torch.empty_like(x)
-    with _on(x):
-        rc = _lib.load().casmvs_layer_norm_forward(x.data_ptr(), _at(weight), _at(bias), y.data_ptr(), _DTYPES[x.dtype], outer, C, inner, eps, slope, _stream(x))
-    _lib.check(rc, "casmvs_layer_norm_forward")
+    _launch("casmvs_layer_norm_forward", x, x.data_ptr(), _at(weight), _at(bias), y.data_ptr(), _DTYPES[x.dtype], outer, C, inner, eps, slope)
     return y
 
 
@@ -996,10 +999,8 @@ def _layer_norm_backward(x, grad_y, weight, bias, outer, C, inner, eps, slope, n
         gw, gb, ws = _affine_gradients(C, nbytes, x.device)
     else:
         gw, gb, ws = None, None, torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    with _on(x):
-        rc = _lib.load().casmvs_layer_norm_backward(x.data_ptr(), grad_y.data_ptr(), _at(weight), _at(bias), _at(gx), _at(gw), _at(gb), ws.data_ptr(), code, outer, C,
-                                                    inner, eps, slope, _stream(x))
-    _lib.check(rc, "casmvs_layer_norm_backward")
+    _launch("casmvs_layer_norm_backward", x, x.data_ptr(), grad_y.data_ptr(), _at(weight), _at(bias), _at(gx), _at(gw), _at(gb), ws.data_ptr(), code, outer, C, inner, eps,
+            slope)
     return gx, gw, gb
 
 
@@ -1053,9 +1054,7 @@ def pack8(x):
     nb = (n + 31) // 32
     codes = torch.empty((rows, nb, 32), dtype=torch.uint8, device=x.device)
     scales = torch.empty((rows, nb), dtype=torch.uint8, device=x.device)
-    with _on(x):
-        rc = _lib.load().casmvs_pack8(_at(x), _DTYPES[x.dtype], rows, n, _at(codes), _at(scales), _stream(x))
-    _lib.check(rc, "casmvs_pack8")
+    _launch("casmvs_pack8", x, x.data_ptr(), _DTYPES[x.dtype], rows, n, codes.data_ptr(), scales.data_ptr())
     return Packed8(codes, scales, x.shape, x.dtype)
 
 
@@ -1083,8 +1082,5 @@ def unpack8(packed):
         if tuple(weight.shape) != (C,) or tuple(bias.shape) != (C,):
             raise ValueError(f"unpack8: affine {tuple(weight.shape)} {tuple(bias.shape)}, expected ({C},)")
     out = torch.empty(packed.shape, dtype=packed.dtype, device=codes.device)
-    with _on(codes):
-        rc = _lib.load().casmvs_unpack8(_at(codes), _at(scales), _at(weight), _at(bias), C, float(slope), _at(out), _DTYPES[packed.dtype], rows, n,
-                                        _stream(codes))
-    _lib.check(rc, "casmvs_unpack8")
+    _launch("casmvs_unpack8", codes, codes.data_ptr(), scales.data_ptr(), _at(weight), _at(bias), C, float(slope), out.data_ptr(), _DTYPES[packed.dtype], rows, n)
     return out

@@ -492,11 +492,8 @@ class _ABNTrain8(torch.autograd.Function):
             if t.shape != (C,) or t.dtype != torch.float32 or t.device != x.device or not t.is_contiguous():
                 raise ValueError(f"abn_train: x {tuple(x.shape)} on {x.device}, a parameter or running statistic is {tuple(t.shape)} {t.dtype} on {t.device}")
         base = buffer.data_ptr()
-        with ops._on(x):
-            rc = _lib.load().casmvs_abn8_forward_f32(x.data_ptr(), w.data_ptr(), bta.data_ptr(), abs_eps, eps, momentum, running_mean.data_ptr() if track else None,
-                                                     running_var.data_ptr() if track else None, base + kept.vec, y.data_ptr(), base, base + kept.scales,
-                                                     base + kept.signs, base + kept.bytes, N, C, n, slope, _stream(x))
-        _lib.check(rc, "casmvs_abn8_forward_f32")
+        ops._launch("casmvs_abn8_forward_f32", x, x.data_ptr(), w.data_ptr(), bta.data_ptr(), abs_eps, eps, momentum, running_mean.data_ptr() if track else None,
+                    running_var.data_ptr() if track else None, base + kept.vec, y.data_ptr(), base, base + kept.scales, base + kept.signs, base + kept.bytes, N, C, n, slope)
         if track:   # the kernel wrote the buffers behind torch's back: bump their version counters (packed-weight caches key on them)
             torch.autograd.graph.increment_version((running_mean, running_var))
         ctx.save_for_backward(buffer, w)
@@ -513,10 +510,8 @@ class _ABNTrain8(torch.autograd.Function):
         gw, gb, ws = ops._affine_gradients(k.C, ops._workspace_bytes("casmvs_abn8_workspace_bytes", k.N, k.C, k.n), gy.device)
         gx = torch.empty_like(gy) if ctx.needs_input_grad[0] else None
         base = buffer.data_ptr()
-        with ops._on(gy):
-            rc = _lib.load().casmvs_abn8_backward_f32(gy.data_ptr(), base, base + k.scales, base + k.signs, w.data_ptr(), ctx.abs_eps, base + k.vec, gw.data_ptr(),
-                                                      gb.data_ptr(), ops._at(gx), ws.data_ptr(), k.N, k.C, k.n, ctx.slope, _stream(gy))
-        _lib.check(rc, "casmvs_abn8_backward_f32")
+        ops._launch("casmvs_abn8_backward_f32", gy, gy.data_ptr(), base, base + k.scales, base + k.signs, w.data_ptr(), ctx.abs_eps, base + k.vec, gw.data_ptr(), gb.data_ptr(),
+                    ops._at(gx), ws.data_ptr(), k.N, k.C, k.n, ctx.slope)
         return gx, gw, gb, None, None, None, None, None, None
 
 
