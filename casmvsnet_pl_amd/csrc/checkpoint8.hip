@@ -38,14 +38,16 @@ __device__ __forceinline__ void load4(const T *p, int left, float (&v)[4]) {
     for (int i = 0; i < 4; ++i) v[i] = i < left ? (float)p[i] : 0.0f;
   }
 }
-template <class T, bool WIDE>
+// PAST: past the caches
+template <class T, bool WIDE, bool PAST>
 __device__ __forceinline__ void store4(T *p, int left, const float (&v)[4]) {
   if (WIDE) {
     if (left > 0) {
       Vec<T, 4> t;
 #pragma unroll
       for (int i = 0; i < 4; ++i) t.v[i] = (T)v[i];
-      casmvs::elem::store<T, 4>(p, t);
+      if (PAST) casmvs::elem::store_past<T, 4>(p, t);
+      else casmvs::elem::store<T, 4>(p, t);
     }
   } else {
 #pragma unroll
@@ -96,7 +98,7 @@ __global__ __launch_bounds__(kThreads) void pack8_kernel(const T *__restrict__ x
 }
 
 // out = the held value, or (AFFINE) act(value * weight[c] + bias[c]) with c = row % C: an ABN's output from what its backward pass keeps
-template <class T, bool WIDE, bool AFFINE>
+template <class T, bool WIDE, bool AFFINE, bool PAST>
 __global__ __launch_bounds__(kThreads) void unpack8_kernel(const unsigned *__restrict__ codes, const unsigned char *__restrict__ scales, T *__restrict__ out,
                                                           const float *__restrict__ weight, const float *__restrict__ bias, int C, float slope, size_t rows,
                                                           size_t n, size_t nb) {
@@ -129,7 +131,7 @@ __global__ __launch_bounds__(kThreads) void unpack8_kernel(const unsigned *__res
           v[i] = z > 0.0f ? z : z * slope;
         }
       }
-      store4<T, WIDE>(out + row * n + first, left_of(n, first), v);
+      store4<T, WIDE, PAST>(out + row * n + first, left_of(n, first), v);
     }
   }
 }
@@ -237,7 +239,7 @@ struct Store {     // the 8-bit checkpoint of the normalised input and the signs
   unsigned *signs;
 };
 // y and the checkpoint of the blocks blk0, blk0 + step, .. (kAhead of them, their loads issued together) of one plane.  Every lane of a wave comes here together.
-template <bool WIDE>
+template <bool WIDE, bool PAST>
 __device__ __forceinline__ void apply_blocks(const float *__restrict__ xp, float *__restrict__ yp, const Store &to, size_t base, size_t blk0, size_t step, size_t n,
                                              size_t nb, int lane, const Channel &c, float slope) {
   float v[kAhead][4];
@@ -263,7 +265,7 @@ __device__ __forceinline__ void apply_blocks(const float *__restrict__ xp, float
     unsigned scale;
     const unsigned q = casmvs::block8::quantise(h, scale);
     const unsigned sign = casmvs::block8::over_block(up << (4 * lane), [](unsigned p, unsigned r) { return p | r; });
-    store4<float, WIDE>(yp + first, left, o);
+    store4<float, WIDE, PAST>(yp + first, left, o);
     if (blk < nb) {
       to.codes[(base + blk) * kLanes + lane] = q;
       if (lane == 0) {
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(kSumThreads) void abn8_sums_kernel(const float *__r
 constexpr int kTurns = 8;   // blocks per group of eight lanes and workgroup: 256 x 32 = 8192 elements share one read of the channel's partial sums
 
 // blockIdx.x = (plane, chunk of kTurns * kGroups blocks)
-template <bool WIDE>
+template <bool WIDE, bool PAST>
 __global__ __launch_bounds__(kThreads) void abn8_apply_kernel(const float *__restrict__ x, const double *__restrict__ sums, int parts, double M, Norm norm,
                                                              float *__restrict__ y, Store to, int C, size_t n, size_t nb, unsigned chunks) {
   const unsigned plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
@@ -301,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void abn8_apply_kernel(const float *__res
   channel_totals(sums, parts, c, s0, s1);
   const Channel k = finish(norm, s0, s1, M, c, C, chunk == 0 && plane == (unsigned)c && threadIdx.x == 0);
   for (int turn = 0; turn < kTurns; turn += kAhead)
-    apply_blocks<WIDE>(x + plane * n, y + plane * n, to, plane * nb, ((size_t)chunk * kTurns + turn) * kGroups + threadIdx.x / kLanes, kGroups, n, nb,
+    apply_blocks<WIDE, PAST>(x + plane * n, y + plane * n, to, plane * nb, ((size_t)chunk * kTurns + turn) * kGroups + threadIdx.x / kLanes, kGroups, n, nb,
                        threadIdx.x & (kLanes - 1), k, norm.slope);
 }
 
@@ -319,7 +321,7 @@ __global__ __launch_bounds__(kWide) void abn8_forward_one_kernel(const float *__
   for (int img = 0; img < N; ++img) {
     const size_t plane = (size_t)img * C + c;
     for (size_t blk = 0; blk < nb; blk += kAhead * groups)
-      apply_blocks<WIDE>(x + plane * n, y + plane * n, to, plane * nb, blk + threadIdx.x / kLanes, groups, n, nb, threadIdx.x & (kLanes - 1), k, norm.slope);
+      apply_blocks<WIDE, false>(x + plane * n, y + plane * n, to, plane * nb, blk + threadIdx.x / kLanes, groups, n, nb, threadIdx.x & (kLanes - 1), k, norm.slope);
   }
 }
 
@@ -407,7 +409,7 @@ __device__ __forceinline__ Means finish_gradients(const Gradients &p, double s0,
   }
   return Means{(float)(s0 / M), (float)(s1 / M), p.vec[c]};
 }
-template <bool WIDE>
+template <bool WIDE, bool PAST>
 __device__ __forceinline__ void gradient_blocks(const float *__restrict__ gy, const Checkpoint &from, float *__restrict__ gx, size_t plane, size_t blk0, size_t step, size_t n,
                                                 size_t nb, const Means &m, float slope) {
   const int lane = threadIdx.x & (kLanes - 1);
@@ -420,11 +422,11 @@ __device__ __forceinline__ void gradient_blocks(const float *__restrict__ gy, co
     float o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = m.a * (behind_activation(k[j], i, slope) - m.m1 - casmvs::block8::value_of(k[j].q, i, k[j].step) * m.m2);
-    store4<float, WIDE>(gx + plane * n + first, left_of(n, first), o);
+    store4<float, WIDE, PAST>(gx + plane * n + first, left_of(n, first), o);
   }
 }
 
-template <bool WIDE>
+template <bool WIDE, bool PAST>
 __global__ __launch_bounds__(kThreads) void abn8_backward_apply_kernel(const float *__restrict__ gy, Checkpoint from, const double *__restrict__ sums, int parts, double M,
                                                                       Gradients p, int C, size_t n, size_t nb, unsigned chunks) {
   const unsigned plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
@@ -434,7 +436,7 @@ __global__ __launch_bounds__(kThreads) void abn8_backward_apply_kernel(const flo
   const Means m = finish_gradients(p, s0, s1, M, c, chunk == 0 && plane == (unsigned)c && threadIdx.x == 0);
   if (!p.gx) return;
   for (int turn = 0; turn < kTurns; turn += kAhead)
-    gradient_blocks<WIDE>(gy, from, p.gx, plane, ((size_t)chunk * kTurns + turn) * kGroups + threadIdx.x / kLanes, kGroups, n, nb, m, p.slope);
+    gradient_blocks<WIDE, PAST>(gy, from, p.gx, plane, ((size_t)chunk * kTurns + turn) * kGroups + threadIdx.x / kLanes, kGroups, n, nb, m, p.slope);
 }
 
 template <bool WIDE>
@@ -448,7 +450,7 @@ __global__ __launch_bounds__(kWide) void abn8_backward_one_kernel(const float *_
   if (!p.gx) return;
   for (int img = 0; img < N; ++img)
     for (size_t blk = 0; blk < nb; blk += kAhead * groups)
-      gradient_blocks<WIDE>(gy, from, p.gx, (size_t)img * C + c, blk + threadIdx.x / kLanes, groups, n, nb, m, p.slope);
+      gradient_blocks<WIDE, false>(gy, from, p.gx, (size_t)img * C + c, blk + threadIdx.x / kLanes, groups, n, nb, m, p.slope);
 }
 
 // Elements of a channel up to which one workgroup does both passes over it: one launch less, on as many CUs as there are channels
@@ -507,14 +509,15 @@ extern "C" int casmvs_unpack8(const void *codes, const void *scales, const float
   const size_t wanted = (total + kGroups - 1) / kGroups;
   const unsigned grid = (unsigned)(wanted < 8192 ? wanted : 8192);
   const bool wide = n % 4 == 0 && aligned16(out);
-#define CASMVS_UNPACK8(W, A)                                                                                                                          \
-  hipLaunchKernelGGL((unpack8_kernel<T, W, A>), dim3(grid), dim3(kThreads), 0, (hipStream_t)stream, (const unsigned *)codes, (const unsigned char *)scales, \
+  const bool past = wide && casmvs::elem::streams(rows * n * casmvs::elem::size_of(dtype));
+#define CASMVS_UNPACK8(W, A, P)                                                                                                                       \
+  hipLaunchKernelGGL((unpack8_kernel<T, W, A, P>), dim3(grid), dim3(kThreads), 0, (hipStream_t)stream, (const unsigned *)codes, (const unsigned char *)scales, \
                      (T *)out, weight, bias, C, slope, rows, n, nb)
   CASMVS_WITH_DTYPE(dtype, {
     if (weight) {
-      if (wide) CASMVS_UNPACK8(true, true); else CASMVS_UNPACK8(false, true);
+      if (past) CASMVS_UNPACK8(true, true, true); else if (wide) CASMVS_UNPACK8(true, true, false); else CASMVS_UNPACK8(false, true, false);
     } else {
-      if (wide) CASMVS_UNPACK8(true, false); else CASMVS_UNPACK8(false, false);
+      if (past) CASMVS_UNPACK8(true, false, true); else if (wide) CASMVS_UNPACK8(true, false, false); else CASMVS_UNPACK8(false, false, false);
     }
   });
 #undef CASMVS_UNPACK8
@@ -548,7 +551,9 @@ extern "C" int casmvs_abn8_forward_f32(const float *x, const float *weight, cons
     return casmvs::check_launch("abn8_forward_one_kernel");
   }
   hipLaunchKernelGGL(wide ? abn8_sums_kernel<true> : abn8_sums_kernel<false>, dim3((unsigned)parts, (unsigned)C), dim3(kSumThreads), 0, st, x, sums, N, C, n);
-  hipLaunchKernelGGL(wide ? abn8_apply_kernel<true> : abn8_apply_kernel<false>, dim3((unsigned)((size_t)N * C * chunks)), dim3(kThreads), 0, st, x, sums, parts, count, norm,
+  const bool past = wide && casmvs::elem::streams((size_t)N * C * n * sizeof(float));
+  auto apply = past ? abn8_apply_kernel<true, true> : wide ? abn8_apply_kernel<true, false> : abn8_apply_kernel<false, false>;
+  hipLaunchKernelGGL(apply, dim3((unsigned)((size_t)N * C * chunks)), dim3(kThreads), 0, st, x, sums, parts, count, norm,
                      y, to, C, n, nb, (unsigned)chunks);
   return casmvs::check_launch("abn8_forward");
 }
@@ -577,7 +582,9 @@ extern "C" int casmvs_abn8_backward_f32(const float *grad_y, const void *codes, 
                      N, C, n, nb, slope);
   // (without grad_x the workgroups of the channels' first chunks write the two vectors, and there are no others)
   const dim3 grid((unsigned)(grad_x ? (size_t)N * C * chunks : (size_t)C * chunks));
-  hipLaunchKernelGGL(wide ? abn8_backward_apply_kernel<true> : abn8_backward_apply_kernel<false>, grid, dim3(kThreads), 0, st, grad_y, from, sums, parts, count, to, C, n, nb,
+  const bool past = wide && casmvs::elem::streams((size_t)N * C * n * sizeof(float));
+  auto apply = past ? abn8_backward_apply_kernel<true, true> : wide ? abn8_backward_apply_kernel<true, false> : abn8_backward_apply_kernel<false, false>;
+  hipLaunchKernelGGL(apply, grid, dim3(kThreads), 0, st, grad_y, from, sums, parts, count, to, C, n, nb,
                      (unsigned)chunks);
   return casmvs::check_launch("abn8_backward");
 }

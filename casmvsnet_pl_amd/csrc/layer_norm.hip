@@ -149,7 +149,7 @@ struct PlaneWeights {
   }
 };
 
-template <class T, int CG, int V, bool FEW>
+template <class T, int CG, int V, bool FEW, bool PAST>
 __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__restrict__ x, const float *__restrict__ w, const float *__restrict__ b,
                                                                     T *__restrict__ y, size_t first, size_t positions, int C, size_t inner, double per_c,
                                                                     float eps, float slope) {
@@ -189,7 +189,8 @@ __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__
         t.v[i] = (T)(float)(z > 0.0 ? z : z * slope);
       }
     }
-    casmvs::elem::store<T, V>(y + base + c * inner, t);
+    if (PAST) casmvs::elem::store_past<T, V>(y + base + c * inner, t);
+    else casmvs::elem::store<T, V>(y + base + c * inner, t);
   }
 }
 
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__
 enum Channels { kFew, kSome, kFull };
 
 // gx, and of every workgroup the sums over its tiles of g h and g per channel: partial[workgroup][0 / 1][c].  AFFINE: the weight gradient is wanted.
-template <class T, int CG, int V, bool AFFINE, Channels CH>
+template <class T, int CG, int V, bool AFFINE, Channels CH, bool PAST>
 __global__ __launch_bounds__(kThreads) void ln_backward_planes_kernel(const T *__restrict__ x, const T *__restrict__ gy, const float *__restrict__ w,
                                                                      const float *__restrict__ b, T *__restrict__ gx, float *__restrict__ partial,
                                                                      size_t positions, size_t tiles, int C, size_t inner, double per_c, float eps, float slope) {
@@ -316,7 +317,8 @@ __global__ __launch_bounds__(kThreads) void ln_backward_planes_kernel(const T *_
               t.v[i] = (T)((float)rstd[i] * (g[r][i] * a.w[r] - (float)m[0][i] - v[r][i] * (float)m[1][i]));
             }
           }
-          casmvs::elem::store<T, V>(gx + base + c * inner, t);
+          if (PAST) casmvs::elem::store_past<T, V>(gx + base + c * inner, t);
+          else casmvs::elem::store<T, V>(gx + base + c * inner, t);
         }
       }
     }
@@ -821,21 +823,27 @@ struct Call {   // arguments of either direction
   }
 };
 
-template <class T, int CG, int V, Channels CH>
-void planes(const Call &a, int &parts) {
+template <class T, int CG, int V, Channels CH, bool PAST>
+void planes_as(const Call &a, int &parts) {
   const size_t tile = (size_t)(kThreads / CG) * V, tiles = (a.positions() + tile - 1) / tile;
   if (!a.gy) {
     for (size_t first = 0; first < tiles; first += kLaunchBlocks)
-      hipLaunchKernelGGL((ln_forward_planes_kernel<T, CG, V, CH == kFew>), dim3(launch_blocks(tiles - first)), dim3(kThreads), 0, a.stream, (const T *)a.x, a.w, a.b,
+      hipLaunchKernelGGL((ln_forward_planes_kernel<T, CG, V, CH == kFew, PAST>), dim3(launch_blocks(tiles - first)), dim3(kThreads), 0, a.stream, (const T *)a.x, a.w, a.b,
                          (T *)a.out, first, a.positions(), a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
     return;
   }
   const unsigned grid = (unsigned)(tiles < backward_blocks(a.C) ? tiles : backward_blocks(a.C));
   parts = (int)grid;
   float *sums = a.sums(parts);
-  auto kernel = a.partial ? ln_backward_planes_kernel<T, CG, V, true, CH> : ln_backward_planes_kernel<T, CG, V, false, CH>;
+  auto kernel = a.partial ? ln_backward_planes_kernel<T, CG, V, true, CH, PAST> : ln_backward_planes_kernel<T, CG, V, false, CH, PAST>;
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0, a.stream, (const T *)a.x, (const T *)a.gy, a.w, a.b, (T *)a.out, sums, a.positions(), tiles,
                      a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
+}
+// (an output past the caches: with pairs of positions only)
+template <class T, int CG, int V, Channels CH>
+void planes(const Call &a, int &parts) {
+  if (V > 1 && casmvs::elem::streams(a.positions() * a.C * sizeof(T))) planes_as<T, CG, V, CH, (V > 1)>(a, parts);
+  else planes_as<T, CG, V, CH, false>(a, parts);
 }
 template <class T, int V>
 void planes_by_groups(const Call &a, int &parts) {

@@ -26,6 +26,7 @@ torch is the autograd tape and the allocator; the skip additions of the U-Net an
 times (18 ms per step at the reference's default training configuration, 15 ms captured as one hipGraph).
 """
 import ctypes
+import functools
 import weakref
 
 import torch
@@ -474,6 +475,9 @@ class _Kept8:
         return buffer[:self.scales].view(planes, nb, 32), buffer[self.scales:self.scales + planes * nb].view(planes, nb), vec[2], vec[3]
 
 
+_kept8 = functools.lru_cache(maxsize=1024)(_Kept8)
+
+
 class _ABNTrain8(torch.autograd.Function):
     """_ABNTrain that keeps 8 bits of the normalised input and one bit per element (casmvs_abn8_*): -> (y, the buffer it keeps)."""
 
@@ -482,15 +486,16 @@ class _ABNTrain8(torch.autograd.Function):
         x = x.contiguous().float()
         N, C = x.shape[:2]
         n = x.numel() // (N * C)
-        kept = _Kept8(N, C, n)
+        kept = _kept8(N, C, n)
         # (the forward's workspace, at most 16 KB, lies behind what is kept)
         buffer = torch.empty(kept.bytes + ops._workspace_bytes("casmvs_abn8_workspace_bytes", N, C, n), dtype=torch.uint8, device=x.device)
         y = torch.empty_like(x)
         w, bta = weight.contiguous().float(), beta.contiguous().float()   # (themselves, as a rule)
         track = running_mean is not None and running_var is not None
+        device = x.device
         for t in (w, bta, running_mean, running_var) if track else (w, bta):
-            if t.shape != (C,) or t.dtype != torch.float32 or t.device != x.device or not t.is_contiguous():
-                raise ValueError(f"abn_train: x {tuple(x.shape)} on {x.device}, a parameter or running statistic is {tuple(t.shape)} {t.dtype} on {t.device}")
+            if t.numel() != C or t.dtype is not torch.float32 or t.device != device or not t.is_contiguous():
+                raise ValueError(f"abn_train: x {tuple(x.shape)} on {device}, a parameter or running statistic is {tuple(t.shape)} {t.dtype} on {t.device}")
         base = buffer.data_ptr()
         ops._launch("casmvs_abn8_forward_f32", x, x.data_ptr(), w.data_ptr(), bta.data_ptr(), abs_eps, eps, momentum, running_mean.data_ptr() if track else None,
                     running_var.data_ptr() if track else None, base + kept.vec, y.data_ptr(), base, base + kept.scales, base + kept.signs, base + kept.bytes, N, C, n, slope)
@@ -565,7 +570,7 @@ def kept_input(x):
         return (source.detach(),), lambda t: ops.layer_norm(t, eps=eps, slope=slope)
     buffer, slope = made_by
     N, C = x.shape[:2]
-    codes, scales, weight, bias = _Kept8(N, C, x.numel() // (N * C)).packed(buffer)
+    codes, scales, weight, bias = _kept8(N, C, x.numel() // (N * C)).packed(buffer)
     return (codes, scales, weight, bias), _unpack(tuple(x.shape), slope)
 
 

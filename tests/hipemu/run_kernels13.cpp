@@ -8,6 +8,7 @@
 inline double hipemu_rsq(double a) { return (double)(float)(1.0 / std::sqrt(a)); }   // an estimate of 24 bits
 #define __builtin_amdgcn_rsq hipemu_rsq
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
+#define __builtin_nontemporal_store(v, p) (*(p) = (v))
 inline int hipemu_bpermute(int from, int v) { return hipemu_lane_exchange(v, (from >> 2) & 63); }
 #define __builtin_amdgcn_ds_bpermute hipemu_bpermute
 
