@@ -149,7 +149,7 @@ struct PlaneWeights {
   }
 };
 
-template <class T, int CG, int V, bool FEW, bool PAST>
+template <class T, int CG, int V, bool FEW>
 __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__restrict__ x, const float *__restrict__ w, const float *__restrict__ b,
                                                                     T *__restrict__ y, size_t first, size_t positions, int C, size_t inner, double per_c,
                                                                     float eps, float slope) {
@@ -189,8 +189,7 @@ __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__
         t.v[i] = (T)(float)(z > 0.0 ? z : z * slope);
       }
     }
-    if (PAST) casmvs::elem::store_past<T, V>(y + base + c * inner, t);
-    else casmvs::elem::store<T, V>(y + base + c * inner, t);
+    casmvs::elem::store<T, V>(y + base + c * inner, t);
   }
 }
 
@@ -198,7 +197,8 @@ __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__
 // form of the last kind: without the tests the compiler holds every channel's values at once, 88 registers instead of 56, and the pass is 15 % slower.
 enum Channels { kFew, kSome, kFull };
 
-// gx, and of every workgroup the sums over its tiles of g h and g per channel: partial[workgroup][0 / 1][c].  AFFINE: the weight gradient is wanted.
+// gx, and of every workgroup the sums over its tiles of g h and g per channel: partial[workgroup][0 / 1][c].  AFFINE: the weight gradient is wanted.  PAST: gx goes
+// past the caches (the forward pass's y does not: 61 and 60 us at 2 x 8 x 32 x 256 x 320).
 template <class T, int CG, int V, bool AFFINE, Channels CH, bool PAST>
 __global__ __launch_bounds__(kThreads) void ln_backward_planes_kernel(const T *__restrict__ x, const T *__restrict__ gy, const float *__restrict__ w,
                                                                      const float *__restrict__ b, T *__restrict__ gx, float *__restrict__ partial,
@@ -823,27 +823,24 @@ struct Call {   // arguments of either direction
   }
 };
 
-template <class T, int CG, int V, Channels CH, bool PAST>
-void planes_as(const Call &a, int &parts) {
+template <class T, int CG, int V, Channels CH>
+void planes(const Call &a, int &parts) {
   const size_t tile = (size_t)(kThreads / CG) * V, tiles = (a.positions() + tile - 1) / tile;
   if (!a.gy) {
     for (size_t first = 0; first < tiles; first += kLaunchBlocks)
-      hipLaunchKernelGGL((ln_forward_planes_kernel<T, CG, V, CH == kFew, PAST>), dim3(launch_blocks(tiles - first)), dim3(kThreads), 0, a.stream, (const T *)a.x, a.w, a.b,
+      hipLaunchKernelGGL((ln_forward_planes_kernel<T, CG, V, CH == kFew>), dim3(launch_blocks(tiles - first)), dim3(kThreads), 0, a.stream, (const T *)a.x, a.w, a.b,
                          (T *)a.out, first, a.positions(), a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
     return;
   }
   const unsigned grid = (unsigned)(tiles < backward_blocks(a.C) ? tiles : backward_blocks(a.C));
   parts = (int)grid;
   float *sums = a.sums(parts);
-  auto kernel = a.partial ? ln_backward_planes_kernel<T, CG, V, true, CH, PAST> : ln_backward_planes_kernel<T, CG, V, false, CH, PAST>;
+  auto kernel = a.partial ? ln_backward_planes_kernel<T, CG, V, true, CH, false> : ln_backward_planes_kernel<T, CG, V, false, CH, false>;
+  if constexpr (CH == kFull && V > 1)   // large outputs of 8 channels per group: 2 x 8 x 32 x 256 x 320 in float32 104 -> 99 us, in bf16 53 -> 49 (a branch in the kernel gains nothing)
+    if (casmvs::elem::streams(a.positions() * a.C * sizeof(T)))
+      kernel = a.partial ? ln_backward_planes_kernel<T, CG, V, true, CH, true> : ln_backward_planes_kernel<T, CG, V, false, CH, true>;
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0, a.stream, (const T *)a.x, (const T *)a.gy, a.w, a.b, (T *)a.out, sums, a.positions(), tiles,
                      a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
-}
-// (an output past the caches: with pairs of positions only)
-template <class T, int CG, int V, Channels CH>
-void planes(const Call &a, int &parts) {
-  if (V > 1 && casmvs::elem::streams(a.positions() * a.C * sizeof(T))) planes_as<T, CG, V, CH, (V > 1)>(a, parts);
-  else planes_as<T, CG, V, CH, false>(a, parts);
 }
 template <class T, int V>
 void planes_by_groups(const Call &a, int &parts) {
@@ -882,9 +879,10 @@ template <class T, int V>
 void rows_by_width(const Call &a, int &parts) {
   const int vectors = (a.C + V - 1) / V;
   constexpr int k16 = 16 / V;   // 16 channels per lane
-  if (a.C < kHeld) rows<T, 8 / V, V, 1, true>(a, parts);
-  else if (vectors <= 4) rows<T, 4, V, 1>(a, parts);
-  else if (vectors <= 8) rows<T, 8, V, 1>(a, parts);
+  if (a.C < kHeld) return rows<T, 8 / V, V, 1, true>(a, parts);
+  if constexpr (V > 1)   // (4 lanes, one channel each: fewer than 8)
+    if (vectors <= 4) return rows<T, 4, V, 1>(a, parts);
+  if (vectors <= 8) rows<T, 8, V, 1>(a, parts);
   else if (vectors <= 16) rows<T, 16, V, 1>(a, parts);
   else if (vectors <= 64) rows<T, 64, V, 1>(a, parts);
   else if (vectors <= 128) rows<T, 64, V, 2>(a, parts);
