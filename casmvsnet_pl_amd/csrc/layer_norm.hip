@@ -149,47 +149,65 @@ struct PlaneWeights {
   }
 };
 
+// The forward pass in 16-bit types goes over several tiles per workgroup, the next one's loads ahead: 2 x 8 x 32 x 256 x 320 in bf16 50 -> 40 us.  In float32, with
+// twice the bytes per tile in flight, one tile per workgroup is faster: 61 and 63 us, 6 x 16 x 256 x 320 11.4 and 13.5.
+template <class T>
+constexpr bool loops() { return sizeof(T) == 2; }
+constexpr size_t kForwardBlocks = 1024;
+
 template <class T, int CG, int V, bool FEW>
 __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__restrict__ x, const float *__restrict__ w, const float *__restrict__ b,
-                                                                    T *__restrict__ y, size_t first, size_t positions, int C, size_t inner, double per_c,
-                                                                    float eps, float slope) {
+                                                                    T *__restrict__ y, size_t first, size_t positions, size_t tiles, int C, size_t inner,
+                                                                    double per_c, float eps, float slope) {
   __shared__ double lds[plane_lds<CG, V>(1)];
   const PlaneTile<CG, V> tile;
-  const size_t p = ((first + blockIdx.x) * PlaneTile<CG, V>::PL + tile.pl) * V;
-  const bool live = p < positions;   // (V divides inner: all V positions or none, in one plane)
-  size_t n, at;
-  casmvs::elem::divide(live ? p : 0, inner, n, at);
-  const size_t base = n * C * inner + at;
-  PlaneLoads<T, V> xs;
-  xs.template load<false>(x, base, inner, tile.cg, CG, C, live);
   const PlaneWeights<CG> a(w, b, tile.cg, C);
-  float v[kHeld][V];
-  xs.widen(v);
-  double mean[V], rstd[V];
-  plane_statistics<1, !FEW, false, CG, V>(tile, v, C, per_c, eps, lds, mean, rstd);
-  if (!live) return;
+  PlaneLoads<T, V> xs;
+  size_t base_ahead;
+  bool live_ahead;
+  auto load_ahead = [&](size_t k) {
+    const size_t p = (k * PlaneTile<CG, V>::PL + tile.pl) * V;
+    live_ahead = p < positions;   // (V divides inner: all V positions or none, in one plane)
+    size_t n, at;
+    casmvs::elem::divide(live_ahead ? p : 0, inner, n, at);
+    base_ahead = n * C * inner + at;
+    xs.template load<false>(x, base_ahead, inner, tile.cg, CG, C, live_ahead);
+  };
+  load_ahead(first + blockIdx.x);
+  for (size_t k = first + blockIdx.x; k < tiles; k += gridDim.x) {
+    const size_t base = base_ahead;
+    const bool live = live_ahead;
+    float v[kHeld][V];
+    xs.widen(v);
+    if (loops<T>() && k + gridDim.x < tiles) load_ahead(k + gridDim.x);
+    double mean[V], rstd[V];
+    plane_statistics<1, !FEW, false, CG, V>(tile, v, C, per_c, eps, lds, mean, rstd);
+    if (live) {
 #pragma unroll
-  for (int r = 0; r < kHeld; ++r) {
-    const int c = tile.cg + r * CG;
-    if (c >= C) break;
-    Vec<T, V> t;
-    bool near = FEW;   // (a channel's store leaves as soon as its z are known: one test for all of them holds every store back, 62 -> 70 us at 2 x 8 x 32 x 256 x 320)
-    if (!FEW) {
+      for (int r = 0; r < kHeld; ++r) {
+        const int c = tile.cg + r * CG;
+        if (c >= C) break;
+        Vec<T, V> t;
+        bool near = FEW;   // (a channel's store leaves as soon as its z are known: one test for all of them holds every store back, 62 -> 70 us at 2 x 8 x 32 x 256 x 320)
+        if (!FEW) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float z = v[r][i] * (float)rstd[i] * a.w[r] + a.b[r];
-        near |= fabsf(z) <= near_zero(a.b[r], slope);
-        t.v[i] = (T)(z > 0.0f ? z : z * slope);
+          for (int i = 0; i < V; ++i) {
+            const float z = v[r][i] * (float)rstd[i] * a.w[r] + a.b[r];
+            near |= fabsf(z) <= near_zero(a.b[r], slope);
+            t.v[i] = (T)(z > 0.0f ? z : z * slope);
+          }
+        }
+        if (near) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const double z = z_of(FEW ? v[r][i] : (float)x[base + c * inner + i], mean[i], rstd[i], a.w[r], a.b[r]);
+            t.v[i] = (T)(float)(z > 0.0 ? z : z * slope);
+          }
+        }
+        casmvs::elem::store<T, V>(y + base + c * inner, t);
       }
     }
-    if (near) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const double z = z_of(FEW ? v[r][i] : (float)x[base + c * inner + i], mean[i], rstd[i], a.w[r], a.b[r]);
-        t.v[i] = (T)(float)(z > 0.0 ? z : z * slope);
-      }
-    }
-    casmvs::elem::store<T, V>(y + base + c * inner, t);
+    if (!loops<T>()) break;
   }
 }
 
@@ -827,9 +845,10 @@ template <class T, int CG, int V, Channels CH>
 void planes(const Call &a, int &parts) {
   const size_t tile = (size_t)(kThreads / CG) * V, tiles = (a.positions() + tile - 1) / tile;
   if (!a.gy) {
-    for (size_t first = 0; first < tiles; first += kLaunchBlocks)
-      hipLaunchKernelGGL((ln_forward_planes_kernel<T, CG, V, CH == kFew>), dim3(launch_blocks(tiles - first)), dim3(kThreads), 0, a.stream, (const T *)a.x, a.w, a.b,
-                         (T *)a.out, first, a.positions(), a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
+    const size_t most = loops<T>() ? kForwardBlocks : kLaunchBlocks;
+    for (size_t first = 0; first < tiles; first += loops<T>() ? tiles : most)
+      hipLaunchKernelGGL((ln_forward_planes_kernel<T, CG, V, CH == kFew>), dim3((unsigned)(tiles - first < most ? tiles - first : most)), dim3(kThreads), 0, a.stream,
+                         (const T *)a.x, a.w, a.b, (T *)a.out, first, a.positions(), tiles, a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
     return;
   }
   const unsigned grid = (unsigned)(tiles < backward_blocks(a.C) ? tiles : backward_blocks(a.C));
