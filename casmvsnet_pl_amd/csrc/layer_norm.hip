@@ -393,21 +393,29 @@ __device__ __forceinline__ void over_row(double (&v)[N], double *lds) {
   }
 }
 
+// A lane's part of a row, as loaded; 0 for a channel or row that is not there
 template <class T, int L, int V, int K>
-__device__ __forceinline__ void load_row(const T *__restrict__ x, size_t base, int t, int C, bool live, float (&v)[K][V]) {
+struct RowLoads {
+  Vec<T, V> t[K];
+  __device__ __forceinline__ void load(const T *__restrict__ x, size_t base, int lane, int C, bool live) {
 #pragma unroll
-  for (int j = 0; j < K; ++j) {
-    const int c = (j * L + t) * V;
-    if (live && c < C) {
-      const Vec<T, V> u = casmvs::elem::load<T, V>(x + base + c);
+    for (int j = 0; j < K; ++j) {
+      const int c = (j * L + lane) * V;
+      if (live && c < C) {
+        t[j] = casmvs::elem::load<T, V>(x + base + c);
+      } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[j][i] = (float)u.v[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[j][i] = 0.0f;
+        for (int i = 0; i < V; ++i) t[j].v[i] = (T)0.0f;
+      }
     }
   }
-}
+  __device__ __forceinline__ void widen(float (&v)[K][V]) const {
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[j][i] = (float)t[j].v[i];
+  }
+};
 
 // (as plane_statistics)
 template <int L, int V, int K, bool CENTRE>
@@ -442,8 +450,10 @@ __global__ __launch_bounds__(row_threads<L>()) void ln_forward_rows_kernel(const
   const size_t row = (first + blockIdx.x) * (row_threads<L>() / L) + threadIdx.x / L;
   const bool live = row < rows;
   const size_t base = live ? row * C : 0;
+  RowLoads<T, L, V, K> xs;
+  xs.load(x, base, t, C, live);
   float v[K][V];
-  load_row<T, L, V, K>(x, base, t, C, live, v);
+  xs.widen(v);
   double mean, rstd;
   row_statistics<L, V, K, !FEW>(v, t, C, per_c, eps, lds, mean, rstd);
   if (!live) return;
@@ -500,13 +510,25 @@ __global__ __launch_bounds__(row_threads<L>()) void ln_backward_rows_kernel(cons
       sw[j][i] = sb[j][i] = 0.0f;
     }
   const size_t turns = (rows + (size_t)gridDim.x * G - 1) / ((size_t)gridDim.x * G);   // the same for every thread: the exchanges need all lanes
-  for (size_t turn = 0; turn < turns; ++turn) {
+  // The next turn's loads are issued before this one is worked on: bf16 65536 x 1024 202 -> 93 us, 8191 x 1000 30 -> 24 (float32: no difference at 8192 x 1024)
+  RowLoads<T, L, V, K> xs, gs;
+  size_t base_ahead;
+  bool live_ahead;
+  auto load_ahead = [&](size_t turn) {
     const size_t row = (turn * gridDim.x + blockIdx.x) * G + threadIdx.x / L;
-    const bool live = row < rows;
-    const size_t base = live ? row * C : 0;
+    live_ahead = row < rows;
+    base_ahead = live_ahead ? row * C : 0;
+    xs.load(x, base_ahead, t, C, live_ahead);
+    gs.load(gy, base_ahead, t, C, live_ahead);   // (g of a missing channel or row is 0)
+  };
+  load_ahead(0);
+  for (size_t turn = 0; turn < turns; ++turn) {
+    const size_t base = base_ahead;
+    const bool live = live_ahead;
     float v[K][V], g[K][V];
-    load_row<T, L, V, K>(x, base, t, C, live, v);
-    load_row<T, L, V, K>(gy, base, t, C, live, g);   // (g of a missing channel or row is 0)
+    xs.widen(v);
+    gs.widen(g);
+    if (turn + 1 < turns) load_ahead(turn + 1);
     double mean, rstd, m[2] = {0.0, 0.0};
     row_statistics<L, V, K, !FEW>(v, t, C, per_c, eps, lds, mean, rstd);
     const float r32 = (float)rstd;
@@ -802,9 +824,10 @@ enum Form { kAny, kPlanes, kRows };
 Form form_of(int C, size_t inner) { return inner == 1 ? (C <= 8192 ? kRows : kAny) : (C <= 64 * kHeld ? kPlanes : kAny); }
 
 // Workgroups of the fused backward pass = rows of its partial sums.  Three per CU are resident (registers) and keep the memory busiest: bf16 2 x 8 x 32 x 256 x 320
-// 49 us with 768, 54 with 512, 57 with 1024.  Past 256 channels a row of sums is as long as a row of data and there are few rows: 8191 x 1000 bf16 30 us
-// with 512, 39 with 768 (rows 983040 x 32: 83 and 72).
-size_t backward_blocks(int C) { return C > 256 ? 512 : 768; }
+// 49 us with 768, 54 with 512, 57 with 1024.  Past 256 channels a row of sums is as long as a row of data and there are few rows: bf16 8191 x 1000 24 us with
+// 512, 30 with 768 (65536 x 1024 93 and 111; but 983040 x 32 in float32 83 and 72), and past 2048 the same again: bf16 1000 x 4096 23 us with 256, 30 with 512
+// (2000 x 2048 in float32 28 and 24).
+size_t backward_blocks(int C) { return C > 2048 ? 256 : C > 256 ? 512 : 768; }
 
 // A launch has fewer than 2^32 threads: a larger forward pass (more than 2^31 elements and up) goes in several
 constexpr size_t kLaunchBlocks = (size_t)1 << 22;
