@@ -104,6 +104,17 @@ def test_layer_norm_and_gradients_against_float64(dev, shape, rows, slope, dtype
     ln_check(dev, x, torch.rand(C, generator=g) + 0.5, torch.randn(C, generator=g) * 0.3, torch.randn(shape, generator=g).to(dtype), slope=slope, channels_last=rows)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape,rows", [((5000, 264), True), ((70000, 9), True), ((600, 2100), True), ((1100, 1030), True), ((70000, 6), True), ((2, 8, 300002), False),
+                                        ((1, 20, 100003), False), ((2, 100, 20004), False), ((3, 3, 300000), False)])
+def test_layer_norm_where_a_workgroup_takes_several_turns(dev, shape, rows, dtype):
+    """More rows / tiles than the passes have workgroups for: what is loaded ahead for the next turn, and the last turn that only some of them have."""
+    g = torch.Generator().manual_seed(sum(shape))
+    C = shape[-1] if rows else shape[1]
+    x = (torch.randn(shape, generator=g) * 1.7 + 0.6).to(dtype)
+    ln_check(dev, x, torch.rand(C, generator=g) + 0.5, torch.randn(C, generator=g) * 0.3, torch.randn(shape, generator=g).to(dtype), channels_last=rows)
+
+
 @pytest.mark.parametrize("rows", [False, True])
 def test_layer_norm_without_affine_and_with_the_relu_slope(dev, rows):
     g = torch.Generator().manual_seed(1)
@@ -576,6 +587,57 @@ def test_the_same_bits_again_on_another_stream_and_in_a_graph(dev, name):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(captured, want))
         assert all(torch.equal(p, q) for p, q in zip(call(), want))   # eager work between the replays
+
+
+def test_two_threads_at_once(dev):
+    """Every operator from two host threads, each on a stream of its own, over and over: the same bits as alone."""
+    import threading
+    calls = [_calls(dev) for _ in range(2)]   # (their norms and inputs apart)
+    want = {name: [t.clone() for t in call()] for name, call in calls[0].items()}
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(mine):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                for name, call in mine.items():
+                    got = call()
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(p, q) for p, q in zip(got, want[name])):
+                        wrong.append(name)
+    threads = [threading.Thread(target=work, args=(mine,)) for mine in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+
+
+def test_gradients_add_up_over_calls_and_have_no_second_derivative(dev):
+    g = torch.Generator().manual_seed(17)
+    x = torch.randn(2, 8, 6, 10, generator=g).to(dev).requires_grad_()
+    cost, values, gt, mask = (t.to(dev) for t in ce_inputs(1, 8, 6, 10, True, F32, 5))
+    cost.requires_grad_()
+    for norm, checkpoint in ((M.LayerNormAct(8), "f32"), (M.ABN(8), "8bit"), (None, None)):
+        if norm is None:
+            leaves, out = [cost], lambda: A.depth_cross_entropy(cost, values, gt, mask)
+        else:
+            norm = norm.to(dev).train()
+            leaves, out = [x, norm.weight, norm.bias], lambda: (T.abn_train(norm, x, checkpoint) ** 2).sum()
+        for t in leaves:
+            t.grad = None
+        out().backward()
+        once = [t.grad.clone() for t in leaves]
+        out().backward()   # into the gradients that are there
+        assert all(torch.equal(t.grad, 2 * p) for t, p in zip(leaves, once))
+        torch.nn.utils.clip_grad_norm_(leaves, 1e-3)   # writes them in place
+        for t in leaves:
+            t.grad.zero_()
+        first = torch.autograd.grad(out(), leaves[0], create_graph=True)[0]
+        assert torch.equal(first.detach(), once[0])
+        # (torch's own words for it: the gradient is cut off from the leaf, or from everything where grad_output is a constant)
+        with pytest.raises(RuntimeError, match="to not have been used in the graph|does not require grad"):
+            torch.autograd.grad(first.sum(), leaves[0])
 
 
 def test_offsets_beyond_32_bits(dev):
