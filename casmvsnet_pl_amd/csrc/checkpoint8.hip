@@ -8,8 +8,11 @@
 // multiplies every gradient element, so it is kept exactly.  The statistics, xhat and z are computed in 64 bits: a block's codes and the sign of z are the
 // ones of the definition, not of one order of float32 roundings.  y itself is the float32 fma of casmvs_abn_train_apply_f32.
 //
-// Everything here waits for memory: forward 4 + 4 + 33/32 + 1/8 bytes per element, backward sums 4 + 37/32, apply 8 + 37/32 (keeping x and y in
-// float32 reads 12 and 12 and writes 4).
+// Everything here waits for memory: forward 4 + 4 + 33/32 + 1/8 bytes read and written per element and 4 for the sums, backward sums 4 + 37/32, apply
+// 8 + 37/32 (keeping x and y in float32 reads 12 and 12 and writes 4).  Measured, both launches of a pass together, forward / backward:
+//   2 x 8 x 32 x 256 x 320   101 us (5.5 TB/s) / 95 us (6.3 TB/s: the second pass finds part of the first one's data in the caches)
+//   6 x 8 x 512 x 640         39 us            / 38 us                 2 x 64 x 6 x 16 x 20   8.4 us / 6.1 us (one launch each)
+// pack8 of 64 x 983040 float32 61 us, unpack8 47 us (5.2 and 6.7 TB/s); of 32 x 160 the time of a launch.
 #include "block8.h"
 
 namespace {
@@ -453,7 +456,9 @@ __global__ __launch_bounds__(kWide) void abn8_backward_one_kernel(const float *_
       gradient_blocks<WIDE, false>(gy, from, p.gx, (size_t)img * C + c, blk + threadIdx.x / kLanes, groups, n, nb, m, p.slope);
 }
 
-// Elements of a channel up to which one workgroup does both passes over it: one launch less, on as many CUs as there are channels
+// Elements of a channel up to which one workgroup does both passes over it: one launch less, on as many CUs as there are channels.  Forward / backward in one launch
+// and in two: 64 channels of 8192 elements 7.1 / 6.5 and 8.6 / 8.9 us, of 16384 8.4 / 8.5 and 9.2 / 8.8, of 32768 14.4 / 12.3 and 11.3 / 10.5; 256 of 16384
+// 11.4 / 11.0 and 14.7 / 13.6.
 constexpr size_t kOneLaunch = 16384;
 
 // Workgroups that form a channel's sums: at least 4096 elements each, at most 1024 workgroups in all (four per CU)

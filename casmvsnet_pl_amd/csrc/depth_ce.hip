@@ -9,6 +9,8 @@
 // equal, and only where equal ones were met they are compared again in 64 bits, where differences of float32 depths are exact: which of two planes is the nearer one does not
 // depend on a rounding.
 // Both passes wait for memory: forward cost + depth value per hypothesis, backward cost in and gradient out.  A pixel whose mask is not set reads nothing.
+// Forward (two launches) / backward: 2 x 48 x 128 x 160 9.3 / 5.5 us - launches -, 2 x 32 x 256 x 320 14 / 9.3, 2 x 8 x 512 x 640 16 / 11 us; bf16 with one set of
+// planes per sample, 192 x 295 x 399: 28 / 24 us (45 MB in, 45 MB out: strides of 117705 elements, so 2-byte loads).
 #include "elem_types.h"
 
 namespace {
