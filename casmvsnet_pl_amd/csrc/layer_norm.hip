@@ -19,7 +19,7 @@
 //
 // Planes and rows touch each element once and wait for memory: 8 bytes per float32 element forward, 12 backward (a copy of gigabytes reaches 4.7 to 5.1 TB/s, one
 // that the caches hold more).  Float32, forward / backward with the weight gradients, the launches and the sums' second kernel included:
-//   2 x 8 x 32 x 256 x 320   61 us (5.5 TB/s) / 99 us (5.1 TB/s)      6 x 8 x 512 x 640   20 us (6.4) / 35 us (5.3)      6 x 16 x 256 x 320   11 / 25 us
+//   2 x 8 x 32 x 256 x 320   60 us (5.6 TB/s) / 99 us (5.1 TB/s)      6 x 8 x 512 x 640   20 us (6.4) / 35 us (5.3)      6 x 16 x 256 x 320   11 / 25 us
 //   983040 rows of 32        45 us (5.6)      / 71 us (5.3)           8192 rows of 1024   14 us (4.9) / 27 us (3.7)
 // and in bf16: 2 x 8 x 32 x 256 x 320   40 us (4.2) / 49 us (5.1)     8191 rows of 1000   11 us (3.0) / 24 us (2.1)     65536 rows of 1024   68 us (3.9) / 93 us (4.3).
 // Small tensors cost their launches: 2 x 64 x 6 x 16 x 20 9 / 16 us.
@@ -162,7 +162,8 @@ template <class T>
 constexpr bool loops() { return sizeof(T) == 2; }
 constexpr size_t kForwardBlocks = 1024;
 
-template <class T, int CG, int V, bool FEW>
+// PAST: y goes past the caches
+template <class T, int CG, int V, bool FEW, bool PAST>
 __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__restrict__ x, const float *__restrict__ w, const float *__restrict__ b,
                                                                     T *__restrict__ y, size_t first, size_t positions, size_t tiles, int C, size_t inner,
                                                                     double per_c, float eps, float slope) {
@@ -211,7 +212,8 @@ __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__
             t.v[i] = (T)(float)(z > 0.0 ? z : z * slope);
           }
         }
-        casmvs::elem::store<T, V>(y + base + c * inner, t);
+        if (PAST) casmvs::elem::store_past<T, V>(y + base + c * inner, t);
+        else casmvs::elem::store<T, V>(y + base + c * inner, t);
       }
     }
     if (!loops<T>()) break;
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(kThreads) void ln_forward_planes_kernel(const T *__
 enum Channels { kFew, kSome, kFull };
 
 // gx, and of every workgroup the sums over its tiles of g h and g per channel: partial[workgroup][0 / 1][c].  AFFINE: the weight gradient is wanted.  PAST: gx goes
-// past the caches (the forward pass's y does not: 61 and 60 us at 2 x 8 x 32 x 256 x 320).
+// past the caches.
 template <class T, int CG, int V, bool AFFINE, Channels CH, bool PAST>
 __global__ __launch_bounds__(kThreads) void ln_backward_planes_kernel(const T *__restrict__ x, const T *__restrict__ gy, const float *__restrict__ w,
                                                                      const float *__restrict__ b, T *__restrict__ gx, float *__restrict__ partial,
@@ -874,20 +876,24 @@ struct Call {   // arguments of either direction
 template <class T, int CG, int V, Channels CH>
 void planes(const Call &a, int &parts) {
   const size_t tile = (size_t)(kThreads / CG) * V, tiles = (a.positions() + tile - 1) / tile;
+  // Large outputs go past the caches (8 channels per group, pairs of positions; a branch in the kernel gains nothing): a forward pass then leaves x there for the
+  // backward pass instead of y.  2 x 8 x 32 x 256 x 320 in float32, forward and the backward pass right behind it 51 + 116 -> 59 + 84 us; on their own 61 -> 60 and
+  // 104 -> 99 us (bf16 backward 53 -> 49).
+  constexpr bool may = CH == kFull && V > 1;
+  const bool past = may && casmvs::elem::streams(a.positions() * a.C * sizeof(T));
   if (!a.gy) {
     const size_t most = loops<T>() ? kForwardBlocks : kLaunchBlocks;
+    auto kernel = past ? ln_forward_planes_kernel<T, CG, V, CH == kFew, may> : ln_forward_planes_kernel<T, CG, V, CH == kFew, false>;
     for (size_t first = 0; first < tiles; first += loops<T>() ? tiles : most)
-      hipLaunchKernelGGL((ln_forward_planes_kernel<T, CG, V, CH == kFew>), dim3((unsigned)(tiles - first < most ? tiles - first : most)), dim3(kThreads), 0, a.stream,
-                         (const T *)a.x, a.w, a.b, (T *)a.out, first, a.positions(), tiles, a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles - first < most ? tiles - first : most)), dim3(kThreads), 0, a.stream, (const T *)a.x, a.w, a.b, (T *)a.out, first,
+                         a.positions(), tiles, a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
     return;
   }
   const unsigned grid = (unsigned)(tiles < backward_blocks(a.C) ? tiles : backward_blocks(a.C));
   parts = (int)grid;
   float *sums = a.sums(parts);
-  auto kernel = a.partial ? ln_backward_planes_kernel<T, CG, V, true, CH, false> : ln_backward_planes_kernel<T, CG, V, false, CH, false>;
-  if constexpr (CH == kFull && V > 1)   // large outputs of 8 channels per group: 2 x 8 x 32 x 256 x 320 in float32 104 -> 99 us, in bf16 53 -> 49 (a branch in the kernel gains nothing)
-    if (casmvs::elem::streams(a.positions() * a.C * sizeof(T)))
-      kernel = a.partial ? ln_backward_planes_kernel<T, CG, V, true, CH, true> : ln_backward_planes_kernel<T, CG, V, false, CH, true>;
+  auto kernel = past ? (a.partial ? ln_backward_planes_kernel<T, CG, V, true, CH, may> : ln_backward_planes_kernel<T, CG, V, false, CH, may>)
+                     : (a.partial ? ln_backward_planes_kernel<T, CG, V, true, CH, false> : ln_backward_planes_kernel<T, CG, V, false, CH, false>);
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0, a.stream, (const T *)a.x, (const T *)a.gy, a.w, a.b, (T *)a.out, sums, a.positions(), tiles,
                      a.C, a.inner, 1.0 / a.C, a.eps, a.slope);
 }
