@@ -20,7 +20,7 @@ What a step keeps for its backward pass: float32 tensors (checkpoint="f32": the 
 (CascadeMVSNet.checkpoint_mode) 8-bit checkpoints: an ABN keeps 8 bits of its normalised input and one bit per element, the convolution behind it rebuilds its
 input from the same bytes (behind a layer norm: from the norm's input, exactly), and a convolution whose input is anything else (a cost volume, a skip sum)
 packs that.  The forward pass is the same to float32's rounding; the gradients carry the rounding of the 8 bits.  One step at 640x512, 3 views: peak memory
-2.31 -> 0.84 GiB with ABN, 2.06 -> 1.32 GiB with layer norm; 1 % and 6 % more time.
+2.31 -> 0.84 GiB with ABN, 2.06 -> 1.32 GiB with layer norm; 1 % and 7 % more time.
 
 torch is the autograd tape and the allocator; the skip additions of the U-Net and the gradient accumulation are torch adds.  Nothing here runs on CPU tensors.  DESIGN.md 2.6 has the kernels and the measured step
 times (18 ms per step at the reference's default training configuration, 15 ms captured as one hipGraph).
@@ -861,18 +861,23 @@ def train_steps(model, batches, optimizer, device="cuda", loss="sl1"):
         raise ValueError(f"train_steps: loss={loss!r} (sl1 or cross_entropy)")
     from .pipeline import DevicePrefetcher
     model.train()
-    if loss == "cross_entropy":
-        model.return_cost = True
     loss_of = sl1_loss if loss == "sl1" else cross_entropy_loss
+    returned = model.return_cost if loss == "cross_entropy" else None   # (as it was, afterwards)
     losses = []
-    for b in DevicePrefetcher(batches, device, depth=2):
-        depths = {k: torch.stack([d[k] for d in b["depths"]]).to(device) for k in b["depths"][0]}
-        masks = {k: torch.stack([m[k] for m in b["masks"]]).to(device) for k in b["masks"][0]}
-        optimizer.zero_grad(set_to_none=True)
-        results = model(b["imgs"], b["proj_mats"], b["init_depth_min"], b["depth_interval"])
-        value = loss_of(results, depths, masks)
-        value.backward()
-        optimizer.step()
-        release_plan()   # the step's graph is consumed
-        losses.append(float(value.detach()))
+    try:
+        if loss == "cross_entropy":
+            model.return_cost = True
+        for b in DevicePrefetcher(batches, device, depth=2):
+            depths = {k: torch.stack([d[k] for d in b["depths"]]).to(device) for k in b["depths"][0]}
+            masks = {k: torch.stack([m[k] for m in b["masks"]]).to(device) for k in b["masks"][0]}
+            optimizer.zero_grad(set_to_none=True)
+            results = model(b["imgs"], b["proj_mats"], b["init_depth_min"], b["depth_interval"])
+            value = loss_of(results, depths, masks)
+            value.backward()
+            optimizer.step()
+            release_plan()   # the step's graph is consumed
+            losses.append(float(value.detach()))
+    finally:
+        if loss == "cross_entropy":
+            model.return_cost = returned
     return losses

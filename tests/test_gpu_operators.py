@@ -697,6 +697,24 @@ def test_training_step_with_the_cross_entropy_loss(dev, norm_act, mode):
     assert res["cost_0"].shape == res["depth_values_0"].shape == (1, 8, 64, 96)
 
 
+@pytest.mark.parametrize("loss", ["sl1", "cross_entropy"])
+def test_train_steps_with_either_loss(dev, loss):
+    """The training loop's first loss is the step's; the model's switches are as they were afterwards."""
+    from casmvsnet_pl_amd.synthetic import make_inputs
+    model, _, value, _ = _step(dev, M.LayerNormAct, "8bit", loss)
+    model.return_cost = False
+    imgs, proj, dmin, dint = make_inputs(1, 3, 64, 96, seed=0)
+    g = torch.Generator().manual_seed(0)
+    depths = {f"level_{l}": dmin + 100 * torch.rand((64 >> l, 96 >> l), generator=g) for l in range(3)}
+    masks = {f"level_{l}": torch.rand((64 >> l, 96 >> l), generator=g) < 0.8 for l in range(3)}
+    batch = {"imgs": imgs, "proj_mats": proj, "init_depth_min": dmin, "depth_interval": dint, "depths": [depths], "masks": [masks]}
+    before = [p.detach().clone() for p in model.parameters()]
+    losses = T.train_steps(model, [batch] * 2, torch.optim.SGD(model.parameters(), lr=1e-4), dev, loss=loss)
+    # (the same kernels on the same values in the same order; torch's own SmoothL1 mean may split its sum otherwise)
+    assert abs(losses[0] - float(value)) <= 1e-6 * float(value) and len(losses) == 2 and losses[1] == losses[1]
+    assert model.return_cost is False and any(not torch.equal(p, q) for p, q in zip(model.parameters(), before))
+
+
 def test_layer_norm_model_in_train_mode_against_torch_on_the_cpu(dev):
     """LayerNormAct in the reference's layers: FeatureNet's and CostRegNet's forwards and weight gradients against torch autograd in float64."""
     import torch.nn.functional as F
