@@ -211,6 +211,7 @@ extern "C" int casmvs_depth_ce_forward(const void *cost, const float *depth_valu
   CASMVS_REQUIRE(loss && share && workspace, "depth_ce_forward: null pointer");
   const size_t pixels = (size_t)B * hw, blocks = pixels ? forward_blocks(pixels, D) : 0;
   CASMVS_REQUIRE(!pixels || (cost && depth_values && depth_gt && stats && target), "depth_ce_forward: null pointer");
+  CASMVS_REQUIRE((((uintptr_t)stats | (uintptr_t)workspace) & 7) == 0, "depth_ce_forward: stats and workspace on 8-byte boundaries");
   hipStream_t st = (hipStream_t)stream;
   double *partial = (double *)workspace;
   if (pixels) {
@@ -234,6 +235,7 @@ extern "C" int casmvs_depth_ce_backward(const void *cost, const float *stats, co
   const size_t pixels = (size_t)B * hw;
   if (!pixels) return CASMVS_OK;
   CASMVS_REQUIRE(cost && stats && target && share && grad_loss && grad_cost, "depth_ce_backward: null pointer");
+  CASMVS_REQUIRE(((uintptr_t)stats & 7) == 0, "depth_ce_backward: stats on an 8-byte boundary");
   const size_t blocks = (pixels + kThreads - 1) / kThreads;
   size_t split = 2048 / blocks;   // few pixels: pieces of the hypothesis axis
   split = split < 1 ? 1 : split > (size_t)D ? (size_t)D : split;

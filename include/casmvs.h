@@ -666,7 +666,8 @@ int casmvs_abn8_backward_f32(const float *grad_y, const void *codes, const void 
  * bytes or NULL.  The class of a pixel is the hypothesis nearest to depth_gt (the lowest index on ties); a pixel counts if its mask is not 0, depth_gt
  * lies inside [min, max] of its hypotheses and some cost is above -inf.  loss = mean over the counted pixels of -log softmax(cost)[class], share = 1 / count
  * (one float each); both 0 where no pixel counts.  stats (B, h*w, 2) floats (8-byte aligned), target (B, h*w): what the backward pass takes beside cost.
- * B h w < 2^31, D <= 65536.  grad_loss: one device float; grad_cost has cost's type, 0 at every pixel that does not count.  workspace: casmvs_depth_ce_workspace_bytes. */
+ * B h w < 2^31, D <= 65536.  grad_loss: one device float; grad_cost has cost's type, 0 at every pixel that does not count.  workspace: casmvs_depth_ce_workspace_bytes,
+ * 8-byte aligned. */
 size_t casmvs_depth_ce_workspace_bytes(int B, int D, size_t hw);
 int casmvs_depth_ce_forward(const void *cost, const float *depth_values, const float *depth_gt, const void *mask, float *stats, int *target, float *loss,
                             float *share, void *workspace, int dtype, int B, int D, size_t hw, int per_pixel, void *stream);

@@ -89,6 +89,9 @@ def test_c_abi_refuses_bad_arguments():
     refused(lib.casmvs_depth_ce_forward(_p(), None, _p(), None, _p(), _p(), _p(), _p(), _p(), 0, 1, 4, 16, 1, None), b"null pointer")
     refused(lib.casmvs_depth_ce_forward(_p(), _p(), _p(), None, _p(), _p(), _p(), None, _p(), 0, 1, 4, 16, 1, None), b"null pointer")
     refused(lib.casmvs_depth_ce_backward(_p(), _p(), _p(), _p(), None, _p(), 0, 1, 4, 16, None), b"null pointer")
+    refused(lib.casmvs_depth_ce_forward(_p(), _p(), _p(), None, _p(12), _p(), _p(), _p(), _p(), 0, 1, 4, 16, 1, None), b"8-byte")
+    refused(lib.casmvs_depth_ce_forward(_p(), _p(), _p(), None, _p(), _p(), _p(), _p(), _p(12), 0, 1, 4, 16, 1, None), b"8-byte")
+    refused(lib.casmvs_depth_ce_backward(_p(), _p(12), _p(), _p(), _p(), _p(), 0, 1, 4, 16, None), b"8-byte")
     assert lib.casmvs_depth_ce_workspace_bytes(0, 4, 16) == 0
 
 
