@@ -262,6 +262,9 @@ __global__ __launch_bounds__(kThreads) void ln_backward_planes_kernel(const T *_
     if (k + gridDim.x < tiles) load_ahead(k + gridDim.x);
     double mean[V], rstd[V], m[2][V];
     plane_statistics<2, !FEW, FULL, CG, V>(tile, v, C, per_c, eps, lds, mean, rstd);
+    // A thread without a position holds zeros, and eps = 0 leaves it 1 / sqrt(0): its h has to stay 0 for the sums over positions
+#pragma unroll
+    for (int i = 0; i < V; ++i) rstd[i] = live ? rstd[i] : 0.0;
     if (FEW) {
 #pragma unroll
       for (int i = 0; i < V; ++i) m[0][i] = m[1][i] = 0.0;

@@ -1,0 +1,113 @@
+// The training-side operators (layer_norm.hip, checkpoint8.hip, depth_ce.hip) on the CPU, as run_kernels13.cpp: the calls at the edge of what their entry points allow.
+// The argument names the part that runs.  Every buffer is a heap allocation of exactly its size.
+#define __shared__ static   // the kernels keep their LDS in function-scope arrays (workgroups run one after the other here)
+#include "support.h"
+
+// what these sources use beyond the emulated subset
+inline double hipemu_rsq(double a) { return (double)(float)(1.0 / std::sqrt(a)); }   // an estimate of 24 bits
+#define __builtin_amdgcn_rsq hipemu_rsq
+#define __builtin_amdgcn_exp2f(x) exp2f(x)
+#define __builtin_nontemporal_store(v, p) (*(p) = (v))
+inline int hipemu_bpermute(int from, int v) { return hipemu_lane_exchange(v, (from >> 2) & 63); }
+#define __builtin_amdgcn_ds_bpermute hipemu_bpermute
+
+#include "block8.h"
+#include "elem_types.h"
+
+namespace ln {
+#include "layer_norm.hip"
+}
+
+template <class T>
+static double value(T v) { return (double)(float)v; }
+
+static double g_worst = 0;
+static void take(const char *what, double err, double limit) {
+  printf("%s: %.2e of the limit\n", what, err / limit);
+  g_worst = std::fmax(g_worst, std::isfinite(err) ? err / limit : 1e9);
+}
+
+// eps = 0: a thread without a position has no spread to divide by, and nothing of it may reach a sum
+template <class T>
+static void no_eps_check(const char *name, int dtype, double half_step, size_t outer, int C, size_t inner) {
+  const size_t numel = outer * C * inner, positions = outer * inner;
+  std::vector<T> x(numel), gy(numel), y(numel), gx(numel);
+  std::vector<float> w(C), b(C), gw(C), gb(C);
+  const float slope = 0.01f;
+  for (size_t i = 0; i < numel; ++i) { x[i] = (T)(rnd() * 2.0f + 0.3f); gy[i] = (T)rnd(); }
+  for (int c = 0; c < C; ++c) { w[c] = 1.0f + 0.4f * rnd(); b[c] = 0.3f * rnd(); }
+  std::vector<char> ws(casmvs_layer_norm_backward_workspace_bytes(dtype, outer, C, inner));
+  if (casmvs_layer_norm_forward(x.data(), w.data(), b.data(), y.data(), dtype, outer, C, inner, 0.0f, slope, nullptr) ||
+      casmvs_layer_norm_backward(x.data(), gy.data(), w.data(), b.data(), gx.data(), gw.data(), gb.data(), ws.data(), dtype, outer, C, inner, 0.0f, slope, nullptr)) {
+    printf("%s: %s\n", name, casmvs_last_error());
+    g_worst = 1e9;
+  }
+  std::vector<double> sw(C, 0.0), sb(C, 0.0), aw(C, 0.0), ab(C, 0.0);
+  double e = 0;
+  auto worse = [&](double off, double limit) { e = std::isfinite(off) ? std::fmax(e, off / limit) : 1e9; };
+  for (size_t p = 0; p < positions; ++p) {
+    const size_t base = p / inner * C * inner + p % inner;
+    double mean = 0, var = 0, m1 = 0, m2 = 0, a1 = 0, a2 = 0;
+    for (int c = 0; c < C; ++c) mean += value(x[base + c * inner]) / C;
+    for (int c = 0; c < C; ++c) var += (value(x[base + c * inner]) - mean) * (value(x[base + c * inner]) - mean) / C;
+    const double r = 1.0 / std::sqrt(var);
+    for (int pass = 0; pass < 2; ++pass)
+      for (int c = 0; c < C; ++c) {
+        const size_t at = base + c * inner;
+        const double h = (value(x[at]) - mean) * r, z = h * w[c] + b[c], g = value(gy[at]) * (z > 0 ? 1.0 : slope), want = z > 0 ? z : z * slope;
+        if (pass == 0) {
+          // z: the rounded x - mean, 1 / sqrt, two products, the sum and the slope, each half a step; then the type's own
+          worse(std::fabs(value(y[at]) - want), std::fabs(want) * half_step + 0x1p-24 * (4 * std::fabs(h * w[c]) + 2 * std::fabs(z)) + 1e-12);
+          m1 += g * w[c] / C;
+          m2 += g * w[c] * h / C;
+          a1 += std::fabs(g * w[c]) / C;
+          a2 += std::fabs(g * w[c] * h) / C;
+          sw[c] += g * h;
+          sb[c] += g;
+          aw[c] += std::fabs(g * h);
+          ab[c] += std::fabs(g);
+        } else {   // at most 16 float32 roundings a term, and the type's own
+          const double gxw = r * (g * w[c] - m1 - h * m2);
+          worse(std::fabs(value(gx[at]) - gxw), std::fabs(gxw) * half_step + 16 * 0x1p-24 * r * (std::fabs(g * w[c]) + a1 + std::fabs(h) * a2) + 1e-12);
+        }
+      }
+  }
+  for (int c = 0; c < C; ++c) {
+    worse(std::fabs(gw[c] - sw[c]), 64 * 0x1p-24 * aw[c] + 1e-12);
+    worse(std::fabs(gb[c] - sb[c]), 64 * 0x1p-24 * ab[c] + 1e-12);
+  }
+  char what[120];
+  snprintf(what, sizeof(what), "eps 0 %s (%zu, %d, %zu)", name, outer, C, inner);
+  take(what, e, 1.05);
+}
+
+int main(int argc, char **argv) {
+  hipemu::g_lds = smem_raw;
+  const std::string part = argc > 1 ? argv[1] : "";
+  using casmvs::elem::bf16;
+  if (part == "eps0") {
+    // fewer positions than a tile holds, or a last tile that is not full: 1, 2, 4, 8, 16 and 64 groups of channels, fewer than 8 channels, pairs and single positions
+    for (size_t inner : {size_t(65), size_t(52)}) {
+      no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 2, 8, inner);
+      no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 1, 3, inner);
+      no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 1, 16, inner);
+      no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 1, 20, inner);
+    }
+    no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 2, 32, 12);
+    no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 3, 64, 21);
+    no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 1, 100, 17);
+    no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 1, 200, 9);
+    no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 1, 520, 3);
+    no_eps_check<bf16>("bf16", CASMVS_DTYPE_BF16, 0x1p-8, 2, 8, 300);
+    no_eps_check<bf16>("bf16", CASMVS_DTYPE_BF16, 0x1p-8, 1, 6, 10);
+    no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 1, 8, 1024);   // a full tile
+    no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 5, 20, 1);     // rows
+    no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 3, 5, 1);
+    no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 2, 300, 1);
+  } else {
+    printf("no part named %s\n", part.c_str());
+    return 2;
+  }
+  printf(g_worst < 1.0 ? "ALL OK (worst %.2e)\n" : "FAILED (worst %.2e)\n", g_worst);
+  return g_worst < 1.0 ? 0 : 1;
+}
