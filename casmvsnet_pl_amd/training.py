@@ -530,7 +530,7 @@ def abn_train(norm, x, checkpoint="f32"):
         x = x.contiguous().float()
         y = norm(x)
         if checkpoint == "8bit":
-            y._casmvs_made_by = (y._version, norm, x)
+            y._casmvs_made_by = (y._version, _NormedFrom(norm, x))
         return y
     if not getattr(norm, "affine", True) or norm.weight is None:
         raise RuntimeError("training: ABN without affine parameters is not supported")
@@ -556,18 +556,31 @@ def _unpack(shape, slope):
     return lambda codes, scales, *affine: ops.unpack8(ops.Packed8(codes, scales, shape, torch.float32, (*affine, slope) if affine else None))
 
 
+class _NormedFrom:
+    """What a layer norm made its output of, as it was then: the tensors that it read with their versions, its eps and slope."""
+
+    __slots__ = ("tensors", "versions", "eps", "slope")
+
+    def __init__(self, norm, x):
+        self.tensors = (x, norm.weight, norm.bias) if norm.affine else (x,)
+        self.versions = [t._version for t in self.tensors]
+        self.eps, self.slope = norm.eps, norm.leaky_slope()
+
+    def unchanged(self):
+        return all(t._version == version for t, version in zip(self.tensors, self.versions))
+
+
 def kept_input(x):
     """What a convolution keeps of its input x under checkpoint "8bit": (tensors, the function that makes x of them, to 8 bits or exactly)."""
     version, *made_by = getattr(x, "_casmvs_made_by", (None,))
-    if version is None or version != x._version:   # not a norm's output, or written to since
+    # not a norm's output, or written to since; or what a layer norm made it of was
+    if version is None or version != x._version or (isinstance(made_by[0], _NormedFrom) and not made_by[0].unchanged()):
         packed = ops.pack8(x.detach().float())
         return (packed.codes, packed.scales), _unpack(tuple(x.shape), 1.0)
-    if isinstance(made_by[0], LayerNormAct):
-        norm, source = made_by
-        eps, slope = norm.eps, norm.leaky_slope()
-        if norm.affine:
-            return (source.detach(), norm.weight.detach(), norm.bias.detach()), lambda t, w, b: ops.layer_norm(t, w, b, eps, slope)
-        return (source.detach(),), lambda t: ops.layer_norm(t, eps=eps, slope=slope)
+    if isinstance(made_by[0], _NormedFrom):
+        source, = made_by
+        eps, slope = source.eps, source.slope
+        return tuple(t.detach() for t in source.tensors), lambda t, *affine: ops.layer_norm(t, *affine, eps=eps, slope=slope)
     buffer, slope = made_by
     N, C = x.shape[:2]
     codes, scales, weight, bias = _kept8(N, C, x.numel() // (N * C)).packed(buffer)

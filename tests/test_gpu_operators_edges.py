@@ -1,7 +1,12 @@
-"""GPU tests of the training-side operators at the edge of what their entry points allow: layer norm without an eps.  Definitions, bounds and fixtures are
+"""GPU tests of the training-side operators at the edge of what their entry points allow: layer norm without an eps, what is kept
+across writes, under other grad modes and in memory.  Definitions, bounds and fixtures are
 test_gpu_operators.py's."""
 import pytest
 import torch
+
+import casmvsnet_pl_amd as M
+from casmvsnet_pl_amd import ops
+from casmvsnet_pl_amd import training as T
 
 from test_gpu_operators import BF16, F16, F32, dev, ln_check   # noqa: F401  (dev is a fixture)
 
@@ -18,3 +23,29 @@ def test_layer_norm_without_an_eps(dev, shape, rows, dtype):   # noqa: F811
     C = shape[-1] if rows else shape[1]
     x = (torch.randn(shape, generator=g) * 1.7 + 0.6).to(dtype)
     ln_check(dev, x, torch.rand(C, generator=g) + 0.5, torch.randn(C, generator=g) * 0.3, torch.randn(shape, generator=g).to(dtype), eps=0.0, channels_last=rows)
+
+
+@pytest.mark.parametrize("written", ["nothing", "source", "weight", "bias", "eps and slope", "another weight"])
+def test_conv8_behind_a_layer_norm_whose_source_is_written_to(dev, written):   # noqa: F811
+    """What the convolution forms its input from again are the tensors that the norm read: written to since, they no longer make it, and it packs its input instead."""
+    g = torch.Generator().manual_seed(7)
+    w = (torch.randn(16, 8, 3, 3, 3, generator=g) * 0.2).to(dev).requires_grad_()
+    source = torch.randn(2, 8, 8, 12, 16, generator=g).to(dev).requires_grad_() * 1.0
+    norm = M.LayerNormAct(8).to(dev)
+    x = T.abn_train(norm, source, checkpoint="8bit")
+    want_x = x.detach().clone()
+    with torch.no_grad():
+        if written == "source":
+            source.mul_(source)
+        elif written in ("weight", "bias"):
+            getattr(norm, written).add_(0.5)
+        elif written == "eps and slope":
+            norm.eps, norm.activation_param = 0.5, 0.3
+        elif written == "another weight":
+            norm.weight = torch.nn.Parameter(norm.weight + 0.5)
+    if written in ("source", "weight", "bias"):
+        want_x = ops.unpack8(ops.pack8(want_x))
+    y = T.conv(x, w, None, ops.CONV_S2, checkpoint="8bit")
+    gy = torch.randn(y.shape, generator=g).to(dev)
+    # (the norm's own backward pass, which would refuse what was written to, is not part of this gradient)
+    assert torch.equal(torch.autograd.grad(y, w, gy)[0], T.conv_wgrad(ops.CONV_S2, want_x, gy, tuple(w.shape)))
