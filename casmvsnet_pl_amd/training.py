@@ -504,11 +504,14 @@ class _ABNTrain8(torch.autograd.Function):
         ctx.save_for_backward(buffer, w)
         ctx.kept, ctx.slope, ctx.abs_eps = kept, slope, abs_eps
         ctx.mark_non_differentiable(buffer)
+        ctx.set_materialize_grads(False)   # (else the backward pass is handed a zero-filled tensor as large as buffer in the place of its gradient)
         return y, buffer
 
     @staticmethod
     @A._once
     def backward(ctx, gy, _):
+        if gy is None:
+            return (None,) * 9
         buffer, w = ctx.saved_tensors
         gy = gy.contiguous().float()
         k = ctx.kept

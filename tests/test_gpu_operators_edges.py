@@ -49,3 +49,32 @@ def test_conv8_behind_a_layer_norm_whose_source_is_written_to(dev, written):   #
     gy = torch.randn(y.shape, generator=g).to(dev)
     # (the norm's own backward pass, which would refuse what was written to, is not part of this gradient)
     assert torch.equal(torch.autograd.grad(y, w, gy)[0], T.conv_wgrad(ops.CONV_S2, want_x, gy, tuple(w.shape)))
+
+
+def test_abn8_backward_allocates_its_gradients_only(dev):   # noqa: F811
+    """No tensor as large as what was kept is made (and filled) on the way: the peak of the backward pass is grad_x, the two vectors and the workspace."""
+    x = torch.randn(2, 8, 32, 64, 64, device=dev, requires_grad=True)
+    norm, gy = M.ABN(8).to(dev), torch.randn(2, 8, 32, 64, 64, device=dev)
+    y = T.abn_train(norm, x, checkpoint="8bit")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    torch.autograd.grad(y, (x, norm.weight, norm.bias), gy)
+    # (8.4 MB of grad_x; 4.8 MB are kept, and the allocator rounds up to 2 MB)
+    assert torch.cuda.max_memory_allocated() - before <= x.numel() * 4 + (1 << 21)
+
+
+def test_abn8_without_a_gradient_of_its_output(dev):   # noqa: F811
+    """A node behind that hands no gradient back: none arrives at the input either."""
+    class Cut(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, t):
+            return t * 1.0
+
+        @staticmethod
+        def backward(ctx, g):
+            return None
+    x = torch.randn(2, 8, 6, 10, device=dev, requires_grad=True)
+    norm = M.ABN(8).to(dev)
+    Cut.apply(T.abn_train(norm, x, checkpoint="8bit")).sum().backward()
+    assert all(t.grad is None or not t.grad.any() for t in (x, norm.weight, norm.bias))
