@@ -8,7 +8,7 @@ import casmvsnet_pl_amd as M
 from casmvsnet_pl_amd import ops
 from casmvsnet_pl_amd import training as T
 
-from test_gpu_operators import BF16, F16, F32, dev, ln_check   # noqa: F401  (dev is a fixture)
+from test_gpu_operators import BF16, F16, F32, _step, dev, ln_check   # noqa: F401  (dev is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,32 @@ def test_abn8_without_a_gradient_of_its_output(dev):   # noqa: F811
     norm = M.ABN(8).to(dev)
     Cut.apply(T.abn_train(norm, x, checkpoint="8bit")).sum().backward()
     assert all(t.grad is None or not t.grad.any() for t in (x, norm.weight, norm.bias))
+
+
+def test_abn8_graph_holds_8_bits_where_f32_holds_two_tensors(dev):   # noqa: F811
+    """What the graph alone holds, its input and output dropped by everyone else."""
+    base = torch.randn(2, 8, 32, 64, 64, device=dev, requires_grad=True)
+    norm = M.ABN(8).to(dev)
+
+    def kept(mode):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        out = T.abn_train(norm, base * 1.0, checkpoint=mode).sum()   # (neither the product with a number nor the sum keeps a tensor)
+        return torch.cuda.memory_allocated() - before, out
+    eight, _ = kept("8bit")
+    two, _ = kept("f32")
+    # (a block of the allocator's may be up to 1 MB larger than what was asked for; x and y in float32 are 16.8 MB, the 8 bits and their scales and signs 2.4)
+    assert eight <= base.numel() * 37 / 32 + (1 << 20) and two >= base.numel() * 8
+
+
+@pytest.mark.parametrize("norm_act,most", [(M.ABN, 0.5), (M.LayerNormAct, 0.75)])
+def test_training_step_with_8_bit_checkpoints_peaks_lower(dev, norm_act, most):   # noqa: F811
+    """(640x512: 0.36 of the float32 mode's peak with ABN, 0.64 with layer norm, which keeps its float32 input)"""
+    def peak(mode):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        _step(dev, norm_act, mode, "sl1", size=(256, 320))
+        return torch.cuda.max_memory_allocated() - before
+    assert peak("8bit") < most * peak("f32")
