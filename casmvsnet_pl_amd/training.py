@@ -532,7 +532,7 @@ def abn_train(norm, x, checkpoint="f32"):
     if isinstance(norm, LayerNormAct):
         x = x.contiguous().float()
         y = norm(x)
-        if checkpoint == "8bit":
+        if checkpoint == "8bit" and y.requires_grad:   # (without a graph nobody asks, y would hold x, and an inference tensor has no version)
             y._casmvs_made_by = (y._version, _NormedFrom(norm, x))
         return y
     if not getattr(norm, "affine", True) or norm.weight is None:

@@ -107,3 +107,17 @@ def test_training_step_with_8_bit_checkpoints_peaks_lower(dev, norm_act, most): 
         _step(dev, norm_act, mode, "sl1", size=(256, 320))
         return torch.cuda.max_memory_allocated() - before
     assert peak("8bit") < most * peak("f32")
+
+
+@pytest.mark.parametrize("norm_act", [M.ABN, M.LayerNormAct])
+def test_8_bit_mode_without_a_graph(dev, norm_act):   # noqa: F811
+    """Under no_grad and inference_mode there is nothing to keep: the float32 mode's results, in train mode too."""
+    net = M.CostRegNet(8, norm_act).to(dev).train()
+    x = torch.randn(1, 8, 8, 16, 24, device=dev)
+    want = T.cost_reg_net_train(net, x).detach()
+    for without in (torch.no_grad, torch.inference_mode):
+        with without():
+            assert torch.equal(T.cost_reg_net_train(net, x, "8bit"), want)
+    norm = norm_act(8).to(dev)
+    with torch.no_grad():
+        assert not hasattr(T.abn_train(norm, x, "8bit"), "_casmvs_made_by")
