@@ -487,8 +487,11 @@ class _ABNTrain8(torch.autograd.Function):
         N, C = x.shape[:2]
         n = x.numel() // (N * C)
         kept = _kept8(N, C, n)
-        # (the forward's workspace, at most 16 KB, lies behind what is kept)
-        buffer = torch.empty(kept.bytes + ops._workspace_bytes("casmvs_abn8_workspace_bytes", N, C, n), dtype=torch.uint8, device=x.device)
+        # the forward's workspace lies behind what is kept up to 16 KB (1024 channels); a larger one, 16 bytes per channel, is not kept until the backward pass
+        workspace = ops._workspace_bytes("casmvs_abn8_workspace_bytes", N, C, n)
+        behind = workspace <= 1 << 14
+        buffer = torch.empty(kept.bytes + (workspace if behind else 0), dtype=torch.uint8, device=x.device)
+        ws = None if behind else torch.empty(workspace, dtype=torch.uint8, device=x.device)
         y = torch.empty_like(x)
         w, bta = weight.contiguous().float(), beta.contiguous().float()   # (themselves, as a rule)
         track = running_mean is not None and running_var is not None
@@ -498,7 +501,7 @@ class _ABNTrain8(torch.autograd.Function):
                 raise ValueError(f"abn_train: x {tuple(x.shape)} on {device}, a parameter or running statistic is {tuple(t.shape)} {t.dtype} on {t.device}")
         base = buffer.data_ptr()
         ops._launch("casmvs_abn8_forward_f32", x, x.data_ptr(), w.data_ptr(), bta.data_ptr(), abs_eps, eps, momentum, running_mean.data_ptr() if track else None,
-                    running_var.data_ptr() if track else None, base + kept.vec, y.data_ptr(), base, base + kept.scales, base + kept.signs, base + kept.bytes, N, C, n, slope)
+                    running_var.data_ptr() if track else None, base + kept.vec, y.data_ptr(), base, base + kept.scales, base + kept.signs, base + kept.bytes if behind else ws.data_ptr(), N, C, n, slope)
         if track:   # the kernel wrote the buffers behind torch's back: bump their version counters (packed-weight caches key on them)
             torch.autograd.graph.increment_version((running_mean, running_var))
         ctx.save_for_backward(buffer, w)

@@ -121,3 +121,13 @@ def test_8_bit_mode_without_a_graph(dev, norm_act):   # noqa: F811
     norm = norm_act(8).to(dev)
     with torch.no_grad():
         assert not hasattr(T.abn_train(norm, x, "8bit"), "_casmvs_made_by")
+
+
+def test_abn8_of_many_channels_keeps_no_workspace(dev):   # noqa: F811
+    base = torch.randn(1, 8192, 8, device=dev, requires_grad=True)
+    norm = M.ABN(8192).to(dev)
+    torch.cuda.synchronize()   # (everything below 1 MB: the allocator counts what was asked for, in steps of 512 bytes)
+    before = torch.cuda.memory_allocated()
+    out = T.abn_train(norm, base * 1.0, checkpoint="8bit").sum()
+    # a block of 37 bytes and 16 bytes of vectors per channel; the forward pass's sums are another 16
+    assert torch.cuda.memory_allocated() - before <= 8192 * (37 + 16) + 4096 and out.requires_grad
