@@ -27,6 +27,7 @@ times (18 ms per step at the reference's default training configuration, 15 ms c
 """
 import ctypes
 import functools
+import threading
 import weakref
 
 import torch
@@ -184,10 +185,11 @@ class PackPlan:
 # model (pack_plan_of), so the module global neither keeps a dropped model's weights and packed images alive nor serves them to another model's step
 # (PackPlan.serves also checks ownership).  release_plan() clears it once a step's graph is consumed (train_steps does, after optimizer.step()).
 _ACTIVE_PLAN = None
+_NO_PLAN = threading.local()   # .forwards: this thread's forwards without a graph that are under way (without_graph); they pack on their own
 
 
 def _active_plan():
-    return None if _ACTIVE_PLAN is None else _ACTIVE_PLAN()
+    return None if _ACTIVE_PLAN is None or getattr(_NO_PLAN, "forwards", 0) else _ACTIVE_PLAN()
 
 
 def set_active_plan(plan):
@@ -742,14 +744,13 @@ def conv_bn_relu_3d(m, x, checkpoint="f32"):
 
 def without_graph(forward, m, x):
     """`forward` (one of the layer-by-layer forwards here) in eval mode: no graph, and no images of a training step's PackPlan - a captured hipGraph packs the weights
-    that it finds at each replay."""
-    global _ACTIVE_PLAN
-    plan, _ACTIVE_PLAN = _ACTIVE_PLAN, None
+    that it finds at each replay.  A step that another thread is in keeps its plan."""
+    _NO_PLAN.forwards = getattr(_NO_PLAN, "forwards", 0) + 1
     try:
         with torch.no_grad():
             return forward(m, x)
     finally:
-        _ACTIVE_PLAN = plan
+        _NO_PLAN.forwards -= 1
 
 
 def feature_net_train(net, x, checkpoint="f32"):

@@ -1,8 +1,13 @@
-"""The training-side operators at the edge of what their entry points allow, without a GPU: the kernels' own source on the CPU (tests/hipemu/run_kernels14.cpp)."""
+"""The training-side operators at the edge of what their entry points allow, without a GPU: the host's side, and the kernels'
+own source on the CPU (tests/hipemu/run_kernels14.cpp)."""
 import os
 import shutil
+import threading
 
 import pytest
+import torch
+
+from casmvsnet_pl_amd import training
 
 import test_hip_emulation as emulation
 
@@ -19,3 +24,34 @@ def kernels(tmp_path_factory):
 def test_layer_norm_without_an_eps(kernels):
     """A thread without a position holds zeros; with eps = 0 its 1 / sqrt(0) stays out of the weight gradient."""
     emulation._run(kernels, ["eps 0 f32 (2, 8, 65)", "eps 0 f32 (1, 3, 65)", "eps 0 bf16"], "eps0")
+
+
+def test_a_forward_without_a_graph_leaves_the_plan_of_another_thread_alone():
+    """A layer-norm model's eval forward packs on its own; the training step of another thread keeps its plan meanwhile, and what it releases stays released."""
+    def elsewhere(call):
+        out = []
+        thread = threading.Thread(target=lambda: out.append(call()))
+        thread.start()
+        thread.join()
+        return out[0]
+    plan = training.PackPlan()
+    seen = []
+
+    def forward(m, x):
+        seen.append(training._active_plan())
+        seen.append(training.without_graph(lambda m, x: training._active_plan(), m, x))   # one inside another
+        seen.append(training._active_plan())
+        seen.append(elsewhere(training._active_plan))
+        elsewhere(training.release_plan)
+        assert not torch.is_grad_enabled()
+        return x
+    try:
+        training.set_active_plan(plan)
+        assert training.without_graph(forward, None, 3) == 3
+        assert seen == [None, None, None, plan] and training._active_plan() is None
+        training.set_active_plan(plan)
+        with pytest.raises(ZeroDivisionError):
+            training.without_graph(lambda m, x: 1 // 0, None, None)
+        assert training._active_plan() is plan
+    finally:
+        training.release_plan()
