@@ -56,11 +56,11 @@ class GraphedForward:
     def refresh_weights(self):
         """After the model's parameters changed (an optimiser step, load_state_dict): re-pack the folded weight images IN
         PLACE, so that the next replay - which reads them through the pointers captured in the graph - sees the new
-        weights.  No re-capture."""
+        weights.  No re-capture.  (A layer-norm model has no folded images: its captured forward packs the weights that each replay finds.)"""
         dev = self.imgs.device
-        self.model.feature.packed_layers(dev)
-        for l in range(self.model.levels):
-            getattr(self.model, f"cost_reg_{l}").packed_layers(dev)
+        for net in [self.model.feature] + [getattr(self.model, f"cost_reg_{l}") for l in range(self.model.levels)]:
+            if getattr(net, "foldable", True):
+                net.packed_layers(dev)
 
     def __call__(self, imgs=None, proj_mats=None, init_depth_min=None, depth_interval=None):
         if imgs is not None and imgs.data_ptr() != self.imgs.data_ptr():

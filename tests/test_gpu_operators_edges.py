@@ -131,3 +131,24 @@ def test_abn8_of_many_channels_keeps_no_workspace(dev):   # noqa: F811
     out = T.abn_train(norm, base * 1.0, checkpoint="8bit").sum()
     # a block of 37 bytes and 16 bytes of vectors per channel; the forward pass's sums are another 16
     assert torch.cuda.memory_allocated() - before <= 8192 * (37 + 16) + 4096 and out.requires_grad
+
+
+def test_layer_norm_model_refreshes_a_captured_forward(dev):   # noqa: F811
+    """GraphedForward.refresh_weights after a weight update: nothing is folded ahead of a layer-norm model's replay, so there is nothing to pack again."""
+    from casmvsnet_pl_amd.graph import ConcurrentForwards, GraphedForward
+    from casmvsnet_pl_amd.synthetic import make_inputs, randomize_state_dict
+    model = M.CascadeMVSNet(num_groups=1, norm_act=M.LayerNormAct)
+    randomize_state_dict(model.state_dict(), seed=2)
+    model = model.to(dev).eval()
+    imgs, proj, dmin, dint = make_inputs(1, 3, 64, 96, seed=5)
+    imgs, proj = imgs.to(dev), proj.to(dev)
+    graphed, two = GraphedForward(model, imgs, proj, dmin, dint), ConcurrentForwards(model, imgs, proj, dmin, dint)
+    with torch.no_grad():
+        for p in model.parameters():
+            p.mul_(1.01)
+    graphed.refresh_weights()
+    two.refresh_weights()
+    want = {k: v.clone() for k, v in model(imgs, proj, dmin, dint).items()}
+    for got in (graphed(imgs, proj), *two.run([(imgs, proj)] * 2)):
+        torch.cuda.synchronize()
+        assert all(torch.equal(got[k], want[k]) for k in want)
