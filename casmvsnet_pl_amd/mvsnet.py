@@ -39,6 +39,18 @@ def _fold_norm(owner, norm):
     return scale, shift, slope
 
 
+def _foldable(owner, norms):
+    """Whether eval mode runs the fused engine, by the layers' norms in their order.  A layer-norm model runs layer by layer, where an ABN takes batch statistics:
+    refused (and a layer norm behind an ABN by _fold_norm), so that eval mode never does."""
+    norms = iter(norms)
+    if not isinstance(next(norms), LayerNormAct):
+        return True
+    other = next((n for n in norms if not isinstance(n, LayerNormAct)), None)
+    if other is not None:
+        raise RuntimeError(f"{owner}: eval mode of a model with both LayerNormAct and {type(other).__name__} layers is not supported")
+    return False
+
+
 def compose_fpn_tail(lat_weight, lat_bias, smooth_weight, smooth_bias):
     """The FPN tail smooth(lat(x) + up(y)) (mvsnet.py:36-38,50-51,54) as ONE 3x3 convolution over [x | up(y)]: nothing
     non-linear sits between the 1x1 lateral conv, the sum and the 3x3 smoothing conv.  Returns
@@ -167,7 +179,7 @@ class FeatureNet(_PackedWeights, nn.Module):
     @property
     def foldable(self):
         """Whether eval mode runs the fused engine: the norm folds into the convolutions (ABN does, layer norm does not)."""
-        return not isinstance(getattr(self.conv0[0], "bn", None), LayerNormAct)
+        return _foldable("FeatureNet", (getattr(m, "bn", None) for seq in (self.conv0, self.conv1, self.conv2) for m in seq))
 
     def packed_layers(self, device):
         """Folded + packed parameter images on `device` (re-packed whenever a tensor changed)."""
@@ -306,7 +318,7 @@ class CostRegNet(_PackedWeights, nn.Module):
     @property
     def foldable(self):
         """Whether eval mode runs the fused engine: the norm folds into the convolutions (ABN does, layer norm does not)."""
-        return not isinstance(getattr(self.conv0, "bn", None), LayerNormAct)
+        return _foldable("CostRegNet", (getattr(m, "bn", None) if isinstance(m, ConvBnReLU3D) else m[1] for m in (getattr(self, n) for n, _ in self._LAYERS[:-1])))
 
     # -- weight folding / packing -------------------------------------------------------------
     def _layer_tensors(self, name):

@@ -152,3 +152,13 @@ def test_layer_norm_model_refreshes_a_captured_forward(dev):   # noqa: F811
     for got in (graphed(imgs, proj), *two.run([(imgs, proj)] * 2)):
         torch.cuda.synchronize()
         assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+def test_norms_of_both_kinds_train_and_are_refused_in_eval_mode(dev):   # noqa: F811
+    net = M.CostRegNet(8, lambda c: M.LayerNormAct(c) if c == 8 else M.ABN(c)).to(dev).train()
+    x = torch.randn(1, 8, 8, 16, 24, device=dev)
+    assert bool(torch.isfinite(net(x)).all())
+    before = {k: v.clone() for k, v in net.state_dict().items()}
+    with pytest.raises(RuntimeError, match="both"):
+        net.eval()(x)
+    assert all(torch.equal(v, before[k]) for k, v in net.state_dict().items())

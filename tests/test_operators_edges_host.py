@@ -7,6 +7,7 @@ import threading
 import pytest
 import torch
 
+import casmvsnet_pl_amd as M
 from casmvsnet_pl_amd import training
 
 import test_hip_emulation as emulation
@@ -55,3 +56,15 @@ def test_a_forward_without_a_graph_leaves_the_plan_of_another_thread_alone():
         assert training._active_plan() is plan
     finally:
         training.release_plan()
+
+
+@pytest.mark.parametrize("first", [0, 1])
+def test_a_model_with_both_kinds_of_norm_is_refused_in_eval_mode(first):
+    """Layer by layer an ABN would take batch statistics (and change its running ones); folded, a layer norm has nothing to fold."""
+    kinds = (M.LayerNormAct, M.ABN) if first == 0 else (M.ABN, M.LayerNormAct)
+    for net in (M.FeatureNet(lambda c: kinds[c != 8](c)), M.CostRegNet(8, lambda c: kinds[c != 8](c))):
+        with pytest.raises(RuntimeError, match="both|no running statistics"):
+            assert net.foldable
+            net.packed_layers("cpu")
+    for norm in (M.ABN, M.InPlaceABN, M.LayerNormAct):
+        assert M.FeatureNet(norm).foldable == M.CostRegNet(8, norm).foldable == (norm is not M.LayerNormAct)
