@@ -6,7 +6,8 @@
 //
 // xhat enters the gradient through ggamma and its product with Q only (both averages over the channel), so its 8 bits cost little there; the side of zero
 // multiplies every gradient element, so it is kept exactly.  The statistics, xhat and z are computed in 64 bits: a block's codes and the sign of z are the
-// ones of the definition, not of one order of float32 roundings.  y itself is the float32 fma of casmvs_abn_train_apply_f32.
+// ones of the definition, not of one order of float32 roundings.  y is formed in float32 from x - mean, with the mean as two floats, on the side of zero that z is
+// on: at most four half steps of gamma xhat, wherever the channel lies, and both passes on the same side of the activation.
 //
 // Everything here waits for memory: forward 4 + 4 + 33/32 + 1/8 bytes read and written per element and 4 for the sums, backward sums 4 + 37/32, apply
 // 8 + 37/32 (keeping x and y in float32 reads 12 and 12 and writes 4).  Measured, both launches of a pass together, forward / backward:
@@ -178,53 +179,68 @@ __device__ __forceinline__ void channel_totals(const double *__restrict__ sums, 
   }
 }
 
-// A workgroup's share [lo, hi) of a channel's planes, in words of four values, added to the sums of x and x^2: in 64 bits from the first addition on (x^2 is exact
-// there), because xhat's codes and the side of zero hang on the mean.
+// The channel's sums are of x - x0, x0 its first element: mean = x0 + s0 / M, var = s1 / M - (s0 / M)^2.  One element's distance to the mean squared is at most
+// M var, whichever element it is, so the difference keeps var to M * 2^-53 however far from zero the channel lies (sums of x itself lose mean^2 / var * 2^-53 of it:
+// 1e-3 at a mean of 3e6 and a spread of 1), and x0 is as a rule a few spreads from the mean: then all but var's last digits are right.
+__device__ __forceinline__ float origin(const float *__restrict__ x, int c, size_t n) {
+  const float x0 = x[c * n];
+  return fabsf(x0) < INFINITY ? x0 : 0.0f;
+}
+
+// A workgroup's share [lo, hi) of a channel's planes, in words of four values, added to the sums of x - x0 and its square: in 64 bits from the first addition on,
+// because xhat's codes and the side of zero hang on the mean.
 template <bool WIDE, int THREADS>
-__device__ __forceinline__ void add_squares(const float *__restrict__ x, int N, int C, int c, size_t n, size_t lo, size_t hi, double &s0, double &s1) {
+__device__ __forceinline__ void add_squares(const float *__restrict__ x, float x0, int N, int C, int c, size_t n, size_t lo, size_t hi, double &s0, double &s1) {
   for (int img = 0; img < N; ++img) {
     const float *xp = x + ((size_t)img * C + c) * n;
     for (size_t e = lo + threadIdx.x; e < hi; e += 4 * THREADS) {
       float v[4][4];
+      int left[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {   // four loads in flight
+      for (int k = 0; k < 4; ++k) {   // four loads in flight, none of which waits for x0
         const size_t at = e + (size_t)k * THREADS;
-        load4<float, WIDE>(xp + 4 * at, at < hi ? left_of(n, 4 * at) : 0, v[k]);
+        left[k] = at < hi ? left_of(n, 4 * at) : 0;
+        load4<float, WIDE>(xp + 4 * at, left[k], v[k]);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 4; ++k) {
+        if (left[k] == 0) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const double d = v[k][i];
+          const double d = (double)(WIDE || i < left[k] ? v[k][i] : x0) - (double)x0;
           s0 += d;
           s1 = fma(d, d, s1);
         }
+      }
     }
   }
 }
 
 struct Channel {   // what the apply pass needs of a channel
   double mean, rstd;
-  float gamma, beta, scale, shift;
+  float high, low;   // of the mean
+  float gamma, beta, scale;
 };
 struct Norm {      // arguments of either form of the forward pass
   const float *weight, *bias;
   float abs_eps, eps, momentum, slope;
   float *rmean, *rvar, *vec;   // vec (4, C): scale = gamma rstd, shift, gamma, beta of the forward pass
 };
-__device__ __forceinline__ Channel finish(const Norm &p, double s0, double s1, double M, int c, int C, bool write) {
+__device__ __forceinline__ Channel finish(const Norm &p, float x0, double s0, double s1, double M, int c, int C, bool write) {
   Channel k;
-  k.mean = s0 / M;
-  double var = s1 / M - k.mean * k.mean;   // biased
+  const double off = s0 / M;
+  k.mean = (double)x0 + off;
+  double var = s1 / M - off * off;   // biased
   var = var > 0.0 ? var : (var != var ? var : 0.0);
   k.rstd = 1.0 / sqrt(var + (double)p.eps);
   k.gamma = p.abs_eps >= 0.0f ? fabsf(p.weight[c]) + p.abs_eps : p.weight[c];
   k.beta = p.bias[c];
   k.scale = (float)((double)k.gamma * k.rstd);
-  k.shift = (float)((double)k.beta - k.mean * (double)k.gamma * k.rstd);
+  k.high = (float)k.mean;
+  k.low = (float)(k.mean - (double)k.high);
   if (write) {
     p.vec[c] = k.scale;
-    p.vec[C + c] = k.shift;
+    p.vec[C + c] = (float)((double)k.beta - k.mean * (double)k.gamma * k.rstd);
     p.vec[2 * C + c] = k.gamma;
     p.vec[3 * C + c] = k.beta;
     if (p.rmean) {   // F.batch_norm: running = (1 - momentum) * running + momentum * batch (running_var: unbiased)
@@ -261,9 +277,11 @@ __device__ __forceinline__ void apply_blocks(const float *__restrict__ xp, float
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       h[i] = i < left ? ((double)v[k][i] - c.mean) * c.rstd : 0.0;
-      up |= (fma(h[i], (double)c.gamma, (double)c.beta) > 0.0 ? 1u : 0u) << i;
-      const float t = fmaf(v[k][i], c.scale, c.shift);
-      o[i] = t > 0.0f ? t : t * slope;
+      const bool above = fma(h[i], (double)c.gamma, (double)c.beta) > 0.0;
+      up |= (above ? 1u : 0u) << i;
+      // (z rounded from 64 bits instead: 60.2 -> 62.9 us at 2 x 8 x 32 x 256 x 320, 7.7 -> 8.6 at 2 x 32 x 30720)
+      const float t = fmaf((v[k][i] - c.high) - c.low, c.scale, c.beta);
+      o[i] = above ? t : t * slope;
     }
     unsigned scale;
     const unsigned q = casmvs::block8::quantise(h, scale);
@@ -286,7 +304,7 @@ __global__ __launch_bounds__(kSumThreads) void abn8_sums_kernel(const float *__r
   const int c = blockIdx.y;
   const size_t words = (n + 3) / 4, per = (words + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < words ? lo + per : words;
   double s0 = 0.0, s1 = 0.0;
-  add_squares<WIDE, kSumThreads>(x, N, C, c, n, lo, hi, s0, s1);
+  add_squares<WIDE, kSumThreads>(x, origin(x, c, n), N, C, c, n, lo, hi, s0, s1);
   workgroup_sums<kSumThreads>(s0, s1);
   if (threadIdx.x == 0) {
     out[((size_t)c * gridDim.x + blockIdx.x) * 2] = s0;
@@ -302,9 +320,10 @@ __global__ __launch_bounds__(kThreads) void abn8_apply_kernel(const float *__res
                                                              float *__restrict__ y, Store to, int C, size_t n, size_t nb, unsigned chunks) {
   const unsigned plane = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
   const int c = (int)(plane % C);
+  const float x0 = origin(x, c, n);   // (ahead of the totals' exchanges, which wait for whatever scalar load is under way)
   double s0, s1;
   channel_totals(sums, parts, c, s0, s1);
-  const Channel k = finish(norm, s0, s1, M, c, C, chunk == 0 && plane == (unsigned)c && threadIdx.x == 0);
+  const Channel k = finish(norm, x0, s0, s1, M, c, C, chunk == 0 && plane == (unsigned)c && threadIdx.x == 0);
   for (int turn = 0; turn < kTurns; turn += kAhead)
     apply_blocks<WIDE, PAST>(x + plane * n, y + plane * n, to, plane * nb, ((size_t)chunk * kTurns + turn) * kGroups + threadIdx.x / kLanes, kGroups, n, nb,
                        threadIdx.x & (kLanes - 1), k, norm.slope);
@@ -318,9 +337,10 @@ __global__ __launch_bounds__(kWide) void abn8_forward_one_kernel(const float *__
   constexpr int groups = kWide / kLanes;
   const int c = blockIdx.x;
   double s0 = 0.0, s1 = 0.0;
-  add_squares<WIDE, kWide>(x, N, C, c, n, 0, (n + 3) / 4, s0, s1);
+  const float x0 = origin(x, c, n);
+  add_squares<WIDE, kWide>(x, x0, N, C, c, n, 0, (n + 3) / 4, s0, s1);
   workgroup_sums<kWide>(s0, s1);
-  const Channel k = finish(norm, s0, s1, M, c, C, threadIdx.x == 0);
+  const Channel k = finish(norm, x0, s0, s1, M, c, C, threadIdx.x == 0);
   for (int img = 0; img < N; ++img) {
     const size_t plane = (size_t)img * C + c;
     for (size_t blk = 0; blk < nb; blk += kAhead * groups)

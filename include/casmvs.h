@@ -648,8 +648,8 @@ int casmvs_pack8(const void *x, int dtype, size_t rows, size_t n, void *codes, v
 int casmvs_unpack8(const void *codes, const void *scales, const float *weight, const float *bias, int C, float slope, void *out, int dtype, size_t rows,
                    size_t n, void *stream);
 
-/* Train-mode ABN (batch statistics, running statistics, leaky ReLU: casmvs_channel_sums_f64 + casmvs_abn_train_apply_f32, the sums in 64 bits from the first
- * addition on) that keeps for its backward pass the 8-bit checkpoint of xhat = (x - mean) rstd over the planes (N C, n) - codes, scales - and signs
+/* Train-mode ABN (batch statistics, running statistics, leaky ReLU: casmvs_channel_sums_f64 + casmvs_abn_train_apply_f32, but with sums, xhat and the side of
+ * zero in 64 bits, the sums about the channel's first element, and y formed from x - mean: a channel far from zero keeps its digits) that keeps for its backward pass the 8-bit checkpoint of xhat = (x - mean) rstd over the planes (N C, n) - codes, scales - and signs
  * (N C, nb) 32-bit words: bit i of a word = [z > 0] of the block's value i.  vec (4, C): scale = gamma rstd, shift, gamma (|weight| + abs_eps where
  * abs_eps >= 0), bias as the forward pass used them; act(gamma * unpacked + bias) is y up to the rounding of the 8 bits.
  * Backward: grad_weight, grad_bias, and grad_x (may be NULL).  workspace: casmvs_abn8_workspace_bytes, for either call on its own.  N * C <= 2^21,

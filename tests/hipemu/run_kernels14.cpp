@@ -17,6 +17,9 @@ inline int hipemu_bpermute(int from, int v) { return hipemu_lane_exchange(v, (fr
 namespace ln {
 #include "layer_norm.hip"
 }
+namespace c8 {
+#include "checkpoint8.hip"
+}
 
 template <class T>
 static double value(T v) { return (double)(float)v; }
@@ -81,6 +84,65 @@ static void no_eps_check(const char *name, int dtype, double half_step, size_t o
   take(what, e, 1.05);
 }
 
+// ABN with 8-bit checkpoints where the channels' means are many times their spread, where the first element of a channel is far from all others, and where all of
+// them are equal: y, the signs, vec and the running statistics are those of 64 bits.
+enum Channels { kShifted, kFirstApart, kConstant };
+static void far_check(int N, int C, size_t n, float offset, Channels kind) {
+  const size_t numel = (size_t)N * C * n, nb = (n + 31) / 32, planes = (size_t)N * C;
+  const double M = (double)N * n;
+  std::vector<float> x(numel), y(numel), w(C), b(C), rm(C, 0.5f), rv(C, 2.0f), vec(4 * C);
+  std::vector<unsigned char> codes(planes * nb * 32), scales(planes * nb);
+  std::vector<unsigned> signs(planes * nb);
+  std::vector<char> ws(casmvs_abn8_workspace_bytes(N, C, n));
+  const float slope = 0.01f;
+  for (size_t i = 0; i < numel; ++i)
+    x[i] = kind == kConstant ? offset : kind == kFirstApart ? (i % n == 0 && i / n < (size_t)C ? offset : rnd()) : 2.0f * rnd() + offset;
+  for (int c = 0; c < C; ++c) { w[c] = (c & 1 ? -1.0f : 1.0f) * (0.9f + 0.4f * rnd()); b[c] = 0.3f * rnd(); }
+  if (casmvs_abn8_forward_f32(x.data(), w.data(), b.data(), -1.0f, 1e-5f, 0.1f, rm.data(), rv.data(), vec.data(), y.data(), codes.data(), scales.data(), signs.data(),
+                              ws.data(), N, C, n, slope, nullptr)) {
+    printf("abn8: %s\n", casmvs_last_error());
+    g_worst = 1e9;
+  }
+  double e = 0;
+  size_t wrong = 0;
+  auto worse = [&](double off, double limit) { e = std::isfinite(off) ? std::fmax(e, off / limit) : 1e9; };
+  for (int c = 0; c < C; ++c) {
+    // two passes over x - x0: a distance from the first element is exact, its sum as good as M values of that size allow
+    double s = 0, var = 0;
+    for (int img = 0; img < N; ++img)
+      for (size_t i = 0; i < n; ++i) s += ((double)x[((size_t)img * C + c) * n + i] - x[c * n]) / M;
+    const double mean = x[c * n] + s;
+    for (int img = 0; img < N; ++img)
+      for (size_t i = 0; i < n; ++i) {
+        const double d = ((double)x[((size_t)img * C + c) * n + i] - x[c * n]) - s;
+        var += d * d / M;
+      }
+    const double r = 1.0 / std::sqrt(var + 1e-5f);
+    // one-pass sums: M 2^-53 of var where the first element is all there is, and as much again for the additions
+    const double rel = 4 * M * 0x1p-53 + 1e-13, mean_off = 8 * 0x1p-53 * std::fabs(mean) + 1e-13 * std::fabs(s);
+    for (int img = 0; img < N; ++img)
+      for (size_t i = 0; i < n; ++i) {
+        const size_t plane = (size_t)img * C + c, at = plane * n + i;
+        const double h = ((double)x[at] - mean) * r, z = h * w[c] + b[c], want = z > 0 ? z : z * slope;
+        const double z_off = mean_off * r * std::fabs(w[c]) + rel * std::fabs(h * w[c]);
+        // y in float32: x - mean's two differences, scale and the product half a step each of |h w|, the sum and the slope of |z|; the mean as two floats
+        const double y_off = 0x1p-24 * 1.001 * (4 * std::fabs(h * w[c]) + 2 * std::fabs(z)) + 0x1p-47 * std::fabs(mean) * r * std::fabs(w[c]) + z_off;
+        worse(std::fabs(y[at] - want), (z > 0 ? 1.0 : slope) * y_off + 1e-30);
+        const bool up = signs[plane * nb + i / 32] >> (i % 32) & 1;
+        wrong += std::fabs(z) > z_off && up != (z > 0);
+        // ... on the side of the activation that the backward pass takes
+        const double side = up ? z : z * slope;
+        worse(std::fabs(y[at] - side), (up ? 1.0 : slope) * y_off + 1e-30);
+      }
+    worse(std::fabs(vec[c] - w[c] * r), 0x1p-24 * 1.001 * std::fabs(w[c] * r) + rel * std::fabs(w[c] * r));
+    worse(std::fabs(rm[c] - (0.45 + 0.1 * mean)), 4 * 0x1p-24 * (0.45 + 0.1 * std::fabs(mean)));
+    worse(std::fabs(rv[c] - (1.8 + 0.1 * var * M / (M - 1))), 4 * 0x1p-24 * (1.8 + 0.1 * var) + rel * var);
+  }
+  char what[120];
+  snprintf(what, sizeof(what), "abn8 %s (%d, %d, %zu) at %g: %zu signs wrong", kind == kConstant ? "constant" : kind == kFirstApart ? "first apart" : "shifted", N, C, n, offset, wrong);
+  take(what, wrong ? 1e9 : e, 1.0);
+}
+
 int main(int argc, char **argv) {
   hipemu::g_lds = smem_raw;
   const std::string part = argc > 1 ? argv[1] : "";
@@ -104,6 +166,17 @@ int main(int argc, char **argv) {
     no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 5, 20, 1);     // rows
     no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 3, 5, 1);
     no_eps_check<float>("f32", CASMVS_DTYPE_F32, 0x1p-24, 2, 300, 1);
+  } else if (part == "far") {
+    for (float offset : {0.0f, 1e4f, -3e6f}) {
+      far_check(2, 3, 70, offset, kShifted);
+      far_check(2, 2, 64, offset, kShifted);
+    }
+    far_check(1, 2, 16500, 3e6f, kShifted);   // (two launches)
+    far_check(1, 1, 16501, -1e5f, kShifted);
+    for (Channels kind : {kFirstApart, kConstant}) {
+      far_check(2, 3, 70, 1e6f, kind);
+      far_check(1, 2, 16500, 1e4f, kind);
+    }
   } else {
     printf("no part named %s\n", part.c_str());
     return 2;

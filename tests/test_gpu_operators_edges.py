@@ -1,6 +1,8 @@
-"""GPU tests of the training-side operators at the edge of what their entry points allow: layer norm without an eps, what is kept
-across writes, under other grad modes and in memory.  Definitions, bounds and fixtures are
+"""GPU tests of the training-side operators at the edge of what their entry points allow: layer norm without an eps,
+8-bit ABN far from zero, what is kept across writes, under other grad modes and in memory, captured forwards, mixed norms.  Definitions, bounds and fixtures are
 test_gpu_operators.py's."""
+import math
+
 import pytest
 import torch
 
@@ -8,7 +10,7 @@ import casmvsnet_pl_amd as M
 from casmvsnet_pl_amd import ops
 from casmvsnet_pl_amd import training as T
 
-from test_gpu_operators import BF16, F16, F32, _step, dev, ln_check   # noqa: F401  (dev is a fixture)
+from test_gpu_operators import BF16, F16, F32, U, _step, abn8_reference, dev, ln_check, rounding, within   # noqa: F401  (dev is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -162,3 +164,56 @@ def test_norms_of_both_kinds_train_and_are_refused_in_eval_mode(dev):   # noqa: 
     with pytest.raises(RuntimeError, match="both"):
         net.eval()(x)
     assert all(torch.equal(v, before[k]) for k, v in net.state_dict().items())
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 70), (2, 8, 4, 16, 20), (1, 2, 8192 + 64), (3, 4, 40001)])
+@pytest.mark.parametrize("offset", [0.0, 1e4, -3e6])
+def test_abn8_far_from_zero(dev, shape, offset):   # noqa: F811
+    """Channels whose mean is many times their spread: y, the side of zero and the gradients as at zero; constant channels are their bias."""
+    g = torch.Generator().manual_seed(sum(shape))
+    C, count = shape[1], math.prod(shape) // shape[1]
+    norm = M.ABN(C).to(dev)
+    x, gy = torch.randn(shape, generator=g) * 1.5 + offset, torch.randn(shape, generator=g)
+    w, b = torch.randn(C, generator=g) * 0.6, torch.randn(C, generator=g) * 0.3
+    with torch.no_grad():
+        norm.weight.copy_(w)
+        norm.bias.copy_(b)
+    y, gx, gw, gb, terms, aw, ab, mean, unbiased = abn8_reference(x, w, b, gy, 0.01, 1e-5, False)
+    xd = x.to(dev).requires_grad_()
+    got = T.abn_train(norm, xd, checkpoint="8bit")
+    # z in 64 bits: the mean is off by a rounding of its own size (8 of them: the reference's too), the variance by less than count of them.  y in float32 from x - mean,
+    # the mean as two floats: both differences, the scale and the product half a step each of |h w|, the sum and the slope of |z|
+    r = (1 / torch.sqrt(unbiased * (count - 1) / count + 1e-5)).view(1, C, 1)
+    far = mean.abs().view(1, C, 1) * r * w.double().abs().view(1, C, 1)
+    z = torch.where(y > 0, y, y / float(torch.tensor(0.01)))
+    hw = (z - b.double().view(1, C, 1)).abs()
+    z_off = 2.0 ** -53 * (8 * far + 4 * count * hw) + 1e-12 * (hw + 1)
+    within(got.reshape(y.shape), y, torch.where(y > 0, 1.0, 0.01) * (U * 1.001 * (4 * hw + 2 * z.abs()) + 2 * U * U * far + z_off))
+    got.backward(gy.to(dev))
+    within(xd.grad.reshape(gx.shape), gx, rounding(gx, F32) + 16 * U * terms)
+    within(norm.weight.grad, gw, 64 * U * aw + rounding(gw, F32))
+    within(norm.bias.grad, gb, 64 * U * ab + rounding(gb, F32))
+    within(norm.running_mean, 0.1 * mean, 4 * U * 0.1 * mean.abs() + 1e-12)
+    within(norm.running_var, 0.9 + 0.1 * unbiased, 4 * U * (0.9 + 0.1 * unbiased))
+    flat = T.abn_train(norm, torch.full(shape, offset, device=dev, requires_grad=True), checkpoint="8bit")
+    assert torch.equal(flat, torch.where(norm.bias > 0, norm.bias, norm.bias * 0.01).view(1, C, *[1] * (len(shape) - 2)).expand(shape))
+
+
+@pytest.mark.parametrize("first", [float("nan"), float("inf"), 1e6])
+def test_abn8_whatever_the_first_element_is(dev, first):   # noqa: F811
+    """A channel's sums are taken about its first element: far from all others it costs no digits, not finite it makes the channel NaN and no other."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(2, 4, 9, 21, generator=g)
+    x[0, 2, 0, 0] = first
+    norm = M.ABN(4).to(dev)
+    xd = x.to(dev).requires_grad_()
+    y = T.abn_train(norm, xd, checkpoint="8bit")
+    y.backward(torch.ones_like(y))
+    if abs(first) < float("inf"):
+        want, _, _, _, _, _, _, mean, unbiased = abn8_reference(x, torch.ones(4), torch.zeros(4), torch.ones_like(x), 0.01, 1e-5, False)
+        within(y.reshape(want.shape), want, 6 * U * want.abs() * 1.001 + 2 * U * U * mean.abs().view(1, 4, 1) + 1e-10)   # (as above, without a bias)
+        within(norm.running_var, 0.9 + 0.1 * unbiased, 4 * U * (0.9 + 0.1 * unbiased))
+    else:
+        assert bool(torch.isnan(y[:, 2]).all()) and bool(torch.isnan(xd.grad[:, 2]).all())
+        others = [0, 1, 3]
+        assert bool(torch.isfinite(y[:, others]).all()) and bool(torch.isfinite(xd.grad[:, others]).all())

@@ -68,3 +68,9 @@ def test_a_model_with_both_kinds_of_norm_is_refused_in_eval_mode(first):
             net.packed_layers("cpu")
     for norm in (M.ABN, M.InPlaceABN, M.LayerNormAct):
         assert M.FeatureNet(norm).foldable == M.CostRegNet(8, norm).foldable == (norm is not M.LayerNormAct)
+
+
+@needs_clang
+def test_abn8_far_from_zero(kernels):
+    """Channels whose mean is many times their spread, whose first element is far from the others, constant ones."""
+    emulation._run(kernels, ["abn8 shifted (2, 3, 70) at -3e+06", "abn8 first apart", "abn8 constant"], "far")
