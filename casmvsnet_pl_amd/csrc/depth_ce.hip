@@ -32,13 +32,14 @@ __device__ __forceinline__ float exp_below(float a, float m) { return __builtin_
 // Is depth `a` nearer to `gt` than `b`, whose rounded distances are equal?
 __device__ __forceinline__ bool nearer(float a, float b, float gt) { return __builtin_fabs((double)a - (double)gt) < __builtin_fabs((double)b - (double)gt); }
 
-// o: the hypotheses behind r's; dp, dstep: the pixel's depths
+// o: the hypotheses behind r's; dp, dstep: the pixel's depths.  A piece without a finite distance has no nearest one to compare: a pixel between its lowest and highest
+// hypothesis is less than float32's largest number away from one of the two.
 __device__ __forceinline__ void join(Running &r, const Running &o, const float *__restrict__ dp, size_t dstep, float gt) {
   const float m = fmaxf(r.m, o.m);
   r.s = r.s * exp_below(r.m, m) + o.s * exp_below(o.m, m);
   r.m = m;
   bool take = o.near < r.near;
-  if (o.near == r.near) take = nearer(dp[o.at * dstep], dp[r.at * dstep], gt);
+  if (o.near == r.near && o.near < INFINITY) take = nearer(dp[o.at * dstep], dp[r.at * dstep], gt);
   r.at = take ? o.at : r.at;
   r.near = fminf(r.near, o.near);
   r.low = fminf(r.low, o.low);
@@ -114,7 +115,8 @@ __global__ __launch_bounds__(kThreads) void depth_ce_forward_kernel(const T *__r
     __syncthreads();
   }
   if (piece == 0) {
-    for (int q = 1; q < PIECES; ++q) join(r, joined[q * kPixels + lane], dp, dstep, true_depth);
+    if (live)
+      for (int q = 1; q < PIECES; ++q) join(r, joined[q * kPixels + lane], dp, dstep, true_depth);
     bool counted = false;
     float cost_at = 0.0f;
     if (live) {

@@ -20,6 +20,10 @@ namespace ln {
 namespace c8 {
 #include "checkpoint8.hip"
 }
+namespace ce {
+#include "depth_ce.hip"
+}
+#include <sys/mman.h>
 
 template <class T>
 static double value(T v) { return (double)(float)v; }
@@ -143,6 +147,53 @@ static void far_check(int N, int C, size_t n, float offset, Channels kind) {
   take(what, wrong ? 1e9 : e, 1.0);
 }
 
+// Cross entropy where every pixel is masked: costs, hypotheses and ground truth lie in memory that must not be read (a read ends the process).
+static void masked_check(int B, int D, size_t hw, bool per_pixel) {
+  const size_t pixels = B * hw, numel = pixels * D;
+  void *apart = mmap(nullptr, numel * 4, PROT_NONE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
+  std::vector<float> stats(2 * pixels, -1.0f), grad(numel, -1.0f);
+  std::vector<int> target(pixels, 7);
+  std::vector<unsigned char> mask(pixels, 0);
+  std::vector<char> ws(casmvs_depth_ce_workspace_bytes(B, D, hw));
+  float loss = -1, share = -1, up = 1;
+  printf("depth_ce masked (%d, %d, %zu)%s\n", B, D, hw, per_pixel ? " per pixel" : "");
+  fflush(stdout);
+  if (apart == MAP_FAILED ||
+      casmvs_depth_ce_forward(apart, (const float *)apart, (const float *)apart, mask.data(), stats.data(), target.data(), &loss, &share, ws.data(), CASMVS_DTYPE_F32, B, D, hw,
+                              per_pixel, nullptr) ||
+      casmvs_depth_ce_backward(apart, stats.data(), target.data(), &share, &up, grad.data(), CASMVS_DTYPE_F32, B, D, hw, nullptr))
+    g_worst = 1e9;
+  if (loss != 0.0f || share != 0.0f) g_worst = 1e9;
+  for (int t : target)
+    if (t != -1) g_worst = 1e9;
+  for (float q : grad)
+    if (q != 0.0f) g_worst = 1e9;
+  munmap(apart, numel * 4);
+}
+
+// ... and where a piece of the axis has no hypotheses, or only ones whose distance is beyond float32: the nearest one is still the class
+static void pieces_check(int D, size_t hw, float scale) {
+  std::vector<float> cost(D * hw), depth(D), gt(hw), stats(2 * hw);
+  std::vector<int> target(hw);
+  std::vector<char> ws(casmvs_depth_ce_workspace_bytes(1, D, hw));
+  float loss = -1, share = -1;
+  for (float &c : cost) c = rnd();
+  for (int k = 0; k < D; ++k) depth[k] = scale * (2.0f * k / (D - 1) - 1.0f);   // from -scale to scale
+  for (size_t s = 0; s < hw; ++s) gt[s] = scale * rnd();
+  if (casmvs_depth_ce_forward(cost.data(), depth.data(), gt.data(), nullptr, stats.data(), target.data(), &loss, &share, ws.data(), CASMVS_DTYPE_F32, 1, D, hw, 0, nullptr))
+    g_worst = 1e9;
+  size_t wrong = 0;
+  for (size_t s = 0; s < hw; ++s) {
+    int near = 0;
+    for (int k = 1; k < D; ++k)
+      if (std::fabs((double)depth[k] - gt[s]) < std::fabs((double)depth[near] - gt[s])) near = k;
+    wrong += target[s] != near;
+  }
+  char what[120];
+  snprintf(what, sizeof(what), "depth_ce pieces (%d, %zu) to %g: %zu targets wrong", D, hw, scale, wrong);
+  take(what, (double)wrong, 0.5);
+}
+
 int main(int argc, char **argv) {
   hipemu::g_lds = smem_raw;
   const std::string part = argc > 1 ? argv[1] : "";
@@ -176,6 +227,16 @@ int main(int argc, char **argv) {
     for (Channels kind : {kFirstApart, kConstant}) {
       far_check(2, 3, 70, 1e6f, kind);
       far_check(1, 2, 16500, 1e4f, kind);
+    }
+  } else if (part == "masked") {
+    for (bool per_pixel : {true, false}) {
+      masked_check(2, 8, 45, per_pixel);      // one piece of the axis
+      masked_check(1, 33, 30, per_pixel);     // four, the last one shorter
+      masked_check(1, 192, 20, per_pixel);    // sixteen
+    }
+    for (float scale : {1.0f, 3e38f}) {
+      pieces_check(33, 300, scale);
+      pieces_check(65, 40, scale);            // sixteen pieces of 5: three are empty
     }
   } else {
     printf("no part named %s\n", part.c_str());

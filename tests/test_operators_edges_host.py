@@ -74,3 +74,9 @@ def test_a_model_with_both_kinds_of_norm_is_refused_in_eval_mode(first):
 def test_abn8_far_from_zero(kernels):
     """Channels whose mean is many times their spread, whose first element is far from the others, constant ones."""
     emulation._run(kernels, ["abn8 shifted (2, 3, 70) at -3e+06", "abn8 first apart", "abn8 constant"], "far")
+
+
+@needs_clang
+def test_depth_cross_entropy_reads_nothing_of_masked_pixels(kernels):
+    """Whatever the number of pieces that a pixel's axis is cut into; and a piece without a hypothesis (or a finite distance) changes no class."""
+    emulation._run(kernels, ["depth_ce masked (1, 192, 20)", "depth_ce pieces (65, 40) to 3e+38"], "masked")
