@@ -591,7 +591,8 @@ extern "C" int casmvs_abn8_backward_f32(const float *grad_y, const void *codes, 
   CASMVS_REQUIRE(grad_y && codes && scales && signs && weight && vec && grad_weight && grad_bias && workspace, "abn8_backward: null pointer");
   CASMVS_REQUIRE((((uintptr_t)codes | (uintptr_t)signs) & 3) == 0 && ((uintptr_t)workspace & 7) == 0,
                  "abn8_backward: codes and signs are 4-byte words, the workspace 8-byte ones");
-  const size_t nb = blocks_of(n), chunks = (nb + kTurns * kGroups - 1) / (kTurns * kGroups);
+  const size_t nb = blocks_of(n);
+  size_t chunks = (nb + kTurns * kGroups - 1) / (kTurns * kGroups);
   const int parts = parts_of(N, C, n);
   const double count = (double)N * (double)n;
   double *sums = (double *)workspace;
@@ -605,8 +606,9 @@ extern "C" int casmvs_abn8_backward_f32(const float *grad_y, const void *codes, 
   }
   hipLaunchKernelGGL(wide ? abn8_backward_sums_kernel<true> : abn8_backward_sums_kernel<false>, dim3((unsigned)parts, (unsigned)C), dim3(kSumThreads), 0, st, grad_y, from, sums,
                      N, C, n, nb, slope);
-  // (without grad_x the workgroups of the channels' first chunks write the two vectors, and there are no others)
-  const dim3 grid((unsigned)(grad_x ? (size_t)N * C * chunks : (size_t)C * chunks));
+  // (without grad_x one workgroup per channel, as if a plane had one chunk, writes the two vectors)
+  if (!grad_x) chunks = 1;
+  const dim3 grid((unsigned)(grad_x ? (size_t)N * C * chunks : (size_t)C));
   const bool past = wide && casmvs::elem::streams((size_t)N * C * n * sizeof(float));
   auto apply = past ? abn8_backward_apply_kernel<true, true> : wide ? abn8_backward_apply_kernel<true, false> : abn8_backward_apply_kernel<false, false>;
   hipLaunchKernelGGL(apply, grid, dim3(kThreads), 0, st, grad_y, from, sums, parts, count, to, C, n, nb,

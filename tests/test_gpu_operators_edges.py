@@ -217,3 +217,15 @@ def test_abn8_whatever_the_first_element_is(dev, first):   # noqa: F811
         assert bool(torch.isnan(y[:, 2]).all()) and bool(torch.isnan(xd.grad[:, 2]).all())
         others = [0, 1, 3]
         assert bool(torch.isfinite(y[:, others]).all()) and bool(torch.isfinite(xd.grad[:, others]).all())
+
+
+@pytest.mark.parametrize("shape", [(2, 8, 6, 10), (3, 5, 40001)])
+def test_abn8_gradients_of_the_affine_alone(dev, shape):   # noqa: F811
+    """An input that no gradient goes to: the two vectors are those of the whole backward pass."""
+    g = torch.Generator().manual_seed(4)
+    x, gy = torch.randn(shape, generator=g).to(dev), torch.randn(shape, generator=g).to(dev)
+    norm = M.InPlaceABN(shape[1]).to(dev)
+    xr = x.clone().requires_grad_()
+    _, *want = torch.autograd.grad(T.abn_train(norm, xr, checkpoint="8bit"), (xr, norm.weight, norm.bias), gy)
+    got = torch.autograd.grad(T.abn_train(norm, x, checkpoint="8bit"), (norm.weight, norm.bias), gy)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
