@@ -174,7 +174,9 @@ def load():
             "casmvsnet_pl_amd has no CPU/PyTorch fallback for the hot path.")
     lib = ctypes.CDLL(LIB_PATH)
     for name, (restype, argtypes) in SYMBOLS.items():
-        fn = getattr(lib, name)  # AttributeError if the .so does not export a declared symbol
+        fn = getattr(lib, name, None)
+        if fn is None:   # (entry points that are only added leave the ABI version as it is)
+            raise CasMVSLibraryError(f"{LIB_PATH} does not export {name}: it was built from older sources (python -m casmvsnet_pl_amd.build)")
         fn.restype = restype
         fn.argtypes = argtypes
     for name, (restype, argtypes) in TRACE_SYMBOLS.items():

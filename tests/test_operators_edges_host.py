@@ -2,13 +2,14 @@
 own source on the CPU (tests/hipemu/run_kernels14.cpp)."""
 import os
 import shutil
+import subprocess
 import threading
 
 import pytest
 import torch
 
 import casmvsnet_pl_amd as M
-from casmvsnet_pl_amd import training
+from casmvsnet_pl_amd import _lib, training
 
 import test_hip_emulation as emulation
 
@@ -80,3 +81,14 @@ def test_abn8_far_from_zero(kernels):
 def test_depth_cross_entropy_reads_nothing_of_masked_pixels(kernels):
     """Whatever the number of pieces that a pixel's axis is cut into; and a piece without a hypothesis (or a finite distance) changes no class."""
     emulation._run(kernels, ["depth_ce masked (1, 192, 20)", "depth_ce pieces (65, 40) to 3e+38"], "masked")
+
+
+def test_a_library_of_older_sources_is_named_as_such(tmp_path, monkeypatch):
+    """Same ABI version, but without an entry point that was added since."""
+    source, path = tmp_path / "old.c", tmp_path / "libold.so"
+    source.write_text("int casmvs_abi_version(void) { return %d; }\n" % _lib.ABI_VERSION)
+    subprocess.run(["gcc", "-shared", "-fPIC", str(source), "-o", str(path)], check=True)
+    monkeypatch.setattr(_lib, "LIB_PATH", str(path))
+    monkeypatch.setattr(_lib, "_lib", None)
+    with pytest.raises(_lib.CasMVSLibraryError, match="older sources"):
+        _lib.load()
