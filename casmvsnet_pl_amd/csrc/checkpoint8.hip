@@ -11,9 +11,9 @@
 //
 // Everything here waits for memory: forward 4 + 4 + 33/32 + 1/8 bytes read and written per element and 4 for the sums, backward sums 4 + 37/32, apply
 // 8 + 37/32 (keeping x and y in float32 reads 12 and 12 and writes 4).  Measured, both launches of a pass together, forward / backward:
-//   2 x 8 x 32 x 256 x 320   101 us (5.5 TB/s) / 95 us (6.3 TB/s: the second pass finds part of the first one's data in the caches)
-//   6 x 8 x 512 x 640         39 us            / 38 us                 2 x 64 x 6 x 16 x 20   8.4 us / 6.1 us (one launch each)
-// pack8 of 64 x 983040 float32 61 us, unpack8 47 us (5.2 and 6.7 TB/s); of 32 x 160 the time of a launch.
+//   2 x 8 x 32 x 256 x 320   103 us (5.4 TB/s) / 95 us (6.3 TB/s: the second pass finds part of the first one's data in the caches)
+//   6 x 8 x 512 x 640         39 us            / 38 us                 2 x 64 x 6 x 16 x 20   8.5 us / 6.8 us (one launch each)
+// pack8 of 64 x 983040 float32 61 us, unpack8 47 us (5.2 and 6.7 TB/s), bf16 53 and 36 us (3.6 and 5.3); of 32 x 160 the time of a launch.
 #include "block8.h"
 
 namespace {
@@ -142,7 +142,8 @@ __global__ __launch_bounds__(kThreads) void unpack8_kernel(const unsigned *__res
 
 // ---- train-mode ABN -------------------------------------------------------------------------------------------------------------------------------------
 // The sums over a channel are formed by kParts workgroups at most, each over its share [lo, hi) of every plane of the channel, and added up by every workgroup
-// of the pass behind: one partial sum per lane of a wave, in a fixed order.
+// of the pass behind: one partial sum per lane of a wave, in a fixed order.  Few channels leave the chip short of workgroups by it: 16 M elements in 1 / 2 / 4 / 8
+// channels take 98 / 65 / 48 / 42 us forward and 82 / 57 / 45 / 42 backward (no layer of the models has fewer than 8).
 constexpr int kParts = 64;
 
 // sums of two values per thread over a workgroup of THREADS, in every thread: lanes by exchange, then the waves' sums in their order

@@ -196,7 +196,8 @@ int check_sizes(const char *what, int dtype, int B, int D, size_t hw) {
   return CASMVS_OK;
 }
 // Pieces of the hypothesis axis: few pixels with many hypotheses would leave CUs idle, each thread walking its axis alone.  1 or 4 pieces, us: 32 hypotheses of
-// 163840 pixels 14.3 / 15.8, 48 of 40960 10.9 / 9.4, 192 of 118400 38 / 30, 256 of 20480 42 / 17.
+// 163840 pixels 14.3 / 15.8, 48 of 40960 10.9 / 9.4, 192 of 118400 38 / 30, 256 of 20480 42 / 17.  4 or 16: 192 of 2000 pixels 10.2 / 8.1, 512 of 1600 17.6 / 10.5,
+// 1024 of 80 29.4 / 12.4, 64 of 2000 7.0 / 7.1.
 int pieces_of(size_t pixels, int D) { return D < 16 || pixels >= (D <= 32 ? 65536u : 524288u) ? 1 : pixels >= 2048 || D < 64 ? 4 : 16; }
 size_t forward_blocks(size_t pixels, int D) { return (pixels * pieces_of(pixels, D) + kThreads - 1) / kThreads; }
 }  // namespace

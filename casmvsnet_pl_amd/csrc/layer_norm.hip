@@ -22,7 +22,13 @@
 //   2 x 8 x 32 x 256 x 320   60 us (5.6 TB/s) / 99 us (5.1 TB/s)      6 x 8 x 512 x 640   20 us (6.4) / 35 us (5.3)      6 x 16 x 256 x 320   11 / 25 us
 //   983040 rows of 32        45 us (5.6)      / 71 us (5.3)           8192 rows of 1024   14 us (4.9) / 27 us (3.7)
 // and in bf16: 2 x 8 x 32 x 256 x 320   40 us (4.2) / 49 us (5.1)     8191 rows of 1000   11 us (3.0) / 24 us (2.1)     65536 rows of 1024   68 us (3.9) / 93 us (4.3).
-// Small tensors cost their launches: 2 x 64 x 6 x 16 x 20 9 / 16 us.
+// Small tensors cost their launches: 2 x 64 x 6 x 16 x 20 9 / 17 us.
+// Maps of more channels, 67 MB, us forward / backward (a copy of them takes 27, the bytes of the backward pass 40):
+//   channels   64         96         128        192         256         384         512         520 (any)
+//   float32    24 / 50    25 / 56    24 / 52    58 / 142    59 / 122    62 / 120    61 / 109    134 / 296
+//   bf16       38 / 66    47 / 95    42 / 79    157 / 492   143 / 379   133 / 272   127 / 231   147 / 348
+// From 129 channels on 64 groups leave a tile 4 x V positions: a wave's loads are runs of 8 (32 bytes in float32, 16 in bf16), and below 256
+// channels more than half of what a thread could hold is missing.  In bf16 that form's backward pass is no faster than the any form's there.
 #include "elem_types.h"
 
 namespace {
@@ -881,7 +887,8 @@ void planes(const Call &a, int &parts) {
   const size_t tile = (size_t)(kThreads / CG) * V, tiles = (a.positions() + tile - 1) / tile;
   // Large outputs go past the caches (8 channels per group, pairs of positions; a branch in the kernel gains nothing): a forward pass then leaves x there for the
   // backward pass instead of y.  2 x 8 x 32 x 256 x 320 in float32, forward and the backward pass right behind it 51 + 116 -> 59 + 84 us; on their own 61 -> 60 and
-  // 104 -> 99 us (bf16 backward 53 -> 49).
+  // 104 -> 99 us (bf16 backward 53 -> 49).  In a training step other tensors lie between the two passes: of two samples at 640x512, 3 views, whose largest outputs this
+  // concerns, 17.08 ms with it and 17.14 without (medians of three).
   constexpr bool may = CH == kFull && V > 1;
   const bool past = may && casmvs::elem::streams(a.positions() * a.C * sizeof(T));
   if (!a.gy) {
@@ -913,7 +920,7 @@ void planes_by_groups(const Call &a, int &parts) {
   else if (a.C <= 2 * kHeld) planes<T, 2, V, kSome>(a, parts);
   else if (a.C <= 4 * kHeld) planes<T, 4, V, kSome>(a, parts);
   else if (a.C <= 8 * kHeld) planes<T, 8, V, kSome>(a, parts);
-  else if (a.C <= 16 * kHeld) planes<T, 16, V, kSome>(a, parts);
+  else if (a.C <= 16 * kHeld) planes<T, 16, V, kSome>(a, parts);   // (67 MB of 100 channels in float32: 26 / 55 us, in 64 groups 74 / 248; bf16 48 / 91 and 231 / 903)
   else planes<T, 64, V, kSome>(a, parts);
 }
 

@@ -3,7 +3,7 @@
 //   grad_weight[c][kz][ky][kx] = sum over (b, z, y, x) of grad_out[b][z][y][x] * in[b][c][z + kz - 1][y + ky - 1][x + kx - 1]
 //
 // The generic kernel (train.hip: conv_wgrad_kernel) puts output channels on the rows of a 16 x 16 MFMA tile: with ONE output
-// channel 15 of 16 rows are padding, and this layer - 216 numbers - cost ~1.0 ms of a 15 ms training step (DESIGN.md 2.6).
+// channel 15 of 16 rows are padding, and this layer - 216 numbers - cost ~1.0 ms of a 15 ms training step.
 // It is 216 dot products over the whole volume, 27 FMAs per (voxel, channel): vector-ALU work.  Here a thread owns four
 // x-consecutive voxels of a 4 x 8 x 32 tile and the 54 accumulators of TWO input channels (blockIdx.y picks the channel pair:
 // all 216 in one thread spilled, and at <= 128 registers four workgroups share a CU and hide each other's load latency -

@@ -1,7 +1,8 @@
 """Tensor-level wrappers over the C ABI (include/casmvs.h): torch is used only for device memory
 and the current HIP stream; every op below is one call into libcasmvs_hip.so.
 
-All inputs must be float32 tensors on a ROCm device ("cuda" in torch); nothing here runs on CPU.
+All inputs must be float32 tensors on a ROCm device ("cuda" in torch) - layer_norm, layer_norm_backward and pack8 take float16 and bfloat16 ones too -; nothing
+here runs on CPU.
 """
 import ctypes
 import functools
