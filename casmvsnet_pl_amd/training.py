@@ -882,11 +882,12 @@ def train_steps(model, batches, optimizer, device="cuda", loss="sl1"):
     from .pipeline import DevicePrefetcher
     model.train()
     loss_of = sl1_loss if loss == "sl1" else cross_entropy_loss
-    returned = model.return_cost if loss == "cross_entropy" else None   # (as it was, afterwards)
+    net = model.module if isinstance(model, (torch.nn.parallel.DistributedDataParallel, torch.nn.DataParallel)) else model
+    returned = net.return_cost if loss == "cross_entropy" else None   # (as it was, afterwards)
     losses = []
     try:
         if loss == "cross_entropy":
-            model.return_cost = True
+            net.return_cost = True
         for b in DevicePrefetcher(batches, device, depth=2):
             depths = {k: torch.stack([d[k] for d in b["depths"]]).to(device) for k in b["depths"][0]}
             masks = {k: torch.stack([m[k] for m in b["masks"]]).to(device) for k in b["masks"][0]}
@@ -899,5 +900,5 @@ def train_steps(model, batches, optimizer, device="cuda", loss="sl1"):
             losses.append(float(value.detach()))
     finally:
         if loss == "cross_entropy":
-            model.return_cost = returned
+            net.return_cost = returned
     return losses

@@ -229,3 +229,21 @@ def test_abn8_gradients_of_the_affine_alone(dev, shape):   # noqa: F811
     _, *want = torch.autograd.grad(T.abn_train(norm, xr, checkpoint="8bit"), (xr, norm.weight, norm.bias), gy)
     got = torch.autograd.grad(T.abn_train(norm, x, checkpoint="8bit"), (norm.weight, norm.bias), gy)
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_train_steps_of_a_wrapped_model_with_the_cross_entropy_loss(dev):   # noqa: F811
+    """The switch is the model's, not its data-parallel wrapper's: the same losses either way, and the switch as it was afterwards."""
+    from casmvsnet_pl_amd.synthetic import make_inputs, randomize_state_dict
+    imgs, proj, dmin, dint = make_inputs(1, 3, 64, 96, seed=0)
+    g = torch.Generator().manual_seed(0)
+    depths = {f"level_{l}": dmin + 100 * torch.rand((64 >> l, 96 >> l), generator=g) for l in range(3)}
+    masks = {f"level_{l}": torch.rand((64 >> l, 96 >> l), generator=g) < 0.8 for l in range(3)}
+    batch = {"imgs": imgs, "proj_mats": proj, "init_depth_min": dmin, "depth_interval": dint, "depths": [depths], "masks": [masks]}
+    losses = []
+    for wrap in (lambda m: m, lambda m: torch.nn.DataParallel(m, device_ids=[0])):
+        model = M.CascadeMVSNet(num_groups=1, norm_act=M.LayerNormAct)
+        randomize_state_dict(model.state_dict(), seed=0)
+        wrapped = wrap(model.to(dev))
+        losses.append(T.train_steps(wrapped, [batch], torch.optim.SGD(model.parameters(), lr=1e-4), dev, loss="cross_entropy"))
+        assert model.return_cost is False
+    assert losses[0] == losses[1] and losses[0][0] > 0
