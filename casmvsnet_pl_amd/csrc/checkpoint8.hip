@@ -280,7 +280,7 @@ __device__ __forceinline__ void apply_blocks(const float *__restrict__ xp, float
       h[i] = i < left ? ((double)v[k][i] - c.mean) * c.rstd : 0.0;
       const bool above = fma(h[i], (double)c.gamma, (double)c.beta) > 0.0;
       up |= (above ? 1u : 0u) << i;
-      // (z rounded from 64 bits instead: 60.2 -> 62.9 us at 2 x 8 x 32 x 256 x 320, 7.7 -> 8.6 at 2 x 32 x 30720)
+      // (z rounded from 64 bits instead: 60.2 -> 62.9 us at 2 x 8 x 32 x 256 x 320, 7.7 -> 8.6 at 2 x 32 x 24 x 32 x 40)
       const float t = fmaf((v[k][i] - c.high) - c.low, c.scale, c.beta);
       o[i] = above ? t : t * slope;
     }

@@ -222,11 +222,11 @@ int main(int argc, char **argv) {
       far_check(2, 3, 70, offset, kShifted);
       far_check(2, 2, 64, offset, kShifted);
     }
-    far_check(1, 2, 16500, 3e6f, kShifted);   // (two launches)
+    far_check(1, 1, 16500, 3e6f, kShifted);   // (two launches)
     far_check(1, 1, 16501, -1e5f, kShifted);
     for (Channels kind : {kFirstApart, kConstant}) {
       far_check(2, 3, 70, 1e6f, kind);
-      far_check(1, 2, 16500, 1e4f, kind);
+      if (kind == kConstant) far_check(1, 1, 16500, 1e4f, kind);
     }
   } else if (part == "masked") {
     for (bool per_pixel : {true, false}) {
